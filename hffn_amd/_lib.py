@@ -10,7 +10,7 @@ import ctypes
 from pathlib import Path
 
 LIBRARY = Path(__file__).resolve().with_name("libhffn_amd.so")
-ABI_VERSION = 20
+ABI_VERSION = 21
 
 OK = 0
 VALUE_F32, VALUE_BF16 = 0, 1
@@ -18,6 +18,7 @@ UP_MODES = {"edges": 1, "rows": 2, "mfma": 3}
 DOWN_MODES = {"edges": 1, "rows": 2, "mfma": 3}
 
 _P, _I, _U32, _U64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_uint32, ctypes.c_uint64
+_I64, _F32, _F64 = ctypes.c_int64, ctypes.c_float, ctypes.c_double
 
 # name -> argument types (return type int for every entry but hffn_last_error)
 SIGNATURES = {
@@ -49,6 +50,15 @@ SIGNATURES = {
     "hffn_backward_planes": [_P] * 13 + [_U64] + [_P] * 3 + [_U32] * 6 + [_P],
     "hffn_backward_prepare": [_P] * 8 + [_U32] * 5 + [_P],
     "hffn_gather_values": [_P, _P, _P, _U32, _P],
+    "hffn_residual_norm": [_I] + [_P, _U64] * 2 + [_P] * 5 + [_F32] * 2 + [_I, _P, _P, _U32, _U32, _P],
+    "hffn_residual_norm_backward_workspace": [_U32, _U32, ctypes.POINTER(_U64)],
+    "hffn_residual_norm_backward": [_I] + [_P, _U64] * 4 + [_P] * 4 + [_F32] * 2 + [_I] + [_P] * 8 + [_U64, _U32, _U32, _P],
+    "hffn_clip_workspace": [_U32, ctypes.POINTER(_U64)],
+    "hffn_grad_norm": [_U32, _P, _P, _P, _I, _P, _U64, _P, _P],
+    "hffn_clip": [_U32] + [_P] * 5 + [_I, _F64, _P, _U64, _P, _P],
+    "hffn_loss_workspace": [_I, _U32, _U32, _U32, _I, _I, ctypes.POINTER(_U64)],
+    "hffn_losses": [_I, _P, _U64, _P, _P, _I64, _I, _I64, _P, _P, _U64, _U32, _U32, _U32, _P],
+    "hffn_loss_step": [_I, _P, _U64, _P, _P, _I64, _I, _I64, _I, _F32] + [_P] * 4 + [_U64, _U32, _U32, _U32, _P],
     "hffn_read_probe": [_P, _U64, _P, _U32, _U32, _P],
     "hffn_output_major_workspace": [_U32, _U32, ctypes.POINTER(_U64)],
     "hffn_output_major": [_I, _P, _P, _P, _U32, _U32, _U32, _P, _P, _P, _P, _U64, _P],

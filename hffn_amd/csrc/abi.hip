@@ -5,10 +5,12 @@
 
 #include <cstdarg>
 #include <cstdio>
+#include <exception>
 #include <initializer_list>
 #include <mutex>
 #include <string>
 #include <unordered_map>
+#include <vector>
 
 #include "../../include/hffn_amd.h"
 #include "launch.hpp"
@@ -962,6 +964,185 @@ int hffn_backward_prepare(const float* gy, float* gy_t, const float* out_val, co
     return launched(hffn::launch_backward_prepare(gy, gy_t, n, d_model, ld, out_val, hid_pos, hid_val, nnz_down, up_val, in_pos, in_val, nnz_up,
                                                   static_cast<hipStream_t>(stream)),
                     "backward_prepare");
+}
+
+namespace {
+// The widths and counts of a norm call, its strides (entries of a row) and its parameters' kinds.
+int check_norm(int value_type, uint32_t n, uint32_t d, std::initializer_list<uint64_t> strides, int layer, bool biases, float eps, const char* what) {
+    if (!valid_value_type(value_type)) return fail(HFFN_ERROR_ARGUMENT, "%s: unknown value type %d", what, value_type);
+    if (n == 0 || n > HFFN_MAX_TOKENS) return fail(HFFN_ERROR_ARGUMENT, "%s: n=%u: unsupported token count", what, n);
+    if (d == 0 || d > HFFN_MAX_NORM_WIDTH) return fail(HFFN_ERROR_ARGUMENT, "%s: d_model=%u: must be in [1, %u]", what, d, HFFN_MAX_NORM_WIDTH);
+    for (uint64_t stride : strides)
+        if (stride < d) return fail(HFFN_ERROR_ARGUMENT, "%s: row stride %llu smaller than d_model=%u", what, static_cast<unsigned long long>(stride), d);
+    if (layer != 0 && layer != 1) return fail(HFFN_ERROR_ARGUMENT, "%s: layer must be 0 or 1, not %d", what, layer);
+    if (!layer && biases) return fail(HFFN_ERROR_ARGUMENT, "%s: an RMS norm has no bias", what);
+    if (!(eps >= 0.0f)) return fail(HFFN_ERROR_ARGUMENT, "%s: eps must not be negative", what);
+    return HFFN_OK;
+}
+
+// Pointers aligned to an entry of their type: float32 parameters, rows of the value type.
+int check_entries(int value_type, std::initializer_list<const void*> rows, std::initializer_list<const void*> floats, const char* what) {
+    for (const void* p : rows)
+        if (reinterpret_cast<uintptr_t>(p) % (value_type == HFFN_VALUE_BF16 ? 2 : 4) != 0) return fail(HFFN_ERROR_ARGUMENT, "%s: misaligned rows", what);
+    for (const void* p : floats)
+        if (reinterpret_cast<uintptr_t>(p) % 4 != 0) return fail(HFFN_ERROR_ARGUMENT, "%s: misaligned float32 array", what);
+    return HFFN_OK;
+}
+}  // namespace
+
+int hffn_residual_norm(int value_type, const void* x, uint64_t x_stride, const void* f, uint64_t f_stride, const float* weight, const float* bias,
+                       const float* gate, const float* post_weight, const float* post_bias, float scale, float eps, int layer, void* r,
+                       void* h, uint32_t d_model, uint32_t n, void* stream) {
+    const char* what = "residual_norm";
+    if (int status = check_norm(value_type, n, d_model, {x_stride, f ? f_stride : d_model}, layer, bias || post_bias, eps, what)) return status;
+    if (!x || !weight || !h || (f && !r)) return fail(HFFN_ERROR_ARGUMENT, "%s: null pointer", what);
+    if (!f && (gate || post_weight)) return fail(HFFN_ERROR_ARGUMENT, "%s: a gate or a post norm without f", what);
+    if (post_bias && !post_weight) return fail(HFFN_ERROR_ARGUMENT, "%s: post_bias without post_weight", what);
+    if (int status = check_entries(value_type, {x, f, r, h}, {weight, bias, gate, post_weight, post_bias}, what)) return status;
+    const hffn::NormForward call{x, f, weight, bias, gate, post_weight, post_bias, r, h, x_stride, f ? f_stride : 0, n, d_model, scale, eps, layer != 0};
+    return launched(hffn::launch_residual_norm(value_type, call, static_cast<hipStream_t>(stream)), what);
+}
+
+int hffn_residual_norm_backward_workspace(uint32_t n, uint32_t d_model, uint64_t* bytes) {
+    if (!bytes) return fail(HFFN_ERROR_ARGUMENT, "residual_norm_backward_workspace: null pointer");
+    if (int status = check_norm(HFFN_VALUE_F32, n, d_model, {}, 0, false, 0.0f, "residual_norm_backward_workspace")) return status;
+    *bytes = static_cast<uint64_t>(hffn::kNormGrads) * hffn::norm_back_blocks(n, d_model) * d_model * sizeof(float);
+    return HFFN_OK;
+}
+
+int hffn_residual_norm_backward(int value_type, const void* r, uint64_t r_stride, const void* f, uint64_t f_stride, const void* gr,
+                                uint64_t gr_stride, const void* gh, uint64_t gh_stride, const float* weight, const float* gate,
+                                const float* post_weight, const float* post_bias, float scale, float eps, int layer, void* gx, void* gf,
+                                float* g_weight, float* g_bias, float* g_gate, float* g_post_weight, float* g_post_bias, void* workspace,
+                                uint64_t workspace_bytes, uint32_t d_model, uint32_t n, void* stream) {
+    const char* what = "residual_norm_backward";
+    if (int status = check_norm(value_type, n, d_model, {r_stride, f ? f_stride : d_model, gr ? gr_stride : d_model, gh_stride}, layer,
+                                post_bias || g_bias || g_post_bias, eps, what))
+        return status;
+    if (!r || !gh || !weight || !gx || !g_weight || !workspace) return fail(HFFN_ERROR_ARGUMENT, "%s: null pointer", what);
+    if ((gate || post_weight) && (!f || !gf)) return fail(HFFN_ERROR_ARGUMENT, "%s: a gate or a post norm without f and gf", what);
+    if ((gate != nullptr) != (g_gate != nullptr) || (post_weight != nullptr) != (g_post_weight != nullptr) ||
+        (post_bias != nullptr) != (g_post_bias != nullptr) || (post_bias && !post_weight))
+        return fail(HFFN_ERROR_ARGUMENT, "%s: gate, post_weight and post_bias come with their gradients", what);
+    if (int status = check_entries(value_type, {r, f, gr, gh, gx, gf},
+                                   {weight, gate, post_weight, post_bias, g_weight, g_bias, g_gate, g_post_weight, g_post_bias, workspace}, what))
+        return status;
+    uint64_t needed = 0;
+    if (int status = hffn_residual_norm_backward_workspace(n, d_model, &needed)) return status;
+    if (workspace_bytes < needed)
+        return fail(HFFN_ERROR_ARGUMENT, "%s: workspace of %llu bytes, %llu needed", what, static_cast<unsigned long long>(workspace_bytes),
+                    static_cast<unsigned long long>(needed));
+    const hffn::NormBackward call{r, f, gr, gh, weight, gate, post_weight, post_bias, gx, gf, static_cast<float*>(workspace), r_stride,
+                                  f ? f_stride : 0, gr ? gr_stride : 0, gh_stride, n, d_model, scale, eps, layer != 0};
+    const hffn::NormGradients grads{{g_weight, g_bias, g_gate, g_post_weight, g_post_bias}};
+    return launched(hffn::launch_residual_norm_backward(value_type, call, grads, static_cast<hipStream_t>(stream)), what);
+}
+
+int hffn_clip_workspace(uint32_t arrays, uint64_t* bytes) {
+    if (!bytes) return fail(HFFN_ERROR_ARGUMENT, "clip_workspace: null pointer");
+    *bytes = hffn::clip_workspace_bytes(arrays);
+    return HFFN_OK;
+}
+
+namespace {
+int clip_arrays(uint32_t arrays, const void* const* p, void* const* out, const uint64_t* counts, const int* types, const int* out_types,
+                const void* workspace, uint64_t workspace_bytes, const float* norm, std::vector<hffn::ClipArray>& list, const char* what) {
+    if (!norm || !workspace || (arrays && (!p || !counts || !types))) return fail(HFFN_ERROR_ARGUMENT, "%s: null pointer", what);
+    if (reinterpret_cast<uintptr_t>(workspace) % 8 != 0) return fail(HFFN_ERROR_ARGUMENT, "%s: the workspace must be 8-byte aligned", what);
+    if (workspace_bytes < hffn::clip_workspace_bytes(arrays))
+        return fail(HFFN_ERROR_ARGUMENT, "%s: workspace of %llu bytes, %llu needed", what, static_cast<unsigned long long>(workspace_bytes),
+                    static_cast<unsigned long long>(hffn::clip_workspace_bytes(arrays)));
+    list.reserve(arrays);
+    for (uint32_t k = 0; k < arrays; ++k) {
+        const int to = out ? out_types[k] : types[k];
+        if (!valid_value_type(types[k]) || !valid_value_type(to)) return fail(HFFN_ERROR_ARGUMENT, "%s: array %u: unknown value type", what, k);
+        if (counts[k] > hffn::kMaxClipEntries) return fail(HFFN_ERROR_ARGUMENT, "%s: array %u has %llu entries", what, k, static_cast<unsigned long long>(counts[k]));
+        if (counts[k] == 0) continue;
+        if (!p[k] || (out && !out[k])) return fail(HFFN_ERROR_ARGUMENT, "%s: array %u: null pointer", what, k);
+        if (int status = check_entries(types[k], {p[k]}, {}, what)) return status;
+        if (out)
+            if (int status = check_entries(to, {out[k]}, {}, what)) return status;
+        list.push_back({p[k], out ? out[k] : const_cast<void*>(p[k]), counts[k], types[k], to});
+    }
+    return HFFN_OK;
+}
+}  // namespace
+
+int hffn_grad_norm(uint32_t arrays, const void* const* p, const uint64_t* counts, const int* types, int largest, void* workspace,
+                   uint64_t workspace_bytes, float* norm, void* stream) try {
+    std::vector<hffn::ClipArray> list;
+    if (int status = clip_arrays(arrays, p, nullptr, counts, types, nullptr, workspace, workspace_bytes, norm, list, "grad_norm")) return status;
+    return launched(hffn::launch_grad_norm(list.data(), static_cast<uint32_t>(list.size()), largest != 0, static_cast<double*>(workspace), norm,
+                                           static_cast<hipStream_t>(stream)),
+                    "grad_norm");
+} catch (const std::exception& error) {
+    return fail(HFFN_ERROR_ARGUMENT, "grad_norm: %s", error.what());
+}
+
+int hffn_clip(uint32_t arrays, void* const* p, void* const* out, const uint64_t* counts, const int* types, const int* out_types, int largest,
+              double limit, void* workspace, uint64_t workspace_bytes, float* norm, void* stream) try {
+    if (!(limit >= 0.0)) return fail(HFFN_ERROR_ARGUMENT, "clip: the limit must not be negative");
+    if (out && !out_types) return fail(HFFN_ERROR_ARGUMENT, "clip: null pointer");
+    std::vector<hffn::ClipArray> list;
+    if (int status = clip_arrays(arrays, const_cast<const void* const*>(p), out, counts, types, out_types, workspace, workspace_bytes, norm, list, "clip"))
+        return status;
+    return launched(hffn::launch_clip(list.data(), static_cast<uint32_t>(list.size()), largest != 0, limit, out == nullptr,
+                                      static_cast<double*>(workspace), norm, static_cast<hipStream_t>(stream)),
+                    "clip");
+} catch (const std::exception& error) {
+    return fail(HFFN_ERROR_ARGUMENT, "clip: %s", error.what());
+}
+
+namespace {
+int check_loss(int value_type, uint32_t n, uint32_t d, uint32_t vocab, const char* what) {
+    if (!valid_value_type(value_type)) return fail(HFFN_ERROR_ARGUMENT, "%s: unknown value type %d", what, value_type);
+    if (n == 0 || n > HFFN_MAX_TOKENS) return fail(HFFN_ERROR_ARGUMENT, "%s: n=%u: unsupported token count", what, n);
+    if (d == 0 || d > HFFN_MAX_WIDTH) return fail(HFFN_ERROR_ARGUMENT, "%s: d_model=%u: must be in [1, %u]", what, d, HFFN_MAX_WIDTH);
+    if (vocab == 0 || vocab > HFFN_MAX_VOCAB) return fail(HFFN_ERROR_ARGUMENT, "%s: vocab=%u: must be in [1, %u]", what, vocab, HFFN_MAX_VOCAB);
+    return HFFN_OK;
+}
+int loss_call(hffn::LossCall& call, uint64_t workspace_bytes, int label_bytes, const char* what) {
+    if (int status = check_loss(call.value_type, call.n, call.d, call.vocab, what)) return status;
+    if (!call.x || !call.weight || !call.labels || !call.workspace) return fail(HFFN_ERROR_ARGUMENT, "%s: null pointer", what);
+    if (call.x_stride < call.d) return fail(HFFN_ERROR_ARGUMENT, "%s: row stride %llu smaller than d_model=%u", what, static_cast<unsigned long long>(call.x_stride), call.d);
+    if (label_bytes != 4 && label_bytes != 8) return fail(HFFN_ERROR_ARGUMENT, "%s: labels of 4 or 8 bytes, not %d", what, label_bytes);
+    if (reinterpret_cast<uintptr_t>(call.labels) % label_bytes != 0) return fail(HFFN_ERROR_ARGUMENT, "%s: misaligned labels", what);
+    if (int status = check_entries(call.value_type, {call.x, call.weight, call.gx, call.gw}, {call.losses, call.loss}, what)) return status;
+    if (reinterpret_cast<uintptr_t>(call.workspace) % 256 != 0) return fail(HFFN_ERROR_ARGUMENT, "%s: the workspace must be 256-byte aligned", what);
+    const uint64_t needed = hffn::loss_workspace_bytes(call.value_type, call.n, call.d, call.vocab, reinterpret_cast<uintptr_t>(call.weight) % 16 == 0, call.gw != nullptr);
+    if (workspace_bytes < needed)
+        return fail(HFFN_ERROR_ARGUMENT, "%s: workspace of %llu bytes, %llu needed", what, static_cast<unsigned long long>(workspace_bytes),
+                    static_cast<unsigned long long>(needed));
+    call.wide_labels = label_bytes == 8;
+    return HFFN_OK;
+}
+}  // namespace
+
+int hffn_loss_workspace(int value_type, uint32_t n, uint32_t d_model, uint32_t vocab, int aligned, int gradients, uint64_t* bytes) {
+    if (!bytes) return fail(HFFN_ERROR_ARGUMENT, "loss_workspace: null pointer");
+    if (int status = check_loss(value_type, n, d_model, vocab, "loss_workspace")) return status;
+    *bytes = hffn::loss_workspace_bytes(value_type, n, d_model, vocab, aligned != 0, gradients != 0);
+    return HFFN_OK;
+}
+
+int hffn_losses(int value_type, const void* x, uint64_t x_stride, const void* weight, const void* labels, int64_t labels_stride, int label_bytes,
+                int64_t ignore_index, float* losses, void* workspace, uint64_t workspace_bytes, uint32_t d_model, uint32_t vocab, uint32_t n,
+                void* stream) {
+    if (!losses) return fail(HFFN_ERROR_ARGUMENT, "losses: null pointer");
+    hffn::LossCall call{x, weight, labels, x_stride, labels_stride, ignore_index, false, false, 1.0f, losses, nullptr, nullptr, nullptr, workspace,
+                        value_type, n, d_model, vocab};
+    if (int status = loss_call(call, workspace_bytes, label_bytes, "losses")) return status;
+    return launched(hffn::launch_loss(call, static_cast<hipStream_t>(stream)), "losses");
+}
+
+int hffn_loss_step(int value_type, const void* x, uint64_t x_stride, const void* weight, const void* labels, int64_t labels_stride, int label_bytes,
+                   int64_t ignore_index, int mean, float scale, float* loss, void* gx, void* gw, void* workspace, uint64_t workspace_bytes,
+                   uint32_t d_model, uint32_t vocab, uint32_t n, void* stream) {
+    if (!loss || !gx || !gw) return fail(HFFN_ERROR_ARGUMENT, "loss_step: null pointer");
+    hffn::LossCall call{x, weight, labels, x_stride, labels_stride, ignore_index, false, mean != 0, scale, nullptr, loss, gx, gw, workspace,
+                        value_type, n, d_model, vocab};
+    if (int status = loss_call(call, workspace_bytes, label_bytes, "loss_step")) return status;
+    return launched(hffn::launch_loss(call, static_cast<hipStream_t>(stream)), "loss_step");
 }
 
 int hffn_read_probe(const void* data, uint64_t bytes, uint32_t* sink, uint32_t sink_words, uint32_t blocks, void* stream) {

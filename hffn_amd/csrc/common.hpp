@@ -81,6 +81,14 @@ __device__ __forceinline__ float gelu_grad(float z) {
 __device__ __forceinline__ float widen(float v) { return v; }
 __device__ __forceinline__ float widen(uint16_t v) { return __uint_as_float(static_cast<uint32_t>(v) << 16); }
 
+// bfloat16 bits of a float32, to the nearest (ties to even); a pair of them, the first in the low half.
+__device__ __forceinline__ uint16_t bf16_bits(float v) { return __builtin_bit_cast(uint16_t, static_cast<__bf16>(v)); }
+__device__ __forceinline__ uint32_t bf16_pair(float low, float high) {
+    typedef float Floats __attribute__((ext_vector_type(2)));
+    typedef __bf16 Halves __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((Floats{low, high}), Halves));
+}
+
 // Sum over the 64 lanes of a wave; every lane receives the same total (fixed xor-butterfly order, 32 first, so the
 // result does not depend on scheduling). On the vector unit's lane paths rather than six dependent permutes through LDS:
 // halves and rows swapped (v + v is the two halves' sum in every lane), then, as lanes 8 (4) apart hold equal sums, the

@@ -6,6 +6,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <initializer_list>
+
 namespace hffn {
 
 enum ValueType : int { kF32 = 0, kBF16 = 1 };
@@ -220,6 +222,76 @@ hipError_t launch_tiles_build(int vt, const int32_t* offsets, const int16_t* idx
 hipError_t launch_tiles_forward(int vt, const float* x, const void* up_store, const int32_t* up_table, const float* b_up,
                                 const void* down_store, const int32_t* down_table, const float* b_down, float* act, float* work,
                                 float* y, uint32_t d, uint32_t h, uint64_t nnz_up, uint64_t nnz_down, uint32_t n, hipStream_t stream);
+
+// The boundary between two blocks (norm.hip): u = post_norm(f) or f, r = x + scale gate u, h = norm(r); rows of d entries
+// of the value type with row strides in entries, parameters float32 [d] (null: none; post_weight null: no post norm;
+// layer: layer norms, else RMS norms and no biases). f null: h = norm(x), r not written.
+constexpr uint32_t kMaxNormWidth = 16384;
+struct NormForward {
+    const void *x, *f;
+    const float *weight, *bias, *gate, *post_weight, *post_bias;
+    void *r, *h;
+    uint64_t x_stride, f_stride;
+    uint32_t n, d;
+    float scale, eps;
+    bool layer;
+};
+hipError_t launch_residual_norm(int vt, const NormForward& call, hipStream_t stream);
+// gx = gr + the gradient of r through h; gf that of f; the parameters' gradients (null where not wanted) in the order
+// weight, bias, gate, post_weight, post_bias, summed over the rows by way of partials [kNormGrads][norm_back_blocks][d].
+// gr null: none; gf null: not written (then f may be null).
+constexpr int kNormGrads = 5;
+struct NormBackward {
+    const void *r, *f, *gr, *gh;
+    const float *weight, *gate, *post_weight, *post_bias;
+    void *gx, *gf;
+    float* partials;
+    uint64_t r_stride, f_stride, gr_stride, gh_stride;
+    uint32_t n, d;
+    float scale, eps;
+    bool layer;
+};
+struct NormGradients {
+    float* grad[kNormGrads];
+};
+uint32_t norm_back_blocks(uint32_t n, uint32_t d);
+hipError_t launch_residual_norm_backward(int vt, const NormBackward& call, const NormGradients& grads, hipStream_t stream);
+
+// The norm over many tensors and their scaling (clip.hip). An array is `count` entries of the value type at p (aligned to
+// an entry); out: where the scaled entries go (p itself for in place), of out_type. norm = the 2-norm or the largest
+// magnitude over all arrays, float32; factor = min(1, limit / (norm + 1e-6)).
+constexpr uint32_t kClipPartials = 1024;  // float64 partials per launch
+constexpr uint32_t kClipArrays = 96;      // arrays per launch
+constexpr uint64_t kMaxClipEntries = 1ull << 38;  // of one array
+struct ClipArray {
+    const void* p;
+    void* out;
+    uint64_t count;
+    int type, out_type;
+};
+uint64_t clip_workspace_bytes(uint32_t arrays);
+hipError_t launch_grad_norm(const ClipArray* arrays, uint32_t count, bool largest, double* partials, float* norm, hipStream_t stream);
+hipError_t launch_clip(const ClipArray* arrays, uint32_t count, bool largest, double limit, bool in_place, double* partials, float* norm,
+                       hipStream_t stream);
+
+// Softmax cross entropy of a head (loss.hip): x [n, d] (rows x_stride entries apart) and weight [vocab, d] of the value type,
+// labels int32 or (wide) int64, labels_stride entries apart; tokens whose label is `ignore` do not count. losses (null:
+// not wanted) [n]; with gw not null also loss [1], gx [n, d], gw [vocab, d] of the value type: the gradients of scale times
+// the mean (or sum) of the counted losses. The workspace (loss_workspace_bytes, 256-byte aligned) may hold anything;
+// `aligned`: the weight starts on a 16-byte boundary.
+struct LossCall {
+    const void *x, *weight, *labels;
+    uint64_t x_stride;
+    int64_t labels_stride, ignore;
+    bool wide_labels, mean;
+    float scale;
+    float *losses, *loss;
+    void *gx, *gw, *workspace;
+    int value_type;
+    uint32_t n, d, vocab;
+};
+uint64_t loss_workspace_bytes(int vt, uint32_t n, uint32_t d, uint32_t vocab, bool aligned, bool gradients);
+hipError_t launch_loss(const LossCall& call, hipStream_t stream);
 
 // probe.hip
 hipError_t launch_read_probe(const void* data, uint64_t bytes, uint32_t* sink, uint32_t blocks, hipStream_t stream);

@@ -27,7 +27,7 @@
 extern "C" {
 #endif
 
-#define HFFN_ABI_VERSION 20
+#define HFFN_ABI_VERSION 21
 
 #define HFFN_OK 0
 #define HFFN_ERROR_ARGUMENT (-1) /* invalid shape, mode, pointer or workspace */
@@ -398,6 +398,55 @@ int hffn_adamw_arrays(uint32_t arrays, float* const* p, const float* const* g, f
 /* dst[j] = src[pos[j]]: the values of a transposed support refreshed from the compact array they index (the
  * reference reads them through the positions inside its kernels, kernels_train.py:142-150, 204-215). */
 int hffn_gather_values(const float* src, const int32_t* pos, float* dst, uint32_t count, void* stream);
+
+/* The boundary between two blocks of a residual stack: u = post_norm(f), or f where post_weight is NULL;
+ * r = x + scale gate u (gate NULL: ones); h = norm(r). Rows of d_model entries of the value type, x and f with row strides
+ * in entries, r and h contiguous; parameters float32[d_model]. layer 1: (v - mean) / sqrt(var + eps) weight + bias (bias NULL:
+ * none); layer 0: v / sqrt(mean(v^2) + eps) weight. f NULL (with gate and post_weight): h = norm(x), r is not written. Row
+ * sums in float32; h is taken from r before r is rounded to the value type. x, f may be any rows, r and h others. */
+#define HFFN_MAX_NORM_WIDTH 16384u
+int hffn_residual_norm(int value_type, const void* x, uint64_t x_stride, const void* f, uint64_t f_stride, const float* weight,
+                       const float* bias, const float* gate, const float* post_weight, const float* post_bias, float scale, float eps,
+                       int layer, void* r, void* h, uint32_t d_model, uint32_t n, void* stream);
+
+/* Its backward from r and f as the forward stored and read them: gx = gr + the gradient of r through h for gh (gr NULL:
+ * none), the gradient of x; gf that of f (NULL: not wanted; needed with a gate or a post norm); float32[d_model] gradients
+ * of the parameters, each summed over the rows in a fixed order (g_bias NULL: none; g_gate, g_post_weight and g_post_bias come
+ * with gate, post_weight and post_bias). Workspace: hffn_residual_norm_backward_workspace bytes, any content. */
+int hffn_residual_norm_backward_workspace(uint32_t n, uint32_t d_model, uint64_t* bytes);
+int hffn_residual_norm_backward(int value_type, const void* r, uint64_t r_stride, const void* f, uint64_t f_stride, const void* gr,
+                                uint64_t gr_stride, const void* gh, uint64_t gh_stride, const float* weight, const float* gate,
+                                const float* post_weight, const float* post_bias, float scale, float eps, int layer, void* gx, void* gf,
+                                float* g_weight, float* g_bias, float* g_gate, float* g_post_weight, float* g_post_bias, void* workspace,
+                                uint64_t workspace_bytes, uint32_t d_model, uint32_t n, void* stream);
+
+/* The norm over all entries of `arrays` arrays (host arrays of device pointers, entry counts and value types; a pointer
+ * aligned to an entry, at most 2^38 entries each): the 2-norm, or the largest magnitude (largest 1), in float64 and rounded
+ * to *norm (a device float32). hffn_clip then scales every entry by min(1, limit / (norm + 1e-6)), in place (out NULL; with a
+ * factor of one nothing is written) or into out[k] of out_types[k] (host arrays; apart from every p). A NaN norm makes
+ * every scaled entry NaN. No two arrays may overlap. Workspace: hffn_clip_workspace bytes, any content, 8-byte aligned. */
+int hffn_clip_workspace(uint32_t arrays, uint64_t* bytes);
+int hffn_grad_norm(uint32_t arrays, const void* const* p, const uint64_t* counts, const int* types, int largest, void* workspace,
+                   uint64_t workspace_bytes, float* norm, void* stream);
+int hffn_clip(uint32_t arrays, void* const* p, void* const* out, const uint64_t* counts, const int* types, const int* out_types,
+              int largest, double limit, void* workspace, uint64_t workspace_bytes, float* norm, void* stream);
+
+/* Softmax cross entropy of a language-model head: x [n, d_model] (row stride in entries) and weight [vocab, d_model]
+ * (contiguous) of the value type; labels (label_bytes 4 or 8, labels_stride entries apart) in [0, vocab) or ignore_index.
+ * losses[t] = log sum_v exp(x_t . w_v) - x_t . w_label, 0 for ignored tokens, NaN for a label outside the vocabulary.
+ * hffn_loss_step: *loss, the mean (mean 1; 0 where every token is ignored) or the sum of the counted losses, and the
+ * gradients of scale times it: gx [n, d_model] (zero rows for ignored tokens, whatever their x holds) and gw [vocab, d_model],
+ * of the value type; a label outside the vocabulary makes all of them NaN. Logits are computed in pieces of the vocabulary and
+ * not kept. Workspace: hffn_loss_workspace bytes (aligned: the weight starts on a 16-byte boundary; gradients: for
+ * hffn_loss_step), any content, 256-byte aligned. Outputs may not overlap inputs. */
+#define HFFN_MAX_VOCAB (1u << 24)
+int hffn_loss_workspace(int value_type, uint32_t n, uint32_t d_model, uint32_t vocab, int aligned, int gradients, uint64_t* bytes);
+int hffn_losses(int value_type, const void* x, uint64_t x_stride, const void* weight, const void* labels, int64_t labels_stride,
+                int label_bytes, int64_t ignore_index, float* losses, void* workspace, uint64_t workspace_bytes, uint32_t d_model,
+                uint32_t vocab, uint32_t n, void* stream);
+int hffn_loss_step(int value_type, const void* x, uint64_t x_stride, const void* weight, const void* labels, int64_t labels_stride,
+                   int label_bytes, int64_t ignore_index, int mean, float scale, float* loss, void* gx, void* gw, void* workspace,
+                   uint64_t workspace_bytes, uint32_t d_model, uint32_t vocab, uint32_t n, void* stream);
 
 /* Measurement only, no counterpart in the reference: a plain streaming read of `bytes` (a nonzero multiple of 16 from
  * a 16-byte aligned pointer) by `blocks` blocks of 4 waves, each wave one contiguous span, one word per wave written to
