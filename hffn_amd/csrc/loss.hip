@@ -7,8 +7,10 @@
 //
 // Every product is out[b][a] = sum_k A[a, k] B[b, k] on 16-bit MFMA operands with float32 sums. bfloat16 calls multiply
 // their entries as they are (D rounded to bfloat16: 2^-8 of an entry, as the gradients themselves are rounded). float32
-// calls hold every operand as fp16 hi + lo of the entry times a power of two of its tensor (the largest entry at
-// 2^12..2^13; 22 bits down to 2^-16 of it) and take hi hi + hi lo + lo hi.
+// calls hold every operand as fp16 hi + lo of the entry times a power of two of its tensor (22 bits down to 2^-12 of the
+// largest entry) and take hi hi + hi lo + lo hi.
+#include <type_traits>
+
 #include "common.hpp"
 #include "launch.hpp"
 
@@ -23,17 +25,17 @@ typedef _Float16 FragH __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) Quad* LdsQuad;
 typedef __attribute__((address_space(3))) const Frag* LdsFrag;
 
-constexpr uint32_t kThreads = 512, kWaves = kThreads / kWave;
-constexpr int kLift = 13;      // operands' largest entries lie below 2^kLift
+constexpr int kLift = 10;      // the entry an operand's power of two is taken from lies in [2^9, 2^10) ...
+constexpr int kRoom = 5;       // ... and its largest up to kRoom binades above
 constexpr int kGradLift = 14;  // |D| <= 1 is kept times 2^kGradLift
 constexpr int kChain = 4;      // k-tiles whose products are summed in the MFMA accumulators (float32 calls)
 
 // What the first launches leave for the others: counted tokens, labels outside the vocabulary, and (float32) the bits of
-// the largest finite magnitudes of the weight and of the counted rows of x.
+// the magnitudes that the powers of two are taken from, and of the samples they were first taken from.
 struct Meta {
-    uint32_t valid, invalid, weight_bits, x_bits;
+    uint32_t valid, invalid, weight_bits, x_bits, weight_sample, x_sample;
 };
-__device__ __forceinline__ int lift_of(uint32_t bits) {  // e with 2^-e times the largest entry in [2^12, 2^13)
+__device__ __forceinline__ int lift_of(uint32_t bits) {  // e with 2^-e times that magnitude in [2^9, 2^10)
     return bits == 0 ? 0 : ilogbf(__uint_as_float(bits)) - (kLift - 1);
 }
 __device__ __forceinline__ float grad_factor(const Meta& meta, float scale, bool mean) {
@@ -51,21 +53,49 @@ __device__ __forceinline__ void split(float v, uint16_t& hi, uint16_t& lo) {
 
 // ------------------------------------------------------------------------------------------------ tokens and operands
 
-// The counted tokens in order: rows[i] the token of compact row i and labels[i] its label; place[t] the compact row of
-// token t or -1. A label outside the vocabulary counts as a token whose loss is NaN. One block.
-constexpr uint32_t kScanThreads = 1024;
-__global__ __launch_bounds__(kScanThreads) void loss_scan_kernel(const void* __restrict__ labels, int64_t stride, bool wide, int64_t ignore,
-                                                                 uint32_t n, uint32_t vocab, int32_t* __restrict__ rows,
-                                                                 int32_t* __restrict__ compact, int32_t* __restrict__ place,
-                                                                 float* __restrict__ losses, Meta* __restrict__ meta) {
+__device__ __forceinline__ int64_t label_of(const void* labels, int64_t at, bool wide) {
+    return wide ? static_cast<const int64_t*>(labels)[at] : static_cast<const int32_t*>(labels)[at];
+}
+
+// What the preparing launches read and write: labels; the counted tokens in order (rows[i] the token of compact row i,
+// compact[i] its label or -1 where that lies outside the vocabulary, place[t] the compact row of token t or -1); the operand
+// rows of x's counted rows (zeros to the next multiple of 64) and, where it is not read in place, of the weight, as
+// [rows][width] bfloat16 or, per 32 entries, 32 hi and 32 lo halves; zeros from d on.
+struct Prepare {
+    const void *labels, *x, *weight;
+    int64_t labels_stride, ignore;
+    uint64_t x_stride;
+    bool wide;
+    uint32_t n, d, width, vocab;
+    int32_t *rows, *compact, *place;
+    float* losses;
+    Meta* meta;
+    uint16_t *x_out, *w_out;
+    uint32_t *x_most, *w_most;  // float32: largest finite magnitude of each block's rows, bits
+    uint32_t x_blocks, w_blocks;
+};
+
+// Calls of more tokens than kScanTokens: the counted tokens' order, one block. (Below that every block of the preparing
+// launch counts the labels itself: a launch less.)
+constexpr uint32_t kScanTokens = 4096, kScanThreads = 1024, kScanAhead = 8;
+__global__ __launch_bounds__(kScanThreads) void loss_scan_kernel(Prepare p) {
     __shared__ uint32_t counts[kScanThreads / kWave], bad[kScanThreads / kWave];
     const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     uint32_t base = 0, invalid = 0;
-    for (uint32_t first = 0; first < n; first += kScanThreads) {
-        const uint32_t t = first + threadIdx.x;
-        int64_t label = ignore;
-        if (t < n) label = wide ? static_cast<const int64_t*>(labels)[t * stride] : static_cast<const int32_t*>(labels)[t * stride];
-        const bool counted = t < n && label != ignore, outside = counted && (label < 0 || label >= static_cast<int64_t>(vocab));
+    int64_t ahead[kScanAhead];
+    for (uint32_t first = 0; first < p.n; first += kScanThreads) {
+        const uint32_t t = first + threadIdx.x, slot = first / kScanThreads % kScanAhead;
+        if (slot == 0) {
+#pragma unroll
+            for (uint32_t k = 0; k < kScanAhead; ++k) {
+                const uint32_t at = t + k * kScanThreads;
+                ahead[k] = at < p.n ? label_of(p.labels, at * p.labels_stride, p.wide) : p.ignore;
+            }
+        }
+        int64_t label = p.ignore;
+#pragma unroll
+        for (uint32_t k = 0; k < kScanAhead; ++k) label = slot == k ? ahead[k] : label;
+        const bool counted = t < p.n && label != p.ignore, outside = counted && (label < 0 || label >= static_cast<int64_t>(p.vocab));
         const uint64_t mask = __ballot(counted);
         if (lane == 0) counts[wave] = __popcll(mask);
         invalid += outside;
@@ -77,12 +107,12 @@ __global__ __launch_bounds__(kScanThreads) void loss_scan_kernel(const void* __r
         }
         at += __popcll(mask & ((uint64_t{1} << lane) - 1));
         if (counted) {
-            rows[at] = static_cast<int32_t>(t);
-            compact[at] = outside ? -1 : static_cast<int32_t>(label);
+            p.rows[at] = static_cast<int32_t>(t);
+            p.compact[at] = outside ? -1 : static_cast<int32_t>(label);
         }
-        if (t < n) {
-            place[t] = counted ? static_cast<int32_t>(at) : -1;
-            if (!counted) losses[t] = 0.0f;
+        if (t < p.n) {
+            p.place[t] = counted ? static_cast<int32_t>(at) : -1;
+            if (!counted) p.losses[t] = 0.0f;
         }
         base += total;
         __syncthreads();
@@ -92,73 +122,216 @@ __global__ __launch_bounds__(kScanThreads) void loss_scan_kernel(const void* __r
     __syncthreads();
     if (threadIdx.x == 0) {
         for (uint32_t w = 1; w < kScanThreads / kWave; ++w) invalid += bad[w];
-        *meta = {base, invalid, 0u, 0u};
+        p.meta->valid = base;
+        p.meta->invalid = invalid;
     }
 }
 
-// float32: the largest finite magnitudes of the weight and of x's counted rows (maxima: any order gives the same).
-__device__ __forceinline__ uint32_t magnitude(float v) {
+__device__ __forceinline__ uint32_t magnitude(float v) {  // bits of |v|, 0 for what is not finite
     const uint32_t bits = __float_as_uint(v) & 0x7fffffffu;
     return bits < 0x7f800000u ? bits : 0u;
 }
-constexpr uint32_t kRangeThreads = 256;
-__global__ __launch_bounds__(kRangeThreads) void loss_range_kernel(const float* __restrict__ weight, uint64_t entries, const float* __restrict__ x,
-                                                                  uint64_t x_stride, uint32_t d, const int32_t* __restrict__ rows,
-                                                                  Meta* __restrict__ meta, uint32_t weight_blocks) {
-    __shared__ uint32_t lds[kRangeThreads / kWave];
-    uint32_t most = 0;
-    const bool of_weight = blockIdx.x < weight_blocks;
-    if (of_weight) {
-        const uint64_t quads = reinterpret_cast<uintptr_t>(weight) % 16 == 0 ? entries / 4 : 0;
-        const uint64_t step = static_cast<uint64_t>(weight_blocks) * kRangeThreads, first = static_cast<uint64_t>(blockIdx.x) * kRangeThreads + threadIdx.x;
-#pragma unroll 4
-        for (uint64_t i = first; i < quads; i += step) {
-            const float4 v = reinterpret_cast<const float4*>(weight)[i];
-            most = max(max(most, max(magnitude(v.x), magnitude(v.y))), max(magnitude(v.z), magnitude(v.w)));
-        }
-        for (uint64_t i = 4 * quads + first; i < entries; i += step) most = max(most, magnitude(weight[i]));
-    } else {
-        const uint32_t valid = meta->valid;
-        for (uint32_t i = blockIdx.x - weight_blocks; i < valid; i += gridDim.x - weight_blocks)
-            for (uint32_t c = threadIdx.x; c < d; c += kRangeThreads) most = max(most, magnitude(x[rows[i] * x_stride + c]));
-    }
-    for (int step = 32; step > 0; step /= 2) most = max(most, static_cast<uint32_t>(__shfl_xor(most, step)));
-    if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = most;
+
+constexpr uint32_t kPrepThreads = 256, kPrepWaves = kPrepThreads / kWave, kWeightRows = 16;  // weight rows a block
+
+// The largest of the threads' values, in every thread (one barrier before and after: lds may be used again).
+__device__ __forceinline__ uint32_t block_most(uint32_t v, uint32_t (&lds)[kPrepWaves]) {
+    for (int step = 32; step > 0; step /= 2) v = max(v, static_cast<uint32_t>(__shfl_xor(v, step)));
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (uint32_t w = 1; w < kRangeThreads / kWave; ++w) most = max(most, lds[w]);
-        atomicMax(of_weight ? &meta->weight_bits : &meta->x_bits, most);
+    if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = v;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t w = 0; w < kPrepWaves; ++w) v = max(v, lds[w]);
+    return v;
+}
+
+// float32 calls take the powers of two from the largest of 1024 entries spread over a tensor, the same in every block, and
+// note each block's largest: only where some entry lies kRoom binades above is the tensor packed again, by its largest.
+// (A pass over the weight for its largest first took 60 us of a 1080 us step of 512 tokens of 1024 x 50304.)
+constexpr uint32_t kSamples = 4;  // per thread
+__device__ __forceinline__ uint32_t sample_of(const Prepare& p, bool of_x, uint32_t (&lds)[kPrepWaves]) {
+    uint32_t most = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < kSamples; ++k) {
+        const uint32_t i = k * kPrepThreads + threadIdx.x, column = i * 40503u % p.d, of = kSamples * kPrepThreads;
+        const uint64_t row = static_cast<uint64_t>(i) * (of_x ? p.n : p.vocab) / of;
+        if (of_x && label_of(p.labels, row * p.labels_stride, p.wide) == p.ignore) continue;
+        const float* from = of_x ? static_cast<const float*>(p.x) + row * p.x_stride : static_cast<const float*>(p.weight) + row * p.d;
+        most = max(most, magnitude(from[column]));
+    }
+    return block_most(most, lds);
+}
+
+// One operand row by a wave, eight entries a lane and step; returns the largest finite magnitude that the lane saw.
+template <typename T>
+__device__ __forceinline__ uint32_t pack_row(const T* __restrict__ from, uint16_t* __restrict__ to, uint32_t d, uint32_t width, int e) {
+    const uint32_t lane = threadIdx.x % kWave;
+    const bool whole = reinterpret_cast<uintptr_t>(from) % 16 == 0;
+    uint32_t most = 0;
+    for (uint32_t c = 8 * lane; c < width; c += 8 * kWave) {
+        if constexpr (sizeof(T) == 4) {
+            float v[8];
+            if (whole && c + 8 <= d) {
+                load_vec<8>(from + c, v);
+            } else {
+#pragma unroll
+                for (uint32_t k = 0; k < 8; ++k) v[k] = c + k < d ? from[c + k] : 0.0f;
+            }
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (uint32_t k = 0; k < 8; k += 2) {
+                uint16_t h[2], l[2];
+                most = max(most, max(magnitude(v[k]), magnitude(v[k + 1])));
+                split(ldexpf(v[k], -e), h[0], l[0]);
+                split(ldexpf(v[k + 1], -e), h[1], l[1]);
+                hi[k / 2] = h[0] | static_cast<uint32_t>(h[1]) << 16;
+                lo[k / 2] = l[0] | static_cast<uint32_t>(l[1]) << 16;
+            }
+            uint16_t* out = to + c / 32 * 64 + c % 32;
+            *reinterpret_cast<uint4*>(out) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            *reinterpret_cast<uint4*>(out + 32) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        } else {
+            uint4 v;
+            if (whole && c + 8 <= d) {
+                v = *reinterpret_cast<const uint4*>(from + c);
+            } else {
+                uint32_t words[4];
+#pragma unroll
+                for (uint32_t k = 0; k < 8; k += 2)
+                    words[k / 2] = (c + k < d ? from[c + k] : 0u) | (c + k + 1 < d ? static_cast<uint32_t>(from[c + k + 1]) : 0u) << 16;
+                v = make_uint4(words[0], words[1], words[2], words[3]);
+            }
+            *reinterpret_cast<uint4*>(to + c) = v;
+        }
+    }
+    return most;
+}
+
+// The weight's rows of block `block`; returns the thread's largest magnitude.
+template <typename T>
+__device__ __forceinline__ uint32_t pack_weight(const Prepare& p, uint32_t block, int e) {
+    constexpr uint64_t kParts = sizeof(T) == 4 ? 2 : 1;
+    uint32_t most = 0;
+    for (uint32_t r = threadIdx.x / kWave; r < kWeightRows; r += kPrepWaves) {
+        const uint64_t row = static_cast<uint64_t>(block) * kWeightRows + r;
+        if (row < p.vocab) most = max(most, pack_row(static_cast<const T*>(p.weight) + row * p.d, p.w_out + row * kParts * p.width, p.d, p.width, e));
+    }
+    return most;
+}
+
+// A block per kPrepWaves tokens (a wave each, and the compact row of the same number where zeros belong) and, after those,
+// one per kWeightRows weight rows to pack.
+template <typename T>
+__global__ __launch_bounds__(kPrepThreads) void loss_prepare_kernel(Prepare p) {
+    constexpr uint64_t kParts = sizeof(T) == 4 ? 2 : 1;
+    __shared__ uint32_t most_lds[kPrepWaves], sums[kPrepWaves][3];
+    const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    if (blockIdx.x >= p.x_blocks) {
+        const uint32_t block = blockIdx.x - p.x_blocks;
+        int e = 0;
+        if constexpr (sizeof(T) == 4) {
+            const uint32_t sample = sample_of(p, false, most_lds);
+            e = lift_of(sample);
+            if (block == 0 && threadIdx.x == 0) p.meta->weight_sample = sample;
+        }
+        const uint32_t most = pack_weight<T>(p, block, e);
+        if constexpr (sizeof(T) == 4) {
+            const uint32_t all = block_most(most, most_lds);
+            if (threadIdx.x == 0) p.w_most[block] = all;
+        }
+        return;
+    }
+    const uint32_t first = blockIdx.x * kPrepWaves, i = first + wave;
+    uint32_t valid, at = 0;
+    bool counted = false;
+    if (p.n > kScanTokens) {
+        valid = p.meta->valid;
+        const int32_t here = i < p.n ? p.place[i] : -1;
+        counted = here >= 0;
+        at = static_cast<uint32_t>(here);
+    } else {
+        uint32_t before = 0, all = 0, outside = 0;  // counted tokens before the block's, all, and those outside, of this wave
+        for (uint32_t t = threadIdx.x; t < (p.n + kWave - 1) / kWave * kWave; t += kPrepThreads) {
+            const int64_t label = t < p.n ? label_of(p.labels, t * p.labels_stride, p.wide) : p.ignore;
+            const bool is = t < p.n && label != p.ignore;
+            all += __popcll(__ballot(is));
+            before += __popcll(__ballot(is && t < first));
+            outside += __popcll(__ballot(is && (label < 0 || label >= static_cast<int64_t>(p.vocab))));
+        }
+        if (lane == 0) {
+            sums[wave][0] = before;
+            sums[wave][1] = all;
+            sums[wave][2] = outside;
+        }
+        __syncthreads();
+        at = valid = outside = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < kPrepWaves; ++w) {
+            at += sums[w][0];
+            valid += sums[w][1];
+            outside += sums[w][2];
+        }
+        for (uint32_t t = first; t <= i && t < p.n; ++t) {
+            const int64_t label = label_of(p.labels, t * p.labels_stride, p.wide);
+            counted = label != p.ignore;
+            if (t < i) {
+                at += counted;
+            } else if (lane == 0) {
+                p.place[t] = counted ? static_cast<int32_t>(at) : -1;
+                if (counted) {
+                    p.rows[at] = static_cast<int32_t>(t);
+                    p.compact[at] = label < 0 || label >= static_cast<int64_t>(p.vocab) ? -1 : static_cast<int32_t>(label);
+                } else {
+                    p.losses[t] = 0.0f;
+                }
+            }
+        }
+        counted = counted && i < p.n;
+        if (blockIdx.x == 0 && threadIdx.x == 0) {
+            p.meta->valid = valid;
+            p.meta->invalid = outside;
+        }
+    }
+    int e = 0;
+    if constexpr (sizeof(T) == 4) {
+        const uint32_t sample = sample_of(p, true, most_lds);
+        e = lift_of(sample);
+        if (blockIdx.x == 0 && threadIdx.x == 0) p.meta->x_sample = sample;
+    }
+    uint32_t most = 0;
+    if (counted) most = pack_row(static_cast<const T*>(p.x) + i * p.x_stride, p.x_out + at * kParts * p.width, p.d, p.width, e);
+    if (i >= valid && i < (valid + 63) / 64 * 64) {
+        uint4* out = reinterpret_cast<uint4*>(p.x_out + i * kParts * p.width);
+        for (uint32_t c = lane; c < kParts * p.width / 8; c += kWave) out[c] = make_uint4(0, 0, 0, 0);
+    }
+    if constexpr (sizeof(T) == 4) {
+        const uint32_t all = block_most(most, most_lds);
+        if (threadIdx.x == 0) p.x_most[blockIdx.x] = all;
     }
 }
 
-// Operand rows: x's counted rows (zeros to the next multiple of 64) and, where it is not read in place, the weight's, as
-// [rows][width] bfloat16 or, per 32 entries, 32 hi and 32 lo halves; zeros from d on. A wave per row.
-constexpr uint32_t kPackThreads = 256, kPackRows = kPackThreads / kWave;
-template <typename T>
-__global__ __launch_bounds__(kPackThreads) void loss_pack_kernel(const T* __restrict__ x, uint64_t x_stride, const T* __restrict__ weight, uint32_t vocab,
-                                                                uint32_t d, uint32_t width, const int32_t* __restrict__ rows,
-                                                                const Meta* __restrict__ meta, uint16_t* __restrict__ x_out,
-                                                                uint16_t* __restrict__ w_out, uint32_t x_blocks) {
-    const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    const bool of_x = blockIdx.x < x_blocks;
-    const uint32_t row = (of_x ? blockIdx.x : blockIdx.x - x_blocks) * kPackRows + wave;
-    const uint32_t valid = meta->valid;
-    if (of_x ? row >= (valid + 63) / 64 * 64 : row >= vocab) return;
-    const bool zero = of_x && row >= valid;
-    const T* from = of_x ? (zero ? x : x + rows[row] * x_stride) : weight + static_cast<uint64_t>(row) * d;
-    if constexpr (sizeof(T) == 4) {
-        const int e = lift_of(of_x ? meta->x_bits : meta->weight_bits);
-        uint16_t* to = (of_x ? x_out : w_out) + static_cast<uint64_t>(row) * 2 * width;
-        for (uint32_t c = lane; c < width; c += kWave) {
-            uint16_t hi, lo;
-            split(zero || c >= d ? 0.0f : ldexpf(from[c], -e), hi, lo);
-            to[c / 32 * 64 + c % 32] = hi;
-            to[c / 32 * 64 + 32 + c % 32] = lo;
-        }
-    } else {
-        uint16_t* to = (of_x ? x_out : w_out) + static_cast<uint64_t>(row) * width;
-        for (uint32_t c = lane; c < width; c += kWave) to[c] = zero || c >= d ? 0 : from[c];
+// float32: the powers of two that hold, from the blocks' largest magnitudes, and the operands packed again where the
+// sample's did not.
+__global__ __launch_bounds__(kPrepThreads) void loss_settle_kernel(Prepare p) {
+    __shared__ uint32_t lds[kPrepWaves];
+    const auto settled = [&](const uint32_t* most, uint32_t blocks, uint32_t sample) -> uint32_t {
+        uint32_t largest = 0;
+        for (uint32_t i = threadIdx.x; i < blocks; i += kPrepThreads) largest = max(largest, most[i]);
+        largest = block_most(largest, lds);
+        return largest == 0 || (sample != 0 && lift_of(largest) - lift_of(sample) <= kRoom) ? sample : largest;
+    };
+    const uint32_t x_sample = p.meta->x_sample, w_sample = p.meta->weight_sample, valid = p.meta->valid;
+    const uint32_t x_bits = settled(p.x_most, p.x_blocks, x_sample), w_bits = settled(p.w_most, p.w_blocks, w_sample);
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        p.meta->x_bits = x_bits;
+        p.meta->weight_bits = w_bits;
     }
+    if (x_bits != x_sample)
+        for (uint32_t i = blockIdx.x * kPrepWaves + threadIdx.x / kWave; i < valid; i += gridDim.x * kPrepWaves)
+            pack_row(static_cast<const float*>(p.x) + p.rows[i] * p.x_stride, p.x_out + static_cast<uint64_t>(i) * 2 * p.width, p.d, p.width,
+                     lift_of(x_bits));
+    if (w_bits != w_sample)
+        for (uint32_t block = blockIdx.x; block < p.w_blocks; block += gridDim.x) pack_weight<float>(p, block, lift_of(w_bits));
 }
 
 // --------------------------------------------------------------------------------------------------------- the product
@@ -170,27 +343,31 @@ __device__ __forceinline__ uint32_t permuted(uint32_t r) { return (r >> 2 & 1) *
 // An operand's tile in LDS, TILE indexes x 64 / PARTS k (128 bytes an index), 16-byte chunks swizzled so that the lanes of
 // a read touch every bank: index-major (memory rows are the operand's indexes, k contiguous; a row's 8 chunks) or k-major
 // (TR: memory rows are k, read through the LDS transpose reads). Transfers of 1 KB go straight from memory to LDS.
-template <int PARTS, bool TR, int TILE>
+template <int PARTS, bool TR, int TILE, int WAVES>
 struct Operand {
-    static constexpr uint32_t kBytes = TILE * 128, kPieces = kBytes / 1024, kPerWave = kPieces / kWaves;
+    static constexpr uint32_t kBytes = TILE * 128, kPieces = kBytes / 1024, kPerWave = kPieces / WAVES;
     static constexpr uint32_t kRow = TR ? TILE * 2 * PARTS : 128, kDepth = 64 / PARTS;
-    static_assert(kPieces % kWaves == 0, "every wave transfers as many pieces");
+    static_assert(kPieces % WAVES == 0, "every wave transfers as many pieces");
 
     const char* base;        // of the tile at k = 0 (index-major) or of its first column (k-major)
     uint64_t stride;         // bytes of a memory row
     uint32_t offset[kPerWave];  // index-major: a lane's byte offset of each piece
+    uint32_t back[kPerWave], whole;  // index-major: bytes back to the row's first chunk where k-tile `whole`, the last, has no more
     uint32_t row[kPerWave], last;  // k-major: the lane's k row of each piece (offset: its column); the last k row to read
 
     __device__ __forceinline__ static uint32_t swizzle(uint32_t r) {
         if constexpr (TR) return (r & 1) * 4 + (r >> 1 & 1) * 9;
         else return ((r & 3) | (r >> 4 & 1) << 2) ^ (r >> 2 & 1);
     }
-    // first: the tile's first index; indexes: memory rows (index-major) or, padded, columns (k-major) there are; depth: k
-    // rows there are (k-major)
+    // first: the tile's first index; indexes: memory rows (index-major) or columns, a multiple of 8 (k-major), there are; depth:
+    // k there are. What lies beyond reads as something else: results that are dropped, or k where the other operand holds
+    // zeros.
     __device__ __forceinline__ void begin(const uint16_t* p, uint64_t row_entries, uint32_t first, uint32_t indexes, uint32_t depth) {
         const uint32_t wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
         stride = row_entries * 2;
         last = depth - 1;
+        whole = depth * PARTS / 64;
+        if (!TR && first >= indexes) first = indexes - 1;
         if constexpr (TR) base = reinterpret_cast<const char*>(p) + static_cast<uint64_t>(first) * 2 * PARTS;
         else base = reinterpret_cast<const char*>(p) + first * stride;
 #pragma unroll
@@ -201,8 +378,9 @@ struct Operand {
                 row[j] = r;
                 offset[j] = (chunk < chunks ? chunk : chunks - 1) * 16;
             } else {
-                const uint32_t left = indexes - first - 1;  // clamped rows repeat the last: their results are dropped
+                const uint32_t left = indexes - first - 1;  // clamped rows repeat the last
                 offset[j] = (r < left ? r : left) * static_cast<uint32_t>(stride) + chunk * 16;
+                back[j] = chunk * 16 >= depth * PARTS * 2 % 128 ? chunk * 16 : 0;
             }
         }
     }
@@ -220,7 +398,7 @@ struct Operand {
         } else {
             const char* from = base + kt * 128;
 #pragma unroll
-            for (uint32_t j = 0; j < kPerWave; ++j) dma16(from, offset[j], lds + (wave * kPerWave + j) * 1024);
+            for (uint32_t j = 0; j < kPerWave; ++j) dma16(from, kt == whole ? offset[j] - back[j] : offset[j], lds + (wave * kPerWave + j) * 1024);
         }
     }
     // a lane's place in the tile for the 32-index blocks from `first` on
@@ -266,7 +444,8 @@ enum class Use { Stats, Grad, GradX, GradW };
 // One product of a loss call: which operands, how far they go, and what becomes of the results.
 struct Product {
     const uint16_t *a, *b;
-    uint64_t a_stride, b_stride;  // entries (16 bits) of a memory row
+    uint64_t a_stride, b_stride;  // 16-bit entries from one memory row to the next
+    uint32_t a_columns, b_columns;  // entries of a memory row: the weight's d in place, padded widths else
     uint32_t a_first;             // Stats, Grad: first vocabulary row of the piece
     uint32_t a_count, b_count;    // GradX, GradW: columns of the output; GradW: its rows
     uint32_t vocab;
@@ -285,25 +464,38 @@ struct Product {
     void* out;                    // GradW: [V, d]
     uint64_t out_stride;
     float scale;
-    bool mean, out_bf16;
+    bool mean, out_bf16, out_whole;  // out_whole: rows of the output start on 16-byte boundaries and hold whole 16-byte pieces
 };
 
-// A block of 8 waves takes WA TA 32 x WB TB 32 results, k-tiles through a ring of STAGES tile pairs: a k-tile's transfers
+// A block of WA x WB waves takes WA TA 32 x WB TB 32 results, k-tiles through a ring of STAGES tile pairs: a k-tile's transfers
 // are issued STAGES - 1 k-tiles ahead, one barrier a k-tile.
 template <int PARTS, Use USE, int WA, int WB, int TA, int TB>
 struct Shape {
     static constexpr bool kATr = USE == Use::GradX || USE == Use::GradW, kBTr = USE == Use::GradW;
     static constexpr int kA = WA * TA * 32, kB = WB * TB * 32;
-    using OpA = Operand<PARTS, kATr, kA>;
-    using OpB = Operand<PARTS, kBTr, kB>;
+    static constexpr int kWaves = WA * WB, kThreads = kWaves * kWave;
+    using OpA = Operand<PARTS, kATr, kA, kWaves>;
+    using OpB = Operand<PARTS, kBTr, kB, kWaves>;
     static constexpr uint32_t kStage = OpA::kBytes + OpB::kBytes;
-    static constexpr int kStages = 163840 / kStage < 4 ? 163840 / kStage : 4;
+    static constexpr int kStages = kWaves == 4 ? 3 : 163840 / kStage < 4 ? 163840 / kStage : 4;  // 4 waves: two blocks a CU
     static constexpr uint32_t kLds = kStage * kStages;
-    static_assert(WA * WB == static_cast<int>(kWaves) && kStages >= 2, "8 waves, two stages at least");
+    static_assert(kStages >= 2, "two stages at least");
 };
 
+// Tiles in groups of kGroup inner ones, a group's outer tiles one after the other: the 32 blocks that an XCD runs at a time
+// share kGroup inner and 4 outer tiles, 12 tiles' transfers through its L2 where rows of 32 inner ones would take 33.
+constexpr uint32_t kGroup = 8;
+struct TilePlace {
+    uint32_t inner, outer;
+};
+__device__ __forceinline__ TilePlace tile_place(uint32_t block, uint32_t inner, uint32_t outer) {
+    const uint32_t group = block / (kGroup * outer), rest = block % (kGroup * outer), left = inner - group * kGroup;
+    const uint32_t width = left < kGroup ? left : kGroup;
+    return {group * kGroup + rest % width, rest / width};
+}
+
 template <int PARTS, Use USE, int WA, int WB, int TA, int TB>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void loss_product_kernel(Product p) {
+__global__ __launch_bounds__(WA* WB* kWave) __attribute__((amdgpu_waves_per_eu(2, 2))) void loss_product_kernel(Product p) {
     using S = Shape<PARTS, USE, WA, WB, TA, TB>;
     using OpA = typename S::OpA;
     using OpB = typename S::OpB;
@@ -311,10 +503,11 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
     constexpr int kSteps = 4 / PARTS;
     const Meta meta = *p.meta;
     const uint32_t per_split = p.a_tiles * p.b_tiles, block = xcd_order(blockIdx.x, gridDim.x);
-    const uint32_t split_at = block / per_split, in_split = block % per_split;
+    const uint32_t split_at = block / per_split;
     // Stats, Grad: the token tiles of a vocabulary tile are neighbours; the others: the width tiles of a row tile
-    const bool tokens_first = USE == Use::Stats || USE == Use::Grad;
-    const uint32_t ta = tokens_first ? in_split / p.b_tiles : in_split % p.a_tiles, tb = tokens_first ? in_split % p.b_tiles : in_split / p.a_tiles;
+    constexpr bool kTokensFirst = USE == Use::Stats || USE == Use::Grad;
+    const TilePlace tile = tile_place(block % per_split, kTokensFirst ? p.b_tiles : p.a_tiles, kTokensFirst ? p.a_tiles : p.b_tiles);
+    const uint32_t ta = kTokensFirst ? tile.outer : tile.inner, tb = kTokensFirst ? tile.inner : tile.outer;
     const uint32_t a0 = ta * S::kA, b0 = tb * S::kB;
     if (USE != Use::GradW && b0 >= meta.valid) return;
 
@@ -328,14 +521,14 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
     OpA a;
     OpB b;
     if constexpr (USE == Use::Stats || USE == Use::Grad) {
-        a.begin(p.a, p.a_stride, p.a_first + a0, p.vocab, 0);
-        b.begin(p.b, p.b_stride, b0, p.n_pad, 0);
+        a.begin(p.a, p.a_stride, p.a_first + a0, p.vocab, p.a_columns);
+        b.begin(p.b, p.b_stride, b0, p.n_pad, p.b_columns);
     } else if constexpr (USE == Use::GradX) {
-        a.begin(p.a, p.a_stride, a0, static_cast<uint32_t>(p.a_stride / PARTS), p.vocab - p.a_first);
-        b.begin(p.b, p.b_stride, b0, p.n_pad, 0);
+        a.begin(p.a, p.a_stride, a0, p.a_columns, p.vocab - p.a_first);
+        b.begin(p.b, p.b_stride, b0, p.n_pad, p.b_columns);
     } else {
-        a.begin(p.a, p.a_stride, a0, static_cast<uint32_t>(p.a_stride / PARTS), p.n_pad);
-        b.begin(p.b, p.b_stride, b0, static_cast<uint32_t>(p.b_stride / PARTS), p.n_pad);
+        a.begin(p.a, p.a_stride, a0, p.a_columns, p.n_pad);
+        b.begin(p.b, p.b_stride, b0, p.b_columns, p.n_pad);
     }
 
     const uint32_t wave = threadIdx.x / kWave, wa = wave % WA, wb = wave / WA, lane = threadIdx.x % kWave;
@@ -356,33 +549,54 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
             acc[i][j] = 0.0f;
             if constexpr (PARTS == 2) sums[i][j] = 0.0f;
         }
-    for (uint32_t kt = k_begin; kt < k_end && kt < k_begin + S::kStages - 1; ++kt) fetch(kt);
-    for (uint32_t kt = k_begin; kt < k_end; ++kt) {
-        if (k_end - kt >= static_cast<uint32_t>(S::kStages) - 1) wait_loads<kTransfers * (S::kStages - 2)>();
-        else wait_loads<0>();
-        asm volatile("" ::: "memory");  // the last k-tile's LDS reads stay before the barrier, this one's behind it
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        if (kt + S::kStages - 1 < k_end) fetch(kt + S::kStages - 1);
+    // The operands of a step (16 k) are read from LDS while the step before it multiplies; the last step of a k-tile reads
+    // the first of the next, behind the barrier that says every wave's transfers of it have landed and every wave has read
+    // the last of the k-tile before it, whose stage the transfers of k-tile kt + STAGES then take.
+    Frag fa[2][TA][PARTS], fb[2][TB][PARTS];
+    const auto read = [&](uint32_t kt, int step, int to) {
         const uint32_t tile_a = lds + (kt - k_begin) % S::kStages * S::kStage, tile_b = tile_a + OpA::kBytes;
 #pragma unroll
+        for (int part = 0; part < PARTS; ++part) {
+#pragma unroll
+            for (int i = 0; i < TA; ++i) fa[to][i][part] = OpA::read(tile_a, a_place, i, step, part);
+#pragma unroll
+            for (int j = 0; j < TB; ++j) fb[to][j][part] = OpB::read(tile_b, b_place, j, step, part);
+        }
+    };
+    // Waits for k-tile kt's transfers of every wave, of whose later ones up to `later` k-tiles' are in flight.
+    const auto arrive = [&](uint32_t kt, auto later) {
+        constexpr int kLater = decltype(later)::value;
+        if (k_end - kt > static_cast<uint32_t>(kLater)) wait_loads<static_cast<int>(kTransfers) * kLater>();
+        else wait_loads<0>();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    static_assert(kSteps % 2 == 0, "a k-tile's first step always reads into the same registers");
+    for (uint32_t kt = k_begin; kt < k_end && kt < k_begin + S::kStages; ++kt) fetch(kt);
+    if (k_begin < k_end) {
+        arrive(k_begin, std::integral_constant<int, S::kStages - 1>{});
+        read(k_begin, 0, 0);
+    }
+    for (uint32_t kt = k_begin; kt < k_end; ++kt) {
+#pragma unroll
         for (int step = 0; step < kSteps; ++step) {
-            Frag fa[TA][PARTS], fb[TB][PARTS];
-#pragma unroll
-            for (int part = 0; part < PARTS; ++part) {
-#pragma unroll
-                for (int i = 0; i < TA; ++i) fa[i][part] = OpA::read(tile_a, a_place, i, step, part);
-#pragma unroll
-                for (int j = 0; j < TB; ++j) fb[j][part] = OpB::read(tile_b, b_place, j, step, part);
+            const int now = step % 2;
+            if (step + 1 < kSteps) {
+                read(kt, step + 1, 1 - now);
+            } else if (kt + 1 < k_end) {
+                arrive(kt + 1, std::integral_constant<int, S::kStages - 2>{});
+                if (kt + S::kStages < k_end) fetch(kt + S::kStages);
+                read(kt + 1, 0, 1 - now);
             }
 #pragma unroll
             for (int i = 0; i < TA; ++i)
 #pragma unroll
                 for (int j = 0; j < TB; ++j) {
-                    acc[i][j] = multiply<PARTS>(fa[i][0], fb[j][0], acc[i][j]);
+                    acc[i][j] = multiply<PARTS>(fa[now][i][0], fb[now][j][0], acc[i][j]);
                     if constexpr (PARTS == 2) {
-                        acc[i][j] = multiply<PARTS>(fa[i][0], fb[j][1], acc[i][j]);
-                        acc[i][j] = multiply<PARTS>(fa[i][1], fb[j][0], acc[i][j]);
+                        acc[i][j] = multiply<PARTS>(fa[now][i][0], fb[now][j][1], acc[i][j]);
+                        acc[i][j] = multiply<PARTS>(fa[now][i][1], fb[now][j][0], acc[i][j]);
                     }
                 }
         }
@@ -526,13 +740,28 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
                         *reinterpret_cast<float4*>(to + r) = v;
                     }
                 } else {
-                    const uint64_t at = at_b * p.out_stride + at_a;
+                    const uint64_t to = at_b * p.out_stride + at_a;
+                    float v[16];
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        if (at_a + r >= p.a_count) continue;
-                        const float v = factor * result(i, j, r);
-                        if (p.out_bf16) static_cast<uint16_t*>(p.out)[at + r] = bf16_bits(v);
-                        else static_cast<float*>(p.out)[at + r] = v;
+                    for (int r = 0; r < 16; ++r) v[r] = factor * result(i, j, r);
+                    if (p.out_whole && p.out_bf16) {
+#pragma unroll
+                        for (int r = 0; r < 16; r += 8)
+                            if (at_a + r < p.a_count)
+                                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + to + r) =
+                                    make_uint4(bf16_pair(v[r], v[r + 1]), bf16_pair(v[r + 2], v[r + 3]), bf16_pair(v[r + 4], v[r + 5]), bf16_pair(v[r + 6], v[r + 7]));
+                    } else if (p.out_whole) {
+#pragma unroll
+                        for (int r = 0; r < 16; r += 4)
+                            if (at_a + r < p.a_count)
+                                *reinterpret_cast<float4*>(static_cast<float*>(p.out) + to + r) = make_float4(v[r], v[r + 1], v[r + 2], v[r + 3]);
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            if (at_a + r >= p.a_count) continue;
+                            if (p.out_bf16) static_cast<uint16_t*>(p.out)[to + r] = bf16_bits(v[r]);
+                            else static_cast<float*>(p.out)[to + r] = v[r];
+                        }
                     }
                 }
             }
@@ -542,15 +771,17 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
 
 // ------------------------------------------------------------------------------------------- the sums over the vocabulary
 
-// lse and loss of every counted token from the slices: 16 tokens a block, 64 threads each over the slices.
-constexpr uint32_t kLseTokens = 16, kLseLanes = 64;
-__global__ __launch_bounds__(kLseTokens* kLseLanes) void loss_lse_kernel(const float2* __restrict__ slices, uint32_t count, uint32_t n_pad,
-                                                                        const float* __restrict__ picked, const int32_t* __restrict__ rows,
-                                                                        const int32_t* __restrict__ labels, const Meta* __restrict__ meta,
-                                                                        float* __restrict__ lse, float* __restrict__ losses) {
-    __shared__ float2 lds[kLseLanes][kLseTokens];
-    const uint32_t in = threadIdx.x % kLseTokens, first = threadIdx.x / kLseTokens, t = blockIdx.x * kLseTokens + in, valid = meta->valid;
-    if (blockIdx.x * kLseTokens >= valid) return;
+// lse and loss of every counted token from the slices: TOKENS tokens a block, 1024 / TOKENS threads each over the slices.
+constexpr uint32_t kLseThreads = 1024;
+template <uint32_t TOKENS>
+__global__ __launch_bounds__(kLseThreads) void loss_lse_kernel(const float2* __restrict__ slices, uint32_t count, uint32_t n_pad,
+                                                              const float* __restrict__ picked, const int32_t* __restrict__ rows,
+                                                              const int32_t* __restrict__ labels, const Meta* __restrict__ meta,
+                                                              float* __restrict__ lse, float* __restrict__ losses) {
+    constexpr uint32_t kLanes = kLseThreads / TOKENS;
+    __shared__ float2 lds[kLanes][TOKENS];
+    const uint32_t in = threadIdx.x % TOKENS, first = threadIdx.x / TOKENS, t = blockIdx.x * TOKENS + in, valid = meta->valid;
+    if (blockIdx.x * TOKENS >= valid) return;
     const auto join = [](float2 a, float2 b) {
         const float most = fmaxf(a.x, b.x);
         if (most == -__builtin_huge_valf()) return make_float2(most, a.y + b.y);
@@ -558,10 +789,11 @@ __global__ __launch_bounds__(kLseTokens* kLseLanes) void loss_lse_kernel(const f
     };
     float2 all = make_float2(-__builtin_huge_valf(), 0.0f);
     if (t < valid)
-        for (uint32_t s = first; s < count; s += kLseLanes) all = join(all, slices[static_cast<uint64_t>(s) * n_pad + t]);
+#pragma unroll 4
+        for (uint32_t s = first; s < count; s += kLanes) all = join(all, slices[static_cast<uint64_t>(s) * n_pad + t]);
     lds[first][in] = all;
     __syncthreads();
-    for (uint32_t step = kLseLanes / 2; step > 0; step /= 2) {
+    for (uint32_t step = kLanes / 2; step > 0; step /= 2) {
         if (first < step) lds[first][in] = join(lds[first][in], lds[first + step][in]);
         __syncthreads();
     }
@@ -572,19 +804,20 @@ __global__ __launch_bounds__(kLseTokens* kLseLanes) void loss_lse_kernel(const f
     losses[rows[t]] = labels[t] < 0 ? __uint_as_float(0x7fc00000u) : value - picked[t];
 }
 
-// gx of every token: the splits' sums in order times the factor; zeros for tokens that do not count. The last block: the
-// loss, the tokens' losses added in a fixed order.
-constexpr uint32_t kFinishThreads = 256;
+// gx of every token: the splits' sums in order times the factor; zeros for tokens that do not count. A wave per token,
+// four entries a lane and step (the partials' rows are padded to whole steps' quarters). The last block: the loss, the
+// tokens' losses added in a fixed order.
+constexpr uint32_t kFinishThreads = 256, kFinishRows = kFinishThreads / kWave;
 template <typename T>
 __global__ __launch_bounds__(kFinishThreads) void loss_finish_kernel(const float* __restrict__ partial, uint32_t splits, uint32_t n_pad, uint32_t width,
                                                                     const int32_t* __restrict__ place, const Meta* __restrict__ meta, uint32_t n,
                                                                     uint32_t d, float scale, bool mean, const float* __restrict__ losses,
-                                                                    float* __restrict__ loss, T* __restrict__ gx) {
+                                                                    float* __restrict__ loss, T* __restrict__ gx, bool whole) {
     const Meta m = *meta;
-    const uint32_t t = blockIdx.x;
-    if (t == n) {
+    if (blockIdx.x == gridDim.x - 1) {
         __shared__ double lds[kFinishThreads];
         double sum = 0.0;
+#pragma unroll 8
         for (uint32_t i = threadIdx.x; i < n; i += kFinishThreads) sum += losses[i];
         lds[threadIdx.x] = sum;
         __syncthreads();
@@ -595,44 +828,68 @@ __global__ __launch_bounds__(kFinishThreads) void loss_finish_kernel(const float
         if (threadIdx.x == 0) *loss = static_cast<float>(mean && m.valid != 0 ? lds[0] / m.valid : lds[0]);
         return;
     }
+    const uint32_t t = blockIdx.x * kFinishRows + threadIdx.x / kWave;
+    if (t >= n) return;
     const int32_t row = place[t];
     const float factor = grad_factor(m, scale, mean);
-    for (uint32_t c = threadIdx.x; c < d; c += kFinishThreads) {
-        float sum = 0.0f;
+    const float* from = partial + static_cast<uint64_t>(row < 0 ? 0 : row) * width;
+    const uint64_t next = static_cast<uint64_t>(n_pad) * width;
+    T* to = gx + static_cast<uint64_t>(t) * d;
+    for (uint32_t c = 4 * (threadIdx.x % kWave); c < d; c += 4 * kWave) {
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         if (row >= 0) {
-            for (uint32_t s = 0; s < splits; ++s) sum += partial[(static_cast<uint64_t>(s) * n_pad + row) * width + c];
-            sum *= factor;
+#pragma unroll 4
+            for (uint32_t s = 0; s < splits; ++s) {
+                const float4 part = *reinterpret_cast<const float4*>(from + s * next + c);
+                v[0] += part.x; v[1] += part.y; v[2] += part.z; v[3] += part.w;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] *= factor;
         } else if (m.invalid != 0) {
-            sum = factor;  // NaN: a label was outside the vocabulary
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = factor;  // NaN: a label was outside the vocabulary
         }
-        if constexpr (sizeof(T) == 4) gx[static_cast<uint64_t>(t) * d + c] = sum;
-        else gx[static_cast<uint64_t>(t) * d + c] = bf16_bits(sum);
+        if (whole) {
+            if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(to + c) = make_float4(v[0], v[1], v[2], v[3]);
+            else *reinterpret_cast<uint2*>(to + c) = make_uint2(bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]));
+        } else {
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k)
+                if (c + k < d) {
+                    if constexpr (sizeof(T) == 4) to[c + k] = v[k];
+                    else to[c + k] = bf16_bits(v[k]);
+                }
+        }
     }
 }
 
 // ------------------------------------------------------------------------------------------------------------ the host
 
-constexpr uint32_t kTile = 256;               // vocabulary rows and width of a tile
+constexpr uint32_t kTile = 256;                // vocabulary rows and width of a tile
+constexpr uint32_t kFewTokens = 64, kFewTile = 128;  // up to so many tokens: tiles of 128 x 64, two blocks a CU
 constexpr uint64_t kGradBytes = 256ull << 20;  // a piece's D at most (or one vocabulary tile's)
-constexpr uint32_t kBlocks = 256;             // CUs
+constexpr uint32_t kCus = 256;
 
 uint32_t ceil_div(uint64_t a, uint32_t b) { return static_cast<uint32_t>((a + b - 1) / b); }
 uint32_t padded(uint32_t v, uint32_t to) { return ceil_div(v, to) * to; }
 
 struct Plan {
-    uint32_t parts, n_pad, width, token_tile, slices, piece, pieces, splits;
-    bool in_place;
-    uint64_t meta, rows, labels, place, lse, picked, losses, slice_sums, x, weight, grad, partial, bytes;
+    uint32_t parts, n_pad, width, vocab_tile, token_tile, slices, piece, pieces, splits;
+    bool few, in_place;
+    uint64_t meta, rows, labels, place, lse, picked, losses, slice_sums, x_most, w_most, x, weight, grad, partial, bytes;
 };
 
+// `aligned`: the weight starts on a 16-byte boundary (bfloat16 weights of whole 16-byte pieces are then read in place).
 Plan plan_of(int vt, uint32_t n, uint32_t d, uint32_t vocab, bool aligned, bool gradients) {
     Plan p{};
     p.parts = vt == kBF16 ? 1 : 2;
-    p.token_tile = p.parts == 1 ? 256 : 128;
-    p.n_pad = padded(n, 256);
+    p.few = n <= kFewTokens;
+    p.vocab_tile = p.few ? kFewTile : kTile;
+    p.token_tile = p.few ? kFewTokens : p.parts == 1 ? 256 : 128;
+    p.n_pad = padded(n, p.few ? kFewTokens : 256);
     p.width = padded(d, 64 / p.parts);
-    p.in_place = p.parts == 1 && d % 64 == 0 && aligned;
-    p.slices = ceil_div(vocab, kTile) * (p.parts == 1 ? 2 : 4);
+    p.in_place = p.parts == 1 && d % 8 == 0 && aligned;
+    p.slices = ceil_div(vocab, p.vocab_tile) * (!p.few && p.parts == 1 ? 2 : 4);  // a slice per wave along the vocabulary
     uint64_t at = 0;
     const auto take = [&](uint64_t bytes) {
         const uint64_t here = at;
@@ -647,6 +904,10 @@ Plan plan_of(int vt, uint32_t n, uint32_t d, uint32_t vocab, bool aligned, bool 
     p.picked = take(4ull * p.n_pad);
     p.losses = take(4ull * p.n_pad);
     p.slice_sums = take(sizeof(float2) * p.slices * p.n_pad);
+    if (p.parts == 2) {
+        p.x_most = take(4ull * ceil_div(p.n_pad, kPrepWaves));
+        p.w_most = take(4ull * ceil_div(vocab, kWeightRows));
+    }
     p.x = take(2ull * p.parts * p.n_pad * p.width);
     p.weight = p.in_place ? 0 : take(2ull * p.parts * vocab * p.width);
     if (gradients) {
@@ -656,9 +917,10 @@ Plan plan_of(int vt, uint32_t n, uint32_t d, uint32_t vocab, bool aligned, bool 
         p.pieces = ceil_div(tiles, fit);
         p.piece = ceil_div(tiles, p.pieces) * kTile;
         p.pieces = ceil_div(vocab, p.piece);
-        const uint32_t blocks = ceil_div(p.width, kTile) * (p.n_pad / p.token_tile), k_tiles = p.piece / (64 / p.parts);
-        const uint32_t fill = ceil_div(kBlocks, blocks);  // splits that give every CU a block
-        p.splits = fill < 1 ? 1 : fill > k_tiles / 8 ? (k_tiles / 8 < 1 ? 1 : k_tiles / 8) : fill;
+        // splits of the vocabulary that give every CU a block (few tokens: two), each of 8 k-tiles at least
+        const uint32_t blocks = ceil_div(p.width, p.vocab_tile) * (p.n_pad / p.token_tile), k_tiles = p.piece / (64 / p.parts);
+        const uint32_t fill = ceil_div(p.few ? 2 * kCus : kCus, blocks), limit = k_tiles / 8 < 1 ? 1 : k_tiles / 8;
+        p.splits = fill < limit ? fill : limit;
         p.grad = take(per_row * p.piece);
         p.partial = take(4ull * p.splits * p.n_pad * p.width);
     }
@@ -668,14 +930,15 @@ Plan plan_of(int vt, uint32_t n, uint32_t d, uint32_t vocab, bool aligned, bool 
 
 template <int PARTS, Use USE, int WA, int WB, int TA, int TB>
 hipError_t launch_product(const Product& p, hipStream_t stream) {
-    const auto kernel = loss_product_kernel<PARTS, USE, WA, WB, TA, TB>;
-    hipLaunchKernelGGL(kernel, dim3(p.a_tiles * p.b_tiles * p.splits), dim3(kThreads), 0, stream, p);
+    hipLaunchKernelGGL((loss_product_kernel<PARTS, USE, WA, WB, TA, TB>), dim3(p.a_tiles * p.b_tiles * p.splits), dim3(WA * WB * kWave), 0, stream, p);
     return hipGetLastError();
 }
 
 template <Use USE>
-hipError_t product(uint32_t parts, const Product& p, hipStream_t stream) {
-    return parts == 1 ? launch_product<1, USE, 2, 4, 4, 2>(p, stream) : launch_product<2, USE, 4, 2, 2, 2>(p, stream);
+hipError_t product(const Plan& plan, const Product& p, hipStream_t stream) {
+    if constexpr (USE != Use::GradW)
+        if (plan.few) return plan.parts == 1 ? launch_product<1, USE, 4, 1, 1, 2>(p, stream) : launch_product<2, USE, 4, 1, 1, 2>(p, stream);
+    return plan.parts == 1 ? launch_product<1, USE, 2, 4, 4, 2>(p, stream) : launch_product<2, USE, 4, 2, 2, 2>(p, stream);
 }
 
 template <typename T>
@@ -689,25 +952,26 @@ hipError_t run(const LossCall& c, hipStream_t stream) {
     float *const lse = reinterpret_cast<float*>(work + plan.lse), *const picked = reinterpret_cast<float*>(work + plan.picked);
     float* const losses = c.losses != nullptr ? c.losses : reinterpret_cast<float*>(work + plan.losses);
     uint16_t* const x = reinterpret_cast<uint16_t*>(work + plan.x);
-    uint16_t* const packed = reinterpret_cast<uint16_t*>(work + plan.weight);
-    const uint16_t* const weight = plan.in_place ? static_cast<const uint16_t*>(c.weight) : packed;
-    const uint64_t row = static_cast<uint64_t>(plan.width) * plan.parts;
-    const auto done = [](hipError_t& status) { return (status = hipGetLastError()) != hipSuccess; };
+    const uint16_t* const weight = plan.in_place ? static_cast<const uint16_t*>(c.weight) : reinterpret_cast<const uint16_t*>(work + plan.weight);
+    const uint64_t x_row = static_cast<uint64_t>(plan.width) * plan.parts, w_row = plan.in_place ? c.d : x_row;
+    const uint32_t w_columns = plan.in_place ? c.d : plan.width, depth = 64 / plan.parts;
+    const auto failed = [](hipError_t& status) { return (status = hipGetLastError()) != hipSuccess; };
     hipError_t status;
 
-    hipLaunchKernelGGL(loss_scan_kernel, dim3(1), dim3(kScanThreads), 0, stream, c.labels, c.labels_stride, c.wide_labels, c.ignore, c.n, c.vocab, rows,
-                       labels, place, losses, meta);
-    if (done(status)) return status;
-    if constexpr (sizeof(T) == 4) {
-        const uint32_t weight_blocks = 8 * kBlocks, x_blocks = c.n < kBlocks ? c.n : kBlocks;
-        hipLaunchKernelGGL(loss_range_kernel, dim3(weight_blocks + x_blocks), dim3(kRangeThreads), 0, stream, static_cast<const float*>(c.weight),
-                           static_cast<uint64_t>(c.vocab) * c.d, static_cast<const float*>(c.x), c.x_stride, c.d, rows, meta, weight_blocks);
-        if (done(status)) return status;
+    const Prepare prepare{c.labels, c.x, c.weight, c.labels_stride, c.ignore, c.x_stride, c.wide_labels, c.n, c.d, plan.width, c.vocab, rows, labels,
+                          place, losses, meta, x, reinterpret_cast<uint16_t*>(work + plan.weight),
+                          reinterpret_cast<uint32_t*>(work + plan.x_most), reinterpret_cast<uint32_t*>(work + plan.w_most),
+                          ceil_div(padded(c.n, 64), kPrepWaves), plan.in_place ? 0 : ceil_div(c.vocab, kWeightRows)};
+    if (c.n > kScanTokens) {
+        hipLaunchKernelGGL(loss_scan_kernel, dim3(1), dim3(kScanThreads), 0, stream, prepare);
+        if (failed(status)) return status;
     }
-    const uint32_t x_blocks = ceil_div(padded(c.n, 64), kPackRows), w_blocks = plan.in_place ? 0 : ceil_div(c.vocab, kPackRows);
-    hipLaunchKernelGGL(loss_pack_kernel<T>, dim3(x_blocks + w_blocks), dim3(kPackThreads), 0, stream, static_cast<const T*>(c.x), c.x_stride,
-                       static_cast<const T*>(c.weight), c.vocab, c.d, plan.width, rows, meta, x, packed, x_blocks);
-    if (done(status)) return status;
+    hipLaunchKernelGGL(loss_prepare_kernel<T>, dim3(prepare.x_blocks + prepare.w_blocks), dim3(kPrepThreads), 0, stream, prepare);
+    if (failed(status)) return status;
+    if constexpr (sizeof(T) == 4) {
+        hipLaunchKernelGGL(loss_settle_kernel, dim3(2 * kCus), dim3(kPrepThreads), 0, stream, prepare);
+        if (failed(status)) return status;
+    }
 
     Product p{};
     p.meta = meta;
@@ -719,63 +983,72 @@ hipError_t run(const LossCall& c, hipStream_t stream) {
     p.mean = c.mean;
     p.out_bf16 = c.value_type == kBF16;
     p.splits = 1;
-    const uint32_t token_tiles = ceil_div(c.n, plan.token_tile), width_tiles = ceil_div(plan.width, kTile);
+    const uint32_t token_tiles = ceil_div(c.n, plan.token_tile);
     Product stats = p;
     stats.a = weight;
-    stats.a_stride = row;
+    stats.a_stride = w_row;
+    stats.a_columns = w_columns;
     stats.b = x;
-    stats.b_stride = row;
-    stats.k_tiles = plan.width / (64 / plan.parts);
-    stats.a_tiles = ceil_div(c.vocab, kTile);
+    stats.b_stride = x_row;
+    stats.b_columns = plan.width;
+    stats.k_tiles = plan.width / depth;
+    stats.a_tiles = ceil_div(c.vocab, plan.vocab_tile);
     stats.b_tiles = token_tiles;
     stats.picked = picked;
     stats.slices = reinterpret_cast<float2*>(work + plan.slice_sums);
-    if ((status = product<Use::Stats>(plan.parts, stats, stream)) != hipSuccess) return status;
-    hipLaunchKernelGGL(loss_lse_kernel, dim3(ceil_div(c.n, kLseTokens)), dim3(kLseTokens * kLseLanes), 0, stream, stats.slices, plan.slices, plan.n_pad,
-                       picked, rows, labels, meta, lse, losses);
-    if (done(status)) return status;
+    if ((status = product<Use::Stats>(plan, stats, stream)) != hipSuccess) return status;
+    if (plan.few) hipLaunchKernelGGL(loss_lse_kernel<1>, dim3(c.n), dim3(kLseThreads), 0, stream, stats.slices, plan.slices, plan.n_pad, picked, rows, labels, meta, lse, losses);
+    else hipLaunchKernelGGL(loss_lse_kernel<16>, dim3(ceil_div(c.n, 16)), dim3(kLseThreads), 0, stream, stats.slices, plan.slices, plan.n_pad, picked, rows, labels, meta, lse, losses);
+    if (failed(status)) return status;
     if (!gradients) return hipSuccess;
 
     for (uint32_t first = 0; first < c.vocab; first += plan.piece) {
         const uint32_t count = c.vocab - first < plan.piece ? c.vocab - first : plan.piece;
         Product grad = stats;
         grad.a_first = first;
-        grad.a_tiles = ceil_div(count, kTile);
+        grad.a_tiles = ceil_div(padded(count, kTile), plan.vocab_tile);
         grad.grad = reinterpret_cast<uint16_t*>(work + plan.grad);
         grad.grad_stride = static_cast<uint64_t>(plan.piece) * plan.parts;
-        if ((status = product<Use::Grad>(plan.parts, grad, stream)) != hipSuccess) return status;
+        if ((status = product<Use::Grad>(plan, grad, stream)) != hipSuccess) return status;
 
         Product gx = p;
-        gx.a = weight + first * row;
-        gx.a_stride = row;
+        gx.a = weight + first * w_row;
+        gx.a_stride = w_row;
+        gx.a_columns = w_columns;
         gx.b = grad.grad;
         gx.b_stride = grad.grad_stride;
+        gx.b_columns = plan.piece;
         gx.a_first = first;
         gx.a_count = plan.width;
-        gx.k_tiles = ceil_div(count, 64 / plan.parts);
-        gx.a_tiles = width_tiles;
+        gx.k_tiles = ceil_div(count, depth);
+        gx.a_tiles = ceil_div(w_columns, plan.vocab_tile);
         gx.b_tiles = token_tiles;
         gx.splits = plan.splits;
         gx.partial = reinterpret_cast<float*>(work + plan.partial);
         gx.out_stride = plan.width;
         gx.add = first != 0;
-        if ((status = product<Use::GradX>(plan.parts, gx, stream)) != hipSuccess) return status;
+        if ((status = product<Use::GradX>(plan, gx, stream)) != hipSuccess) return status;
 
         Product gw = p;
         gw.a = x;
-        gw.a_stride = row;
+        gw.a_stride = x_row;
+        gw.a_columns = plan.width;
         gw.b = grad.grad;
         gw.b_stride = grad.grad_stride;
+        gw.b_columns = plan.piece;
         gw.a_count = c.d;
         gw.b_count = count;
-        gw.a_tiles = width_tiles;
-        gw.b_tiles = ceil_div(count, plan.token_tile);
+        gw.a_tiles = ceil_div(c.d, kTile);
+        gw.b_tiles = ceil_div(count, plan.parts == 1 ? 256 : 128);
         gw.out = static_cast<T*>(c.gw) + static_cast<uint64_t>(first) * c.d;
         gw.out_stride = c.d;
-        if ((status = product<Use::GradW>(plan.parts, gw, stream)) != hipSuccess) return status;
+        gw.out_whole = c.d % (16 / sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(c.gw) % 16 == 0;
+        if ((status = product<Use::GradW>(plan, gw, stream)) != hipSuccess) return status;
     }
-    hipLaunchKernelGGL(loss_finish_kernel<T>, dim3(c.n + 1), dim3(kFinishThreads), 0, stream, reinterpret_cast<const float*>(work + plan.partial), plan.splits,
-                       plan.n_pad, plan.width, place, meta, c.n, c.d, c.scale, c.mean, losses, c.loss, static_cast<T*>(c.gx));
+    const bool whole = c.d % 4 == 0 && reinterpret_cast<uintptr_t>(c.gx) % 16 == 0;
+    hipLaunchKernelGGL(loss_finish_kernel<T>, dim3(ceil_div(c.n, kFinishRows) + 1), dim3(kFinishThreads), 0, stream,
+                       reinterpret_cast<const float*>(work + plan.partial), plan.splits, plan.n_pad, plan.width, place, meta, c.n, c.d, c.scale, c.mean,
+                       losses, c.loss, static_cast<T*>(c.gx), whole);
     return hipGetLastError();
 }
 

@@ -85,7 +85,7 @@ def run_both(n, d, vocab, dtype, ignored=0.0, seed=0, std=1.0):
 @pytest.mark.parametrize("dtype", (BF16, F32))
 @pytest.mark.parametrize("n,d,vocab", [
     (1, 64, 256), (1, 1, 1), (1, 2048, 3000), (2, 17, 2), (63, 64, 255), (64, 128, 257), (65, 100, 1000), (128, 520, 31),
-    (129, 1001, 513), (255, 32, 2999), (257, 320, 1024), (300, 1104, 777), (700, 96, 512), (1030, 64, 300),
+    (129, 1001, 513), (255, 32, 2999), (9, 104, 100), (50, 1608, 385), (200, 1104, 129), (4097, 72, 640), (5000, 40, 257), (257, 320, 1024), (300, 1104, 777), (700, 96, 512), (1030, 64, 300),
 ])
 def test_sizes(n, d, vocab, dtype):
     run_both(n, d, vocab, dtype)
@@ -164,6 +164,23 @@ def test_weight_rows_of_zero_and_of_other_scales():
     ref = reference(x, weight, labels)
     check_losses(head.losses(x, labels), ref)
     check_step(head.step(x, labels), ref, x, weight, 140)
+
+
+@pytest.mark.parametrize("which", ("weight", "x", "both", "first rows"))
+def test_lone_large_entries(which):
+    """One entry 1e4 times the others in float32 tensors, wherever it lies, and tensors whose other rows are zeros."""
+    x, weight, labels = make(300, 160, 2000, F32, ignored=0.1, seed=13)
+    x *= 1e-2
+    if which in ("weight", "both"):
+        weight[1234, 77] = 1e4 * 0.08
+    if which in ("x", "both"):
+        x[int((labels != IGNORE).nonzero()[37]), 131] = 1e4 * 1e-2
+    if which == "first rows":
+        weight[3:], x[5:] = 0.0, 0.0
+    head = HeadLoss(weight)
+    ref = reference(x, weight, labels)
+    check_losses(head.losses(x, labels), ref)
+    check_step(head.step(x, labels), ref, x, weight, int((labels != IGNORE).sum()))
 
 
 @pytest.mark.parametrize("dtype", (BF16, F32))
