@@ -467,23 +467,24 @@ struct Product {
     bool mean, out_bf16, out_whole;  // out_whole: rows of the output start on 16-byte boundaries and hold whole 16-byte pieces
 };
 
-// A block of WA x WB waves takes WA TA 32 x WB TB 32 results, k-tiles through a ring of STAGES tile pairs: a k-tile's transfers
-// are issued STAGES - 1 k-tiles ahead, one barrier a k-tile.
-template <int PARTS, Use USE, int WA, int WB, int TA, int TB>
+// WA x WB waves of TA x TB 32 x 32 results each; k-tiles go through a ring of kStages tile pairs.
+template <int PARTS_, Use USE_, int WA_, int WB_, int TA_, int TB_>
 struct Shape {
+    static constexpr int PARTS = PARTS_, WA = WA_, WB = WB_, TA = TA_, TB = TB_;
+    static constexpr Use USE = USE_;
     static constexpr bool kATr = USE == Use::GradX || USE == Use::GradW, kBTr = USE == Use::GradW;
-    static constexpr int kA = WA * TA * 32, kB = WB * TB * 32;
-    static constexpr int kWaves = WA * WB, kThreads = kWaves * kWave;
+    static constexpr int kA = WA * TA * 32, kB = WB * TB * 32, kWaves = WA * WB;
     using OpA = Operand<PARTS, kATr, kA, kWaves>;
     using OpB = Operand<PARTS, kBTr, kB, kWaves>;
-    static constexpr uint32_t kStage = OpA::kBytes + OpB::kBytes;
+    static constexpr uint32_t kStage = OpA::kBytes + OpB::kBytes, kTransfers = OpA::kPerWave + OpB::kPerWave;
     static constexpr int kStages = kWaves == 4 ? 3 : 163840 / kStage < 4 ? 163840 / kStage : 4;  // 4 waves: two blocks a CU
     static constexpr uint32_t kLds = kStage * kStages;
     static_assert(kStages >= 2, "two stages at least");
 };
 
 // Tiles in groups of kGroup inner ones, a group's outer tiles one after the other: the 32 blocks that an XCD runs at a time
-// share kGroup inner and 4 outer tiles, 12 tiles' transfers through its L2 where rows of 32 inner ones would take 33.
+// share kGroup inner and 4 outer tiles, 12 tiles' transfers through its L2 where rows of 32 inner ones would take 33
+// (8192 tokens of 2048 x 50304: the forward's product 1510 -> 1460 us).
 constexpr uint32_t kGroup = 8;
 struct TilePlace {
     uint32_t inner, outer;
@@ -494,90 +495,112 @@ __device__ __forceinline__ TilePlace tile_place(uint32_t block, uint32_t inner, 
     return {group * kGroup + rest % width, rest / width};
 }
 
-template <int PARTS, Use USE, int WA, int WB, int TA, int TB>
-__global__ __launch_bounds__(WA* WB* kWave) __attribute__((amdgpu_waves_per_eu(2, 2))) void loss_product_kernel(Product p) {
-    using S = Shape<PARTS, USE, WA, WB, TA, TB>;
-    using OpA = typename S::OpA;
-    using OpB = typename S::OpB;
-    __shared__ __attribute__((aligned(1024))) char ring[S::kLds];
-    constexpr int kSteps = 4 / PARTS;
-    const Meta meta = *p.meta;
-    const uint32_t per_split = p.a_tiles * p.b_tiles, block = xcd_order(blockIdx.x, gridDim.x);
-    const uint32_t split_at = block / per_split;
-    // Stats, Grad: the token tiles of a vocabulary tile are neighbours; the others: the width tiles of a row tile
-    constexpr bool kTokensFirst = USE == Use::Stats || USE == Use::Grad;
-    const TilePlace tile = tile_place(block % per_split, kTokensFirst ? p.b_tiles : p.a_tiles, kTokensFirst ? p.a_tiles : p.b_tiles);
-    const uint32_t ta = kTokensFirst ? tile.outer : tile.inner, tb = kTokensFirst ? tile.inner : tile.outer;
-    const uint32_t a0 = ta * S::kA, b0 = tb * S::kB;
-    if (USE != Use::GradW && b0 >= meta.valid) return;
+// Where a tile's results lie.
+struct TileAt {
+    uint32_t a0, b0, split;
+};
 
-    uint32_t k_begin = 0, k_end = p.k_tiles;
-    if (USE == Use::GradX) {
-        k_begin = static_cast<uint64_t>(p.k_tiles) * split_at / p.splits;
-        k_end = static_cast<uint64_t>(p.k_tiles) * (split_at + 1) / p.splits;
+// One tile: where it lies, its operands and its k-tiles.
+template <typename S>
+struct Tile {
+    TileAt at;
+    uint32_t k_begin, k_end;
+    typename S::OpA a;
+    typename S::OpB b;
+
+    // part `part` (of tiles WHOLE::kA x WHOLE::kB cut into tiles of this shape) of tile `index` of the live_b token tiles;
+    // false where it has no results
+    template <typename WHOLE>
+    __device__ __forceinline__ bool begin(const Product& p, uint32_t valid, uint32_t live_b, uint32_t index, uint32_t part) {
+        constexpr Use USE = S::USE;
+        constexpr bool kTokensFirst = USE == Use::Stats || USE == Use::Grad;
+        const uint32_t per_split = p.a_tiles * live_b;
+        at.split = index / per_split;
+        const TilePlace tile = tile_place(index % per_split, kTokensFirst ? live_b : p.a_tiles, kTokensFirst ? p.a_tiles : live_b);
+        constexpr uint32_t kPartsA = WHOLE::kA / S::kA;
+        at.a0 = (kTokensFirst ? tile.outer : tile.inner) * WHOLE::kA + part % kPartsA * S::kA;
+        at.b0 = (kTokensFirst ? tile.inner : tile.outer) * WHOLE::kB + part / kPartsA * S::kB;
+        k_begin = 0;
+        k_end = p.k_tiles;
+        if constexpr (USE == Use::Stats || USE == Use::Grad) {
+            if (at.b0 >= valid) return false;
+            a.begin(p.a, p.a_stride, p.a_first + at.a0, p.vocab, p.a_columns);
+            b.begin(p.b, p.b_stride, at.b0, p.n_pad, p.b_columns);
+        } else if constexpr (USE == Use::GradX) {
+            if (at.b0 >= valid || at.a0 >= p.a_columns) return false;
+            k_begin = static_cast<uint64_t>(p.k_tiles) * at.split / p.splits;
+            k_end = static_cast<uint64_t>(p.k_tiles) * (at.split + 1) / p.splits;
+            a.begin(p.a, p.a_stride, at.a0, p.a_columns, p.vocab - p.a_first);
+            b.begin(p.b, p.b_stride, at.b0, p.n_pad, p.b_columns);
+        } else {
+            if (at.b0 >= p.b_count || at.a0 >= p.a_count) return false;
+            k_end = (valid + S::OpA::kDepth - 1) / S::OpA::kDepth;
+            a.begin(p.a, p.a_stride, at.a0, p.a_columns, p.n_pad);
+            b.begin(p.b, p.b_stride, at.b0, p.b_columns, p.n_pad);
+        }
+        return true;
     }
-    if (USE == Use::GradW) k_end = (meta.valid + OpA::kDepth - 1) / OpA::kDepth;
-
-    OpA a;
-    OpB b;
-    if constexpr (USE == Use::Stats || USE == Use::Grad) {
-        a.begin(p.a, p.a_stride, p.a_first + a0, p.vocab, p.a_columns);
-        b.begin(p.b, p.b_stride, b0, p.n_pad, p.b_columns);
-    } else if constexpr (USE == Use::GradX) {
-        a.begin(p.a, p.a_stride, a0, p.a_columns, p.vocab - p.a_first);
-        b.begin(p.b, p.b_stride, b0, p.n_pad, p.b_columns);
-    } else {
-        a.begin(p.a, p.a_stride, a0, p.a_columns, p.n_pad);
-        b.begin(p.b, p.b_stride, b0, p.b_columns, p.n_pad);
-    }
-
-    const uint32_t wave = threadIdx.x / kWave, wa = wave % WA, wb = wave / WA, lane = threadIdx.x % kWave;
-    const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(ring));
-    const uint32_t a_place = OpA::place(wa * TA * 32), b_place = OpB::place(wb * TB * 32);
-    constexpr uint32_t kTransfers = OpA::kPerWave + OpB::kPerWave;
-    const auto fetch = [&](uint32_t kt) {
-        char* stage = ring + (kt - k_begin) % S::kStages * S::kStage;
+    __device__ __forceinline__ void fetch(uint32_t kt, const char* ring) const {
+        const char* stage = ring + (kt - k_begin) % S::kStages * S::kStage;
         a.fetch(kt, stage);
-        b.fetch(kt, stage + OpA::kBytes);
-    };
+        b.fetch(kt, stage + S::OpA::kBytes);
+    }
+    __device__ __forceinline__ void ahead(const char* ring) const {  // the first k-tiles
+        for (uint32_t kt = k_begin; kt < k_end && kt < k_begin + S::kStages; ++kt) fetch(kt, ring);
+    }
+};
 
-    Acc acc[TA][TB], sums[PARTS == 2 ? TA : 1][PARTS == 2 ? TB : 1];
+// Every wave's LDS reads so far and, of its transfers, all but the last `kLater` are done.
+template <int kLater>
+__device__ __forceinline__ void meet() {
+    wait_loads<kLater>();
+    asm volatile("" ::: "memory");  // LDS reads stay on their side
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// The sums of a tile whose first k-tiles are under way. Operands of a step (16 k) are read from LDS while the step before it
+// multiplies; the last step of a k-tile reads the first of the next, behind the barrier that says every wave's transfers
+// of it have landed and every wave has read the last of the k-tile before it, whose stage the transfers of k-tile
+// kt + kStages then take. float32: sums of kChain k-tiles in the MFMA accumulators (whose own sums round downwards), added to
+// others.
+template <typename S>
+__device__ __forceinline__ void accumulate(const Tile<S>& tile, const char* ring, Acc (&sums)[S::TA][S::TB]) {
+    constexpr int PARTS = S::PARTS, TA = S::TA, TB = S::TB, kSteps = 4 / PARTS, kTransfers = static_cast<int>(S::kTransfers);
+    static_assert(kSteps % 2 == 0, "a k-tile's first step always reads into the same registers");
+    const uint32_t wave = threadIdx.x / kWave, lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(ring));
+    const uint32_t a_place = S::OpA::place(wave % S::WA * TA * 32), b_place = S::OpB::place(wave / S::WA * TB * 32);
+    const uint32_t k_begin = tile.k_begin, k_end = tile.k_end;
 #pragma unroll
     for (int i = 0; i < TA; ++i)
 #pragma unroll
-        for (int j = 0; j < TB; ++j) {
-            acc[i][j] = 0.0f;
-            if constexpr (PARTS == 2) sums[i][j] = 0.0f;
-        }
-    // The operands of a step (16 k) are read from LDS while the step before it multiplies; the last step of a k-tile reads
-    // the first of the next, behind the barrier that says every wave's transfers of it have landed and every wave has read
-    // the last of the k-tile before it, whose stage the transfers of k-tile kt + STAGES then take.
+        for (int j = 0; j < TB; ++j) sums[i][j] = 0.0f;
+    if (k_begin >= k_end) return;
+    Acc chain[PARTS == 2 ? TA : 1][PARTS == 2 ? TB : 1];
+    if constexpr (PARTS == 2) {
+#pragma unroll
+        for (int i = 0; i < TA; ++i)
+#pragma unroll
+            for (int j = 0; j < TB; ++j) chain[i][j] = 0.0f;
+    }
+    const auto acc = [&](int i, int j) -> Acc& {
+        if constexpr (PARTS == 2) return chain[i][j];
+        else return sums[i][j];
+    };
     Frag fa[2][TA][PARTS], fb[2][TB][PARTS];
     const auto read = [&](uint32_t kt, int step, int to) {
-        const uint32_t tile_a = lds + (kt - k_begin) % S::kStages * S::kStage, tile_b = tile_a + OpA::kBytes;
+        const uint32_t tile_a = lds + (kt - k_begin) % S::kStages * S::kStage, tile_b = tile_a + S::OpA::kBytes;
 #pragma unroll
         for (int part = 0; part < PARTS; ++part) {
 #pragma unroll
-            for (int i = 0; i < TA; ++i) fa[to][i][part] = OpA::read(tile_a, a_place, i, step, part);
+            for (int i = 0; i < TA; ++i) fa[to][i][part] = S::OpA::read(tile_a, a_place, i, step, part);
 #pragma unroll
-            for (int j = 0; j < TB; ++j) fb[to][j][part] = OpB::read(tile_b, b_place, j, step, part);
+            for (int j = 0; j < TB; ++j) fb[to][j][part] = S::OpB::read(tile_b, b_place, j, step, part);
         }
     };
-    // Waits for k-tile kt's transfers of every wave, of whose later ones up to `later` k-tiles' are in flight.
-    const auto arrive = [&](uint32_t kt, auto later) {
-        constexpr int kLater = decltype(later)::value;
-        if (k_end - kt > static_cast<uint32_t>(kLater)) wait_loads<static_cast<int>(kTransfers) * kLater>();
-        else wait_loads<0>();
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-    };
-    static_assert(kSteps % 2 == 0, "a k-tile's first step always reads into the same registers");
-    for (uint32_t kt = k_begin; kt < k_end && kt < k_begin + S::kStages; ++kt) fetch(kt);
-    if (k_begin < k_end) {
-        arrive(k_begin, std::integral_constant<int, S::kStages - 1>{});
-        read(k_begin, 0, 0);
-    }
+    if (k_end - k_begin >= static_cast<uint32_t>(S::kStages)) meet<kTransfers * (S::kStages - 1)>();
+    else meet<0>();
+    read(k_begin, 0, 0);
     for (uint32_t kt = k_begin; kt < k_end; ++kt) {
 #pragma unroll
         for (int step = 0; step < kSteps; ++step) {
@@ -585,18 +608,19 @@ __global__ __launch_bounds__(WA* WB* kWave) __attribute__((amdgpu_waves_per_eu(2
             if (step + 1 < kSteps) {
                 read(kt, step + 1, 1 - now);
             } else if (kt + 1 < k_end) {
-                arrive(kt + 1, std::integral_constant<int, S::kStages - 2>{});
-                if (kt + S::kStages < k_end) fetch(kt + S::kStages);
+                if (k_end - kt >= static_cast<uint32_t>(S::kStages)) meet<kTransfers * (S::kStages - 2)>();
+                else meet<0>();
+                if (kt + S::kStages < k_end) tile.fetch(kt + S::kStages, ring);
                 read(kt + 1, 0, 1 - now);
             }
 #pragma unroll
             for (int i = 0; i < TA; ++i)
 #pragma unroll
                 for (int j = 0; j < TB; ++j) {
-                    acc[i][j] = multiply<PARTS>(fa[now][i][0], fb[now][j][0], acc[i][j]);
+                    acc(i, j) = multiply<PARTS>(fa[now][i][0], fb[now][j][0], acc(i, j));
                     if constexpr (PARTS == 2) {
-                        acc[i][j] = multiply<PARTS>(fa[now][i][0], fb[now][j][1], acc[i][j]);
-                        acc[i][j] = multiply<PARTS>(fa[now][i][1], fb[now][j][0], acc[i][j]);
+                        acc(i, j) = multiply<PARTS>(fa[now][i][0], fb[now][j][1], acc(i, j));
+                        acc(i, j) = multiply<PARTS>(fa[now][i][1], fb[now][j][0], acc(i, j));
                     }
                 }
         }
@@ -606,16 +630,23 @@ __global__ __launch_bounds__(WA* WB* kWave) __attribute__((amdgpu_waves_per_eu(2
                 for (int i = 0; i < TA; ++i)
 #pragma unroll
                     for (int j = 0; j < TB; ++j) {
-                        sums[i][j] += acc[i][j];
-                        acc[i][j] = 0.0f;
+                        sums[i][j] += chain[i][j];
+                        chain[i][j] = 0.0f;
                     }
             }
         }
     }
+}
 
-    // a lane's results: index b0 + (wb TB + j) 32 + permuted(lane % 32) of B, indexes a0 + (wa TA + i) 32 + 16 (lane / 32)
-    // + 0..15 of A
-    const uint32_t half = lane / 32;
+// What becomes of a tile's sums. A lane's: index b0 + (wb TB + j) 32 + permuted(lane % 32) of B, indexes
+// a0 + (wa TA + i) 32 + 16 (lane / 32) + 0..15 of A. SLICES: the forward's slices of a whole tile, of which a wave of a
+// whole tile fills several (one with its sums, the others empty).
+template <typename S, uint32_t SLICES, int WHOLE_A>
+__device__ __forceinline__ void finish(const Product& p, const Meta& meta, const TileAt& tile, Acc (&sums)[S::TA][S::TB]) {
+    constexpr int PARTS = S::PARTS, WA = S::WA, TA = S::TA, TB = S::TB;
+    constexpr Use USE = S::USE;
+    const uint32_t wave = threadIdx.x / kWave, wa = wave % WA, wb = wave / WA, lane = threadIdx.x % kWave, half = lane / 32;
+    const uint32_t a0 = tile.a0, b0 = tile.b0, split_at = tile.split, a_lane = a0 + wa * TA * 32 + 16 * half;
     float power = 1.0f;
     if constexpr (PARTS == 2) {
         const int ew = lift_of(meta.weight_bits), ex = lift_of(meta.x_bits);
@@ -629,18 +660,10 @@ __global__ __launch_bounds__(WA* WB* kWave) __attribute__((amdgpu_waves_per_eu(2
                     for (int r = 0; r < 16; ++r) sums[i][j][r] = ldexpf(sums[i][j][r], ew + ex);
         }
     }
-    const auto result = [&](int i, int j, int r) -> float {
-        if constexpr (PARTS == 2) return sums[i][j][r];
-        else return acc[i][j][r];
-    };
-    const uint32_t a_lane = a0 + wa * TA * 32 + 16 * half;
-    // the value held for result (i, j, r)
-    const auto at = [&](int i, int j) -> Acc& {
-        if constexpr (PARTS == 2) return sums[i][j];
-        else return acc[i][j];
-    };
+    const auto result = [&](int i, int j, int r) -> float { return sums[i][j][r]; };
     if constexpr (USE == Use::Stats) {
-        const uint32_t slice = ta * WA + wa;
+        constexpr uint32_t kFill = SLICES * S::kA / (WHOLE_A * WA);  // slices a wave fills
+        const uint32_t slice = a0 / WHOLE_A * SLICES + (a0 % WHOLE_A / (WA * TA * 32) * WA + wa) * kFill;
         if (a0 + S::kA > p.vocab) {  // the last vocabulary tile: what lies beyond adds nothing
 #pragma unroll
             for (int i = 0; i < TA; ++i)
@@ -648,7 +671,7 @@ __global__ __launch_bounds__(WA* WB* kWave) __attribute__((amdgpu_waves_per_eu(2
                 for (int r = 0; r < 16; ++r)
                     if (a_lane + i * 32 + r >= p.vocab)
 #pragma unroll
-                        for (int j = 0; j < TB; ++j) at(i, j)[r] = -__builtin_huge_valf();
+                        for (int j = 0; j < TB; ++j) sums[i][j][r] = -__builtin_huge_valf();
         }
 #pragma unroll
         for (int j = 0; j < TB; ++j) {
@@ -667,7 +690,11 @@ __global__ __launch_bounds__(WA* WB* kWave) __attribute__((amdgpu_waves_per_eu(2
                 for (int r = 0; r < 16; ++r) sum += exponential<PARTS>(result(i, j, r) - shift);
             sum += __shfl_xor(sum, 32);
             if (t >= meta.valid) continue;
-            if (half == 0) p.slices[static_cast<uint64_t>(slice) * p.n_pad + t] = make_float2(most, sum);
+            if (half == 0) {
+#pragma unroll
+                for (uint32_t k = 0; k < kFill; ++k)
+                    p.slices[static_cast<uint64_t>(slice + k) * p.n_pad + t] = k == 0 ? make_float2(most, sum) : make_float2(-__builtin_huge_valf(), 0.0f);
+            }
             const uint32_t label = static_cast<uint32_t>(p.labels[t]) - a_lane;  // a label outside: far from every lane
             if (label < TA * 32 && (label & 16) == 0) {
                 float logit = 0.0f;
@@ -766,6 +793,64 @@ __global__ __launch_bounds__(WA* WB* kWave) __attribute__((amdgpu_waves_per_eu(2
                 }
             }
         }
+    }
+}
+
+// Part `part` of tile `index`, alone.
+template <typename S, typename WHOLE, uint32_t SLICES>
+__device__ __forceinline__ void take_part(const Product& p, const Meta& meta, uint32_t live_b, uint32_t index, uint32_t part, const char* ring) {
+    Tile<S> tile;
+    if (!tile.template begin<WHOLE>(p, meta.valid, live_b, index, part)) return;
+    tile.ahead(ring);
+    Acc sums[S::TA][S::TB];
+    accumulate<S>(tile, ring, sums);
+    finish<S, SLICES, WHOLE::kA>(p, meta, tile.at, sums);
+}
+
+// A launch's blocks stay: block b, on XCD b % 8, takes every (blocks / 8)-th tile of the XCD's share and requests a tile's
+// first k-tiles before it finishes the tile before. Tiles that would leave most CUs idle in a last round are cut into halves
+// or quarters, one a block (1 / 2 or 1 / 4 of the whole shape): 788 tiles of 256 blocks take 3.1 rounds, not 4.
+constexpr int kXcds = 8;
+template <int PARTS, Use USE, int WA, int WB, int TA, int TB>
+__global__ __launch_bounds__(WA* WB* kWave) __attribute__((amdgpu_waves_per_eu(2, 2))) void loss_product_kernel(Product p) {
+    constexpr bool kCut = TA % 2 == 0 && TB % 2 == 0;
+    using Whole = Shape<PARTS, USE, WA, WB, TA, TB>;
+    using Half = Shape<PARTS, USE, WA, WB, TA, kCut ? TB / 2 : TB>;
+    using Quarter = Shape<PARTS, USE, WA, WB, kCut ? TA / 2 : TA, kCut ? TB / 2 : TB>;
+    constexpr uint32_t kSlices = kCut ? 2 * WA : WA;
+    constexpr uint32_t kLds = Whole::kLds > Quarter::kLds ? (Whole::kLds > Half::kLds ? Whole::kLds : Half::kLds)
+                                                          : (Quarter::kLds > Half::kLds ? Quarter::kLds : Half::kLds);
+    __shared__ __attribute__((aligned(1024))) char ring[kLds];
+    const Meta meta = *p.meta;
+    const uint32_t live_b = USE == Use::GradW ? p.b_tiles : (meta.valid + Whole::kB - 1) / Whole::kB;
+    const uint64_t tiles = static_cast<uint64_t>(p.a_tiles) * live_b * p.splits;
+    const uint32_t xcd = blockIdx.x % kXcds, local = blockIdx.x / kXcds, blocks = gridDim.x / kXcds;
+    const uint32_t first = static_cast<uint32_t>(tiles * xcd / kXcds), share = static_cast<uint32_t>(tiles * (xcd + 1) / kXcds) - first;
+    const uint32_t rest = share % blocks, pieces = !kCut || rest == 0 || 2 * rest > blocks ? 1 : 4 * rest > blocks ? 2 : 4;
+    const uint32_t whole = pieces == 1 ? share : share - rest;
+    {
+        Tile<Whole> tile;
+        uint32_t index = local;
+        bool live = false;
+        const auto next = [&]() {  // the block's next tile that has results
+            for (live = false; index < whole && !live; index += blocks) live = tile.template begin<Whole>(p, meta.valid, live_b, first + index, 0);
+            if (live) tile.ahead(ring);
+        };
+        next();
+        Acc sums[TA][TB];
+        while (live) {
+            accumulate<Whole>(tile, ring, sums);
+            const TileAt at = tile.at;
+            meet<0>();  // every wave has read its last
+            next();
+            finish<Whole, kSlices, Whole::kA>(p, meta, at, sums);
+        }
+    }
+    if constexpr (kCut) {
+        if (pieces == 1 || local >= pieces * rest) return;
+        const uint32_t index = first + whole + local / pieces, part = local % pieces;
+        if (pieces == 2) take_part<Half, Whole, kSlices>(p, meta, live_b, index, part, ring);
+        else take_part<Quarter, Whole, kSlices>(p, meta, live_b, index, part, ring);
     }
 }
 
@@ -889,7 +974,7 @@ Plan plan_of(int vt, uint32_t n, uint32_t d, uint32_t vocab, bool aligned, bool 
     p.n_pad = padded(n, p.few ? kFewTokens : 256);
     p.width = padded(d, 64 / p.parts);
     p.in_place = p.parts == 1 && d % 8 == 0 && aligned;
-    p.slices = ceil_div(vocab, p.vocab_tile) * (!p.few && p.parts == 1 ? 2 : 4);  // a slice per wave along the vocabulary
+    p.slices = ceil_div(vocab, p.vocab_tile) * (!p.few && p.parts == 2 ? 8 : 4);  // as many as waves of quarter tiles along the vocabulary
     uint64_t at = 0;
     const auto take = [&](uint64_t bytes) {
         const uint64_t here = at;
@@ -930,7 +1015,8 @@ Plan plan_of(int vt, uint32_t n, uint32_t d, uint32_t vocab, bool aligned, bool 
 
 template <int PARTS, Use USE, int WA, int WB, int TA, int TB>
 hipError_t launch_product(const Product& p, hipStream_t stream) {
-    hipLaunchKernelGGL((loss_product_kernel<PARTS, USE, WA, WB, TA, TB>), dim3(p.a_tiles * p.b_tiles * p.splits), dim3(WA * WB * kWave), 0, stream, p);
+    constexpr uint32_t kBlocks = WA * WB == 4 ? 2 * kCus : kCus;  // as many as the CUs hold
+    hipLaunchKernelGGL((loss_product_kernel<PARTS, USE, WA, WB, TA, TB>), dim3(kBlocks), dim3(WA * WB * kWave), 0, stream, p);
     return hipGetLastError();
 }
 
