@@ -43,6 +43,14 @@ __device__ __forceinline__ float grad_factor(const Meta& meta, float scale, bool
     return mean && meta.valid != 0 ? scale / static_cast<float>(meta.valid) : scale;
 }
 
+// An exponential in [0, 1] in 16 bits: the float32 without sign, first exponent bit (both 0) and last 14 bits, to the nearest
+// (2^-10 of it, down to 2^-126).
+__device__ __forceinline__ uint32_t kept_bits(float e) {
+    const uint32_t bits = __float_as_uint(e);
+    return (bits + 0x1fff + (bits >> 14 & 1)) >> 14 & 0xffff;
+}
+__device__ __forceinline__ float kept_value(uint32_t bits) { return __uint_as_float((bits & 0xffff) << 14); }
+__device__ __forceinline__ float half_value(uint32_t bits) { return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(bits))); }
 __device__ __forceinline__ void split(float v, uint16_t& hi, uint16_t& lo) {
     const _Float16 h = static_cast<_Float16>(v);
     const float rest = v - static_cast<float>(h);
@@ -386,7 +394,7 @@ struct Operand {
     }
     // the tile of k-tile kt into LDS
     __device__ __forceinline__ void fetch(uint32_t kt, const char* lds) const {
-        const uint32_t wave = threadIdx.x / kWave;
+        const uint32_t wave = uniform(threadIdx.x / kWave);
         if constexpr (TR) {
             const uint32_t k0 = kt * kDepth;
             const char* from = base + k0 * stride;
@@ -439,14 +447,15 @@ __device__ __forceinline__ float exponential(float v) {
     else return __expf(v);
 }
 
-enum class Use { Stats, Grad, GradX, GradW };
+// Stats: slices' maxima and sums; Keep: those, and the exponentials kept where D belongs; Grad: D.
+enum class Use { Stats, Keep, Grad, GradX, GradW };
 
 // One product of a loss call: which operands, how far they go, and what becomes of the results.
 struct Product {
     const uint16_t *a, *b;
     uint64_t a_stride, b_stride;  // 16-bit entries from one memory row to the next
     uint32_t a_columns, b_columns;  // entries of a memory row: the weight's d in place, padded widths else
-    uint32_t a_first;             // Stats, Grad: first vocabulary row of the piece
+    uint32_t a_first;             // first vocabulary row of the piece
     uint32_t a_count, b_count;    // GradX, GradW: columns of the output; GradW: its rows
     uint32_t vocab;
     uint32_t k_tiles;             // all (GradX: of the piece)
@@ -454,9 +463,10 @@ struct Product {
     const Meta* meta;
     const int32_t* labels;        // compact
     const float* lse;             // Grad, compact
-    float* picked;                // Stats: the label's logit, compact
-    float2* slices;               // Stats: [slice][n_pad] maximum and sum of exponentials
-    uint16_t* grad;               // Grad: D, [n_pad][piece]
+    float* picked;                // Stats, Keep: the label's logit, compact
+    float2* slices;               // Stats, Keep: [slice][n_pad] maximum and sum of exponentials
+    uint32_t slice_first;         // the piece's first
+    uint16_t* grad;               // Grad: D, [n_pad][piece]; Keep: the exponentials
     uint64_t grad_stride;
     uint32_t n_pad;
     float* partial;               // GradX: [split][n_pad][d]
@@ -513,7 +523,7 @@ struct Tile {
     template <typename WHOLE>
     __device__ __forceinline__ bool begin(const Product& p, uint32_t valid, uint32_t live_b, uint32_t index, uint32_t part) {
         constexpr Use USE = S::USE;
-        constexpr bool kTokensFirst = USE == Use::Stats || USE == Use::Grad;
+        constexpr bool kTokensFirst = USE == Use::Stats || USE == Use::Keep || USE == Use::Grad;
         const uint32_t per_split = p.a_tiles * live_b;
         at.split = index / per_split;
         const TilePlace tile = tile_place(index % per_split, kTokensFirst ? live_b : p.a_tiles, kTokensFirst ? p.a_tiles : live_b);
@@ -522,7 +532,7 @@ struct Tile {
         at.b0 = (kTokensFirst ? tile.inner : tile.outer) * WHOLE::kB + part / kPartsA * S::kB;
         k_begin = 0;
         k_end = p.k_tiles;
-        if constexpr (USE == Use::Stats || USE == Use::Grad) {
+        if constexpr (kTokensFirst) {
             if (at.b0 >= valid) return false;
             a.begin(p.a, p.a_stride, p.a_first + at.a0, p.vocab, p.a_columns);
             b.begin(p.b, p.b_stride, at.b0, p.n_pad, p.b_columns);
@@ -651,7 +661,7 @@ __device__ __forceinline__ void finish(const Product& p, const Meta& meta, const
     if constexpr (PARTS == 2) {
         const int ew = lift_of(meta.weight_bits), ex = lift_of(meta.x_bits);
         power = ldexpf(1.0f, USE == Use::GradX ? ew - kGradLift : USE == Use::GradW ? ex - kGradLift : 0);
-        if constexpr (USE == Use::Stats || USE == Use::Grad) {
+        if constexpr (USE == Use::Stats || USE == Use::Keep || USE == Use::Grad) {
 #pragma unroll
             for (int i = 0; i < TA; ++i)
 #pragma unroll
@@ -661,21 +671,32 @@ __device__ __forceinline__ void finish(const Product& p, const Meta& meta, const
         }
     }
     const auto result = [&](int i, int j, int r) -> float { return sums[i][j][r]; };
-    if constexpr (USE == Use::Stats) {
+    // 16 consecutive 16-bit entries of a lane (float32: hi and lo) into row t of D, from its block i on
+    const auto store = [&](uint32_t t, int i, const uint32_t (&hi)[8], const uint32_t (&lo)[8]) {
+        uint16_t* to = p.grad + t * p.grad_stride + (a_lane - 16 * half + i * 32) * PARTS + 16 * half;
+        *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(to + 8) = make_uint4(hi[4], hi[5], hi[6], hi[7]);
+        if constexpr (PARTS == 2) {
+            *reinterpret_cast<uint4*>(to + 32) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            *reinterpret_cast<uint4*>(to + 40) = make_uint4(lo[4], lo[5], lo[6], lo[7]);
+        }
+    };
+    if constexpr (USE == Use::Stats || USE == Use::Keep) {
         constexpr uint32_t kFill = SLICES * S::kA / (WHOLE_A * WA);  // slices a wave fills
-        const uint32_t slice = a0 / WHOLE_A * SLICES + (a0 % WHOLE_A / (WA * TA * 32) * WA + wa) * kFill;
-        if (a0 + S::kA > p.vocab) {  // the last vocabulary tile: what lies beyond adds nothing
+        const uint32_t slice = p.slice_first + a0 / WHOLE_A * SLICES + (a0 % WHOLE_A / (WA * TA * 32) * WA + wa) * kFill;
+        const uint32_t first = p.a_first + a_lane;  // vocabulary row of the lane's first result
+        if (p.a_first + a0 + S::kA > p.vocab) {     // the last vocabulary tile: what lies beyond adds nothing
 #pragma unroll
             for (int i = 0; i < TA; ++i)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    if (a_lane + i * 32 + r >= p.vocab)
+                    if (first + i * 32 + r >= p.vocab)
 #pragma unroll
-                        for (int j = 0; j < TB; ++j) sums[i][j][r] = -__builtin_huge_valf();
+                        for (int j = 0; j < S::TB; ++j) sums[i][j][r] = -__builtin_huge_valf();
         }
 #pragma unroll
-        for (int j = 0; j < TB; ++j) {
-            const uint32_t t = b0 + (wb * TB + j) * 32 + permuted(lane % 32);
+        for (int j = 0; j < S::TB; ++j) {
+            const uint32_t t = b0 + (wb * S::TB + j) * 32 + permuted(lane % 32);
             float most = -__builtin_huge_valf();
 #pragma unroll
             for (int i = 0; i < TA; ++i)
@@ -684,18 +705,7 @@ __device__ __forceinline__ void finish(const Product& p, const Meta& meta, const
             most = fmaxf(most, __shfl_xor(most, 32));
             const float shift = most == -__builtin_huge_valf() ? 0.0f : most;
             float sum = 0.0f;
-#pragma unroll
-            for (int i = 0; i < TA; ++i)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) sum += exponential<PARTS>(result(i, j, r) - shift);
-            sum += __shfl_xor(sum, 32);
-            if (t >= meta.valid) continue;
-            if (half == 0) {
-#pragma unroll
-                for (uint32_t k = 0; k < kFill; ++k)
-                    p.slices[static_cast<uint64_t>(slice + k) * p.n_pad + t] = k == 0 ? make_float2(most, sum) : make_float2(-__builtin_huge_valf(), 0.0f);
-            }
-            const uint32_t label = static_cast<uint32_t>(p.labels[t]) - a_lane;  // a label outside: far from every lane
+            const uint32_t label = t < meta.valid ? static_cast<uint32_t>(p.labels[t]) - first : 0xffffffffu;  // outside: far from every lane
             if (label < TA * 32 && (label & 16) == 0) {
                 float logit = 0.0f;
 #pragma unroll
@@ -704,6 +714,31 @@ __device__ __forceinline__ void finish(const Product& p, const Meta& meta, const
                     for (int r = 0; r < 16; ++r) logit = label == static_cast<uint32_t>(i * 32 + r) ? result(i, j, r) : logit;
                 p.picked[t] = logit;
             }
+#pragma unroll
+            for (int i = 0; i < TA; ++i) {
+                uint32_t hi[8], lo[8];
+#pragma unroll
+                for (int r = 0; r < 16; r += 2) {
+                    const float e[2] = {exponential<PARTS>(result(i, j, r) - shift), exponential<PARTS>(result(i, j, r + 1) - shift)};
+                    sum += e[0];
+                    sum += e[1];
+                    if constexpr (USE == Use::Keep && PARTS == 1) {
+                        hi[r / 2] = kept_bits(e[0]) | kept_bits(e[1]) << 16;
+                    } else if constexpr (USE == Use::Keep) {
+                        uint16_t h[2], l[2];
+                        split(e[0] * (1 << kGradLift), h[0], l[0]);
+                        split(e[1] * (1 << kGradLift), h[1], l[1]);
+                        hi[r / 2] = h[0] | static_cast<uint32_t>(h[1]) << 16;
+                        lo[r / 2] = l[0] | static_cast<uint32_t>(l[1]) << 16;
+                    }
+                }
+                if constexpr (USE == Use::Keep)
+                    if (t < meta.valid) store(t, i, hi, lo);
+            }
+            sum += __shfl_xor(sum, 32);
+            if (t >= meta.valid || half != 0) continue;
+#pragma unroll
+            for (uint32_t k = 0; k < kFill; ++k) p.slices[static_cast<uint64_t>(slice + k) * p.n_pad + t] = make_float2(most, k == 0 ? sum : 0.0f);
         }
     } else if constexpr (USE == Use::Grad) {
 #pragma unroll
@@ -734,13 +769,7 @@ __device__ __forceinline__ void finish(const Product& p, const Meta& meta, const
                         lo[r / 2] = l[0] | static_cast<uint32_t>(l[1]) << 16;
                     }
                 }
-                uint16_t* to = p.grad + t * p.grad_stride + (a_lane - 16 * half + i * 32) * PARTS + 16 * half;
-                *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                *reinterpret_cast<uint4*>(to + 8) = make_uint4(hi[4], hi[5], hi[6], hi[7]);
-                if constexpr (PARTS == 2) {
-                    *reinterpret_cast<uint4*>(to + 32) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                    *reinterpret_cast<uint4*>(to + 40) = make_uint4(lo[4], lo[5], lo[6], lo[7]);
-                }
+                store(t, i, hi, lo);
             }
         }
     } else {
@@ -889,6 +918,55 @@ __global__ __launch_bounds__(kLseThreads) void loss_lse_kernel(const float2* __r
     losses[rows[t]] = labels[t] < 0 ? __uint_as_float(0x7fc00000u) : value - picked[t];
 }
 
+// The kept exponentials of a piece, taken against their slice's maximum m, turned into D in place: e exp(m - lse) - onehot;
+// zero rows from the counted tokens to the next multiple of 64. bfloat16 calls keep them to 2^-10 (kept_bits; D is then rounded
+// to 2^-8), float32 ones as hi + lo. A block per row and kTurnThreads groups of 8 entries. For a piece that fits, this and the
+// stores take less than its logits again: 2048 tokens of 1024 x 50304 bfloat16 75 + 25 against 283 us, 512 float32 40 + 5
+// against 222 us.
+constexpr uint32_t kTurnThreads = 256;
+template <int PARTS>
+__global__ __launch_bounds__(kTurnThreads) void loss_turn_kernel(uint16_t* __restrict__ grad, uint64_t stride, uint32_t first, uint32_t count, uint32_t across,
+                                                                const float2* __restrict__ slices, uint32_t slice_rows, uint32_t n_pad,
+                                                                const float* __restrict__ lse, const int32_t* __restrict__ labels,
+                                                                const Meta* __restrict__ meta) {
+    const uint32_t t = blockIdx.x / across, valid = meta->valid, c = (blockIdx.x % across * kTurnThreads + threadIdx.x) * 8;
+    if (t >= (valid + 63) / 64 * 64 || c >= count) return;
+    uint4* const at = reinterpret_cast<uint4*>(grad + t * stride + (PARTS == 2 ? c / 32 * 64 + c % 32 : c));
+    uint4* const low = at + 4;  // the lo halves
+    if (t >= valid) {
+        *at = make_uint4(0, 0, 0, 0);
+        if constexpr (PARTS == 2) *low = make_uint4(0, 0, 0, 0);
+        return;
+    }
+    const float most = slices[static_cast<uint64_t>(c / slice_rows) * n_pad + t].x;
+    const float factor = exponential<2>(most - lse[t]) * (PARTS == 2 ? 1.0f / (1 << kGradLift) : 1.0f);
+    const uint32_t label = static_cast<uint32_t>(labels[t]) - first - c;
+    const uint4 kept = *at, rest = PARTS == 2 ? *low : make_uint4(0, 0, 0, 0);
+    const uint32_t hi[4] = {kept.x, kept.y, kept.z, kept.w}, lo[4] = {rest.x, rest.y, rest.z, rest.w};
+    float v[8];
+#pragma unroll
+    for (uint32_t k = 0; k < 8; ++k) {
+        const uint32_t shift = 16 * (k % 2);
+        const float e = PARTS == 1 ? kept_value(hi[k / 2] >> shift) : half_value(hi[k / 2] >> shift) + half_value(lo[k / 2] >> shift);
+        v[k] = e * factor - (label == k ? 1.0f : 0.0f);
+    }
+    if constexpr (PARTS == 1) {
+        *at = make_uint4(bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]), bf16_pair(v[4], v[5]), bf16_pair(v[6], v[7]));
+    } else {
+        uint32_t h[4], l[4];
+#pragma unroll
+        for (uint32_t k = 0; k < 8; k += 2) {
+            uint16_t a[2], b[2];
+            split(v[k] * (1 << kGradLift), a[0], b[0]);
+            split(v[k + 1] * (1 << kGradLift), a[1], b[1]);
+            h[k / 2] = a[0] | static_cast<uint32_t>(a[1]) << 16;
+            l[k / 2] = b[0] | static_cast<uint32_t>(b[1]) << 16;
+        }
+        *at = make_uint4(h[0], h[1], h[2], h[3]);
+        *low = make_uint4(l[0], l[1], l[2], l[3]);
+    }
+}
+
 // gx of every token: the splits' sums in order times the factor; zeros for tokens that do not count. A wave per token,
 // four entries a lane and step (the partials' rows are padded to whole steps' quarters). The last block: the loss, the
 // tokens' losses added in a fixed order.
@@ -959,7 +1037,7 @@ uint32_t ceil_div(uint64_t a, uint32_t b) { return static_cast<uint32_t>((a + b 
 uint32_t padded(uint32_t v, uint32_t to) { return ceil_div(v, to) * to; }
 
 struct Plan {
-    uint32_t parts, n_pad, width, vocab_tile, token_tile, slices, piece, pieces, splits;
+    uint32_t parts, n_pad, width, vocab_tile, token_tile, per_tile, slices, piece, pieces, splits;
     bool few, in_place;
     uint64_t meta, rows, labels, place, lse, picked, losses, slice_sums, x_most, w_most, x, weight, grad, partial, bytes;
 };
@@ -974,7 +1052,8 @@ Plan plan_of(int vt, uint32_t n, uint32_t d, uint32_t vocab, bool aligned, bool 
     p.n_pad = padded(n, p.few ? kFewTokens : 256);
     p.width = padded(d, 64 / p.parts);
     p.in_place = p.parts == 1 && d % 8 == 0 && aligned;
-    p.slices = ceil_div(vocab, p.vocab_tile) * (!p.few && p.parts == 2 ? 8 : 4);  // as many as waves of quarter tiles along the vocabulary
+    p.per_tile = !p.few && p.parts == 2 ? 8 : 4;  // slices: as many as waves of quarter tiles along the vocabulary
+    p.slices = padded(vocab, kTile) / p.vocab_tile * p.per_tile;
     uint64_t at = 0;
     const auto take = [&](uint64_t bytes) {
         const uint64_t here = at;
@@ -1078,24 +1157,53 @@ hipError_t run(const LossCall& c, hipStream_t stream) {
     stats.b_stride = x_row;
     stats.b_columns = plan.width;
     stats.k_tiles = plan.width / depth;
-    stats.a_tiles = ceil_div(c.vocab, plan.vocab_tile);
+    stats.a_tiles = padded(c.vocab, kTile) / plan.vocab_tile;
     stats.b_tiles = token_tiles;
     stats.picked = picked;
     stats.slices = reinterpret_cast<float2*>(work + plan.slice_sums);
-    if ((status = product<Use::Stats>(plan, stats, stream)) != hipSuccess) return status;
-    if (plan.few) hipLaunchKernelGGL(loss_lse_kernel<1>, dim3(c.n), dim3(kLseThreads), 0, stream, stats.slices, plan.slices, plan.n_pad, picked, rows, labels, meta, lse, losses);
-    else hipLaunchKernelGGL(loss_lse_kernel<16>, dim3(ceil_div(c.n, 16)), dim3(kLseThreads), 0, stream, stats.slices, plan.slices, plan.n_pad, picked, rows, labels, meta, lse, losses);
+    // The last piece's exponentials stay where its D belongs. Not those of a few bfloat16 tokens, whose products wait for the
+    // weight and whose gradients may come from a single entry of D: it is rounded once.
+    const bool keeps = gradients && (plan.parts == 2 || !plan.few);
+    const uint32_t last = keeps ? (plan.pieces - 1) * plan.piece : c.vocab;
+    Product keep = stats;
+    if (keeps) {
+        keep.a_first = last;
+        keep.a_tiles = padded(c.vocab - last, kTile) / plan.vocab_tile;
+        keep.slice_first = last / plan.vocab_tile * plan.per_tile;
+        stats.a_tiles = last / plan.vocab_tile;
+    }
+    keep.grad = reinterpret_cast<uint16_t*>(work + plan.grad);
+    keep.grad_stride = static_cast<uint64_t>(plan.piece) * plan.parts;
+    if (stats.a_tiles != 0 && (status = product<Use::Stats>(plan, stats, stream)) != hipSuccess) return status;
+    if (keeps && (status = product<Use::Keep>(plan, keep, stream)) != hipSuccess) return status;
+    const auto lse_of = [&](auto tokens) {
+        constexpr uint32_t kTokens = decltype(tokens)::value;
+        hipLaunchKernelGGL(loss_lse_kernel<kTokens>, dim3(ceil_div(c.n, kTokens)), dim3(kLseThreads), 0, stream, stats.slices, plan.slices, plan.n_pad,
+                           picked, rows, labels, meta, lse, losses);
+    };
+    // tokens a block: one where few are all there are, more where that still fills the CUs (runs of 128 bytes of a slice; 8192
+    // tokens: 15 us, in fours 46; 512 float32 tokens in fours 10 us, in sixteens 16)
+    if (plan.few) lse_of(std::integral_constant<uint32_t, 1>{});
+    else if (c.n < 1024) lse_of(std::integral_constant<uint32_t, 4>{});
+    else lse_of(std::integral_constant<uint32_t, 16>{});
     if (failed(status)) return status;
     if (!gradients) return hipSuccess;
 
-    for (uint32_t first = 0; first < c.vocab; first += plan.piece) {
-        const uint32_t count = c.vocab - first < plan.piece ? c.vocab - first : plan.piece;
-        Product grad = stats;
-        grad.a_first = first;
-        grad.a_tiles = ceil_div(padded(count, kTile), plan.vocab_tile);
-        grad.grad = reinterpret_cast<uint16_t*>(work + plan.grad);
-        grad.grad_stride = static_cast<uint64_t>(plan.piece) * plan.parts;
-        if ((status = product<Use::Grad>(plan, grad, stream)) != hipSuccess) return status;
+    for (uint32_t piece = plan.pieces; piece-- > 0;) {
+        const uint32_t first = piece * plan.piece, count = c.vocab - first < plan.piece ? c.vocab - first : plan.piece;
+        Product grad = keep;
+        if (first == last) {
+            const uint32_t columns = padded(count, kTile), slice_rows = plan.vocab_tile / plan.per_tile, across = ceil_div(columns, 8 * kTurnThreads);
+            const dim3 grid(across * padded(c.n, 64));
+            const float2* slices = stats.slices + static_cast<uint64_t>(keep.slice_first) * plan.n_pad;
+            if (plan.parts == 1) hipLaunchKernelGGL(loss_turn_kernel<1>, grid, dim3(kTurnThreads), 0, stream, grad.grad, grad.grad_stride, first, columns, across, slices, slice_rows, plan.n_pad, lse, labels, meta);
+            else hipLaunchKernelGGL(loss_turn_kernel<2>, grid, dim3(kTurnThreads), 0, stream, grad.grad, grad.grad_stride, first, columns, across, slices, slice_rows, plan.n_pad, lse, labels, meta);
+            if (failed(status)) return status;
+        } else {
+            grad.a_first = first;
+            grad.a_tiles = padded(count, kTile) / plan.vocab_tile;
+            if ((status = product<Use::Grad>(plan, grad, stream)) != hipSuccess) return status;
+        }
 
         Product gx = p;
         gx.a = weight + first * w_row;
@@ -1112,7 +1220,7 @@ hipError_t run(const LossCall& c, hipStream_t stream) {
         gx.splits = plan.splits;
         gx.partial = reinterpret_cast<float*>(work + plan.partial);
         gx.out_stride = plan.width;
-        gx.add = first != 0;
+        gx.add = piece + 1 != plan.pieces;
         if ((status = product<Use::GradX>(plan, gx, stream)) != hipSuccess) return status;
 
         Product gw = p;
