@@ -56,9 +56,9 @@ SIGNATURES = {
     "hffn_clip_workspace": [_U32, ctypes.POINTER(_U64)],
     "hffn_grad_norm": [_U32, _P, _P, _P, _I, _P, _U64, _P, _P],
     "hffn_clip": [_U32] + [_P] * 5 + [_I, _F64, _P, _U64, _P, _P],
-    "hffn_loss_workspace": [_I, _U32, _U32, _U32, _I, _I, ctypes.POINTER(_U64)],
+    "hffn_loss_workspace": [_I, _U32, _U32, _U32, _I, _I, _U64, ctypes.POINTER(_U64)],
     "hffn_losses": [_I, _P, _U64, _P, _P, _I64, _I, _I64, _P, _P, _U64, _U32, _U32, _U32, _P],
-    "hffn_loss_step": [_I, _P, _U64, _P, _P, _I64, _I, _I64, _I, _F32] + [_P] * 4 + [_U64, _U32, _U32, _U32, _P],
+    "hffn_loss_step": [_I, _P, _U64, _P, _P, _I64, _I, _I64, _I, _F32, _U64] + [_P] * 4 + [_U64, _U32, _U32, _U32, _P],
     "hffn_read_probe": [_P, _U64, _P, _U32, _U32, _P],
     "hffn_output_major_workspace": [_U32, _U32, ctypes.POINTER(_U64)],
     "hffn_output_major": [_I, _P, _P, _P, _U32, _U32, _U32, _P, _P, _P, _P, _U64, _P],

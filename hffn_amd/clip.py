@@ -11,16 +11,18 @@ or permuted dimensions of that). Sums are float64; the result does not depend on
 """
 from __future__ import annotations
 
-import ctypes
+import functools
 import math
+from array import array
 from collections.abc import Iterable
 
 import torch
 
 from . import _lib
-from .runtime import _VALUE_TYPES, _device
+from .runtime import _VALUE_TYPES, _device, current_stream
 
 NORM_TYPES = (2.0, math.inf)
+_CUDA = torch.device("cuda", 0)
 
 
 def _dense(t: torch.Tensor) -> bool:
@@ -35,74 +37,65 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
-class _Arrays:
-    """The host arrays of a call: pointers, entry counts, value types."""
-
-    def __init__(self, tensors: Iterable[torch.Tensor], what: str) -> None:
-        self.tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-        count = len(self.tensors)
-        self.device = self.tensors[0].device if count else torch.device("cuda", 0)
-        types = []
-        for t in self.tensors:
-            kind = _VALUE_TYPES.get(t.dtype)
-            if kind is None or t.device != self.device:
-                raise ValueError(f"{what}: float32 or bfloat16 tensors of one device are required, not {t.dtype} on {t.device}")
+def _table(tensors: Iterable[torch.Tensor], what: str) -> tuple[list, array, array, array, bool]:
+    """(tensors, pointers, entry counts, value types, whether all are contiguous) of a call's tensors, checked."""
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    types = [_VALUE_TYPES.get(t.dtype, -1) for t in tensors]
+    if -1 in types or any([t.get_device() for t in tensors]):
+        raise ValueError(f"{what}: float32 or bfloat16 tensors of one device, cuda:0, are required; found "
+                         + ", ".join(sorted({f"{t.dtype} on {t.device}" for t in tensors})))
+    contiguous = all([t.is_contiguous() for t in tensors])
+    if not contiguous:
+        for t in tensors:
             if not _dense(t):
                 raise ValueError(f"{what}: a tensor of shape {list(t.shape)} and strides {list(t.stride())} does not fill its memory")
-            types.append(kind)
-        at, entries = [t.data_ptr() for t in self.tensors], [t.numel() for t in self.tensors]
-        self.pointers, self.counts = (ctypes.c_void_p * count)(*at), (ctypes.c_uint64 * count)(*entries)
-        self.types = (ctypes.c_int * count)(*types)
-        self.spans = sorted((p, p + n * (2 if kind == _lib.VALUE_BF16 else 4)) for p, n, kind in zip(at, entries, types) if n)
+    return (tensors, array("Q", [t.data_ptr() for t in tensors]), array("Q", [t.numel() for t in tensors]), array("i", types), contiguous)
 
 
-def _check_apart(spans: list, what: str) -> None:
-    for (_, end), (start, _) in zip(spans, spans[1:]):
-        if start < end:
-            raise ValueError(f"{what}: two tensors share memory")
+def _at(values: array) -> int:
+    return values.buffer_info()[0]
 
 
-def _call(tensors: Iterable[torch.Tensor], norm_type: float) -> tuple:
+@functools.lru_cache(maxsize=None)
+def _workspace_floats(count: int) -> int:
+    return _lib.query_bytes(_lib.load().hffn_clip_workspace, count) // 4
+
+
+def _buffers(count: int, norm_type: float) -> tuple:
     if norm_type not in NORM_TYPES:
         raise ValueError(f"norm_type is 2 or inf, not {norm_type!r}")
-    arrays = _Arrays(tensors, "tensors")
-    device = _device(arrays.device)
-    lib = _lib.load()
-    work = torch.empty(_lib.query_bytes(lib.hffn_clip_workspace, len(arrays.tensors)), dtype=torch.uint8, device=device)
-    return arrays, lib, work, torch.empty((), device=device), torch.cuda.current_stream(device).cuda_stream
+    device = _device(None) if count == 0 else _CUDA  # the tensors lie there
+    return torch.empty(_workspace_floats(count), device=device), torch.empty((), device=device), current_stream(device)
 
 
-@torch.no_grad()
 def grad_norm(tensors: Iterable[torch.Tensor], norm_type: float = 2.0) -> torch.Tensor:
     """The 2-norm (or, ``norm_type=inf``, the largest magnitude) over all entries of all tensors: float32 0-d on the device,
     zero for no entries, NaN where an entry is."""
-    arrays, lib, work, norm, stream = _call(tensors, norm_type)
-    _lib.check(lib.hffn_grad_norm(len(arrays.tensors), arrays.pointers, arrays.counts, arrays.types, int(norm_type == math.inf),
-                                  work.data_ptr(), work.numel(), norm.data_ptr(), stream), "gradient norm")
+    tensors, pointers, counts, types, _ = _table(tensors, "tensors")
+    work, norm, stream = _buffers(len(tensors), norm_type)
+    _lib.check(_lib.load().hffn_grad_norm(len(tensors), _at(pointers), _at(counts), _at(types), int(norm_type == math.inf), work.data_ptr(),
+                                          4 * work.numel(), norm.data_ptr(), stream), "gradient norm")
     return norm
 
 
-@torch.no_grad()
 def clip_grad_norm_(tensors: Iterable[torch.Tensor], max_norm: float, norm_type: float = 2.0,
                     out: Iterable[torch.Tensor] | None = None) -> torch.Tensor:
     """``grad_norm`` of the tensors, every entry of which is then scaled by ``min(1, max_norm / (norm + 1e-6))``: in place, or into
-    ``out``, a tensor of the same shape and strides for each (float32 or bfloat16, sharing no memory with any). Returns the norm
-    before scaling. An infinite norm makes the entries zero (infinite ones NaN), a NaN one makes all NaN; ``max_norm=inf``
-    scales nothing while the norm is finite."""
+    ``out``, a tensor of the same shape and strides for each (float32 or bfloat16). No two tensors may share memory. Returns the
+    norm before scaling. An infinite norm makes the entries zero (infinite ones NaN), a NaN one makes all NaN;
+    ``max_norm=inf`` scales nothing while the norm is finite."""
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm={max_norm} must not be negative")
-    arrays, lib, work, norm, stream = _call(tensors, norm_type)
-    spans, into = arrays.spans, None
+    tensors, pointers, counts, types, contiguous = _table(tensors, "tensors")
+    to = (None, None)
     if out is not None:
-        into = _Arrays(out, "out")
-        if len(into.tensors) != len(arrays.tensors) or any(a.shape != b.shape or a.stride() != b.stride() or a.device != b.device
-                                                           for a, b in zip(arrays.tensors, into.tensors)):
-            raise ValueError("out must hold a tensor of the same shape, strides and device for each tensor")
-        _check_apart(sorted(spans + into.spans), "out")
-    else:
-        _check_apart(spans, "tensors")
-    _lib.check(lib.hffn_clip(len(arrays.tensors), arrays.pointers, into and into.pointers, arrays.counts, arrays.types,
-                             into and into.types, int(norm_type == math.inf), max_norm, work.data_ptr(), work.numel(), norm.data_ptr(),
-                             stream), "clip")
+        into, to_pointers, _, to_types, to_contiguous = _table(out, "out")
+        same = [t.shape for t in tensors] == [t.shape for t in into]
+        if not same or not (contiguous and to_contiguous) and [t.stride() for t in tensors] != [t.stride() for t in into]:
+            raise ValueError("out must hold a tensor of the same shape and strides for each tensor")
+        to = (_at(to_pointers), _at(to_types))
+    work, norm, stream = _buffers(len(tensors), norm_type)
+    _lib.check(_lib.load().hffn_clip(len(tensors), _at(pointers), to[0], _at(counts), _at(types), to[1], int(norm_type == math.inf), max_norm,
+                                     work.data_ptr(), 4 * work.numel(), norm.data_ptr(), stream), "clip")
     return norm

@@ -3,6 +3,7 @@
 // entry point replaces, are in include/hffn_amd.h.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
 #include <exception>
@@ -10,6 +11,7 @@
 #include <mutex>
 #include <string>
 #include <unordered_map>
+#include <utility>
 #include <vector>
 
 #include "../../include/hffn_amd.h"
@@ -1046,13 +1048,16 @@ int hffn_clip_workspace(uint32_t arrays, uint64_t* bytes) {
 
 namespace {
 int clip_arrays(uint32_t arrays, const void* const* p, void* const* out, const uint64_t* counts, const int* types, const int* out_types,
-                const void* workspace, uint64_t workspace_bytes, const float* norm, std::vector<hffn::ClipArray>& list, const char* what) {
+                const void* workspace, uint64_t workspace_bytes, const float* norm, bool apart, std::vector<hffn::ClipArray>& list, const char* what) {
     if (!norm || !workspace || (arrays && (!p || !counts || !types))) return fail(HFFN_ERROR_ARGUMENT, "%s: null pointer", what);
     if (reinterpret_cast<uintptr_t>(workspace) % 8 != 0) return fail(HFFN_ERROR_ARGUMENT, "%s: the workspace must be 8-byte aligned", what);
     if (workspace_bytes < hffn::clip_workspace_bytes(arrays))
         return fail(HFFN_ERROR_ARGUMENT, "%s: workspace of %llu bytes, %llu needed", what, static_cast<unsigned long long>(workspace_bytes),
                     static_cast<unsigned long long>(hffn::clip_workspace_bytes(arrays)));
     list.reserve(arrays);
+    std::vector<std::pair<uintptr_t, uintptr_t>> spans;  // of what a clip reads and writes
+    const auto span = [&](const void* at, uint64_t bytes) { spans.push_back({reinterpret_cast<uintptr_t>(at), reinterpret_cast<uintptr_t>(at) + bytes}); };
+    if (apart) spans.reserve(out ? 2 * arrays : arrays);
     for (uint32_t k = 0; k < arrays; ++k) {
         const int to = out ? out_types[k] : types[k];
         if (!valid_value_type(types[k]) || !valid_value_type(to)) return fail(HFFN_ERROR_ARGUMENT, "%s: array %u: unknown value type", what, k);
@@ -1063,7 +1068,12 @@ int clip_arrays(uint32_t arrays, const void* const* p, void* const* out, const u
         if (out)
             if (int status = check_entries(to, {out[k]}, {}, what)) return status;
         list.push_back({p[k], out ? out[k] : const_cast<void*>(p[k]), counts[k], types[k], to});
+        if (apart) span(p[k], counts[k] * (types[k] == HFFN_VALUE_BF16 ? 2 : 4));
+        if (apart && out) span(out[k], counts[k] * (to == HFFN_VALUE_BF16 ? 2 : 4));
     }
+    std::sort(spans.begin(), spans.end());
+    for (size_t k = 1; k < spans.size(); ++k)
+        if (spans[k].first < spans[k - 1].second) return fail(HFFN_ERROR_ARGUMENT, "%s: two arrays share memory", what);
     return HFFN_OK;
 }
 }  // namespace
@@ -1071,7 +1081,7 @@ int clip_arrays(uint32_t arrays, const void* const* p, void* const* out, const u
 int hffn_grad_norm(uint32_t arrays, const void* const* p, const uint64_t* counts, const int* types, int largest, void* workspace,
                    uint64_t workspace_bytes, float* norm, void* stream) try {
     std::vector<hffn::ClipArray> list;
-    if (int status = clip_arrays(arrays, p, nullptr, counts, types, nullptr, workspace, workspace_bytes, norm, list, "grad_norm")) return status;
+    if (int status = clip_arrays(arrays, p, nullptr, counts, types, nullptr, workspace, workspace_bytes, norm, false, list, "grad_norm")) return status;
     return launched(hffn::launch_grad_norm(list.data(), static_cast<uint32_t>(list.size()), largest != 0, static_cast<double*>(workspace), norm,
                                            static_cast<hipStream_t>(stream)),
                     "grad_norm");
@@ -1084,7 +1094,7 @@ int hffn_clip(uint32_t arrays, void* const* p, void* const* out, const uint64_t*
     if (!(limit >= 0.0)) return fail(HFFN_ERROR_ARGUMENT, "clip: the limit must not be negative");
     if (out && !out_types) return fail(HFFN_ERROR_ARGUMENT, "clip: null pointer");
     std::vector<hffn::ClipArray> list;
-    if (int status = clip_arrays(arrays, const_cast<const void* const*>(p), out, counts, types, out_types, workspace, workspace_bytes, norm, list, "clip"))
+    if (int status = clip_arrays(arrays, const_cast<const void* const*>(p), out, counts, types, out_types, workspace, workspace_bytes, norm, true, list, "clip"))
         return status;
     return launched(hffn::launch_clip(list.data(), static_cast<uint32_t>(list.size()), largest != 0, limit, out == nullptr,
                                       static_cast<double*>(workspace), norm, static_cast<hipStream_t>(stream)),
@@ -1109,7 +1119,7 @@ int loss_call(hffn::LossCall& call, uint64_t workspace_bytes, int label_bytes, c
     if (reinterpret_cast<uintptr_t>(call.labels) % label_bytes != 0) return fail(HFFN_ERROR_ARGUMENT, "%s: misaligned labels", what);
     if (int status = check_entries(call.value_type, {call.x, call.weight, call.gx, call.gw}, {call.losses, call.loss}, what)) return status;
     if (reinterpret_cast<uintptr_t>(call.workspace) % 256 != 0) return fail(HFFN_ERROR_ARGUMENT, "%s: the workspace must be 256-byte aligned", what);
-    const uint64_t needed = hffn::loss_workspace_bytes(call.value_type, call.n, call.d, call.vocab, reinterpret_cast<uintptr_t>(call.weight) % 16 == 0, call.gw != nullptr);
+    const uint64_t needed = hffn::loss_workspace_bytes(call.value_type, call.n, call.d, call.vocab, reinterpret_cast<uintptr_t>(call.weight) % 16 == 0, call.gw != nullptr, call.piece_bytes);
     if (workspace_bytes < needed)
         return fail(HFFN_ERROR_ARGUMENT, "%s: workspace of %llu bytes, %llu needed", what, static_cast<unsigned long long>(workspace_bytes),
                     static_cast<unsigned long long>(needed));
@@ -1118,10 +1128,11 @@ int loss_call(hffn::LossCall& call, uint64_t workspace_bytes, int label_bytes, c
 }
 }  // namespace
 
-int hffn_loss_workspace(int value_type, uint32_t n, uint32_t d_model, uint32_t vocab, int aligned, int gradients, uint64_t* bytes) {
+int hffn_loss_workspace(int value_type, uint32_t n, uint32_t d_model, uint32_t vocab, int aligned, int gradients, uint64_t piece_bytes,
+                        uint64_t* bytes) {
     if (!bytes) return fail(HFFN_ERROR_ARGUMENT, "loss_workspace: null pointer");
     if (int status = check_loss(value_type, n, d_model, vocab, "loss_workspace")) return status;
-    *bytes = hffn::loss_workspace_bytes(value_type, n, d_model, vocab, aligned != 0, gradients != 0);
+    *bytes = hffn::loss_workspace_bytes(value_type, n, d_model, vocab, aligned != 0, gradients != 0, piece_bytes);
     return HFFN_OK;
 }
 
@@ -1130,17 +1141,17 @@ int hffn_losses(int value_type, const void* x, uint64_t x_stride, const void* we
                 void* stream) {
     if (!losses) return fail(HFFN_ERROR_ARGUMENT, "losses: null pointer");
     hffn::LossCall call{x, weight, labels, x_stride, labels_stride, ignore_index, false, false, 1.0f, losses, nullptr, nullptr, nullptr, workspace,
-                        value_type, n, d_model, vocab};
+                        0, value_type, n, d_model, vocab};
     if (int status = loss_call(call, workspace_bytes, label_bytes, "losses")) return status;
     return launched(hffn::launch_loss(call, static_cast<hipStream_t>(stream)), "losses");
 }
 
 int hffn_loss_step(int value_type, const void* x, uint64_t x_stride, const void* weight, const void* labels, int64_t labels_stride, int label_bytes,
-                   int64_t ignore_index, int mean, float scale, float* loss, void* gx, void* gw, void* workspace, uint64_t workspace_bytes,
-                   uint32_t d_model, uint32_t vocab, uint32_t n, void* stream) {
+                   int64_t ignore_index, int mean, float scale, uint64_t piece_bytes, float* loss, void* gx, void* gw, void* workspace,
+                   uint64_t workspace_bytes, uint32_t d_model, uint32_t vocab, uint32_t n, void* stream) {
     if (!loss || !gx || !gw) return fail(HFFN_ERROR_ARGUMENT, "loss_step: null pointer");
     hffn::LossCall call{x, weight, labels, x_stride, labels_stride, ignore_index, false, mean != 0, scale, nullptr, loss, gx, gw, workspace,
-                        value_type, n, d_model, vocab};
+                        piece_bytes, value_type, n, d_model, vocab};
     if (int status = loss_call(call, workspace_bytes, label_bytes, "loss_step")) return status;
     return launched(hffn::launch_loss(call, static_cast<hipStream_t>(stream)), "loss_step");
 }

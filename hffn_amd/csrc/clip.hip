@@ -1,6 +1,8 @@
 // The global norm over many tensors and the clipping of their entries to it: two launches per table of kClipArrays arrays.
 // The first leaves one float64 partial per block; every block of the second adds the partials up again (8 KB a table out
 // of L2), so that no block waits for another, and scales its share.
+#include <vector>
+
 #include "common.hpp"
 #include "launch.hpp"
 
@@ -153,7 +155,10 @@ __device__ __forceinline__ void scale_chunk(const T* p, U* out, uint64_t count, 
             U* to = out + before + i * V;
             if constexpr (sizeof(U) == 4) {
 #pragma unroll
-                for (uint32_t k = 0; k < V; k += 4) *reinterpret_cast<float4*>(to + k) = make_float4(w[k], w[k + 1], w[k + 2], w[k + 3]);
+                for (uint32_t k = 0; k < V; k += 4) {
+                    typedef float Four __attribute__((ext_vector_type(4)));
+                    __builtin_nontemporal_store((Four{w[k], w[k + 1], w[k + 2], w[k + 3]}), reinterpret_cast<Four*>(to + k));
+                }
             } else {
 #pragma unroll
                 for (uint32_t k = 0; k < V; k += 4)
@@ -164,7 +169,7 @@ __device__ __forceinline__ void scale_chunk(const T* p, U* out, uint64_t count, 
     for (uint32_t i = before + pieces * V + threadIdx.x; i < all; i += kThreads) put(out + i, factor * widen(p[i]));
 }
 
-// The arrays of one table scaled; `count` partials are all tables'. In place with a factor of one nothing is written:
+// The arrays of one table scaled, last entries first: they were read last and lie in the caches. `count` partials are all tables'. In place with a factor of one nothing is written:
 // every entry would be itself.
 template <bool LARGEST>
 __global__ __launch_bounds__(kThreads) void clip_kernel(Table table, const double* __restrict__ partials, uint32_t count, double limit,
@@ -175,8 +180,9 @@ __global__ __launch_bounds__(kThreads) void clip_kernel(Table table, const doubl
     const double quotient = limit / (value + 1e-6);
     const float factor = quotient >= 1.0 ? 1.0f : static_cast<float>(quotient);  // a NaN norm makes every entry NaN
     if (in_place && factor == 1.0f) return;
-    for (uint32_t chunk = blockIdx.x; chunk < table.first[table.arrays]; chunk += gridDim.x) {
-        const uint32_t which = array_of(table, chunk);
+    const uint32_t chunks = table.first[table.arrays];
+    for (uint32_t turn = blockIdx.x; turn < chunks; turn += gridDim.x) {
+        const uint32_t chunk = chunks - 1 - turn, which = array_of(table, chunk);
         const uint64_t start = (chunk - table.first[which]) * kChunk, left = table.count[which] - start, n = left < kChunk ? left : kChunk;
         const float* p = static_cast<const float*>(table.p[which]) + start;
         const uint16_t* q = static_cast<const uint16_t*>(table.p[which]) + start;
@@ -238,7 +244,13 @@ hipError_t norm_and_clip(const ClipArray* arrays, uint32_t count, bool clip, dou
         return hipGetLastError();
     }
     Table table;
+    std::vector<uint32_t> starts;  // the tables' first arrays
     for (uint32_t next = 0; next < count;) {
+        starts.push_back(next);
+        fill(table, arrays, count, &next);
+    }
+    for (size_t k = starts.size(); k-- > 0;) {
+        uint32_t next = starts[k];
         const uint32_t chunks = fill(table, arrays, count, &next);
         if (chunks == 0) continue;
         const uint32_t blocks = chunks < 2 * kClipPartials ? chunks : 2 * kClipPartials;

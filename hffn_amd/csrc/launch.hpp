@@ -287,10 +287,12 @@ struct LossCall {
     float scale;
     float *losses, *loss;
     void *gx, *gw, *workspace;
+    uint64_t piece_bytes;  // a piece's D at most (a vocabulary tile's at least); 0: kLossPieceBytes
     int value_type;
     uint32_t n, d, vocab;
 };
-uint64_t loss_workspace_bytes(int vt, uint32_t n, uint32_t d, uint32_t vocab, bool aligned, bool gradients);
+constexpr uint64_t kLossPieceBytes = 512ull << 20;
+uint64_t loss_workspace_bytes(int vt, uint32_t n, uint32_t d, uint32_t vocab, bool aligned, bool gradients, uint64_t piece_bytes);
 hipError_t launch_loss(const LossCall& call, hipStream_t stream);
 
 // probe.hip

@@ -1030,7 +1030,6 @@ __global__ __launch_bounds__(kFinishThreads) void loss_finish_kernel(const float
 
 constexpr uint32_t kTile = 256;                // vocabulary rows and width of a tile
 constexpr uint32_t kFewTokens = 64, kFewTile = 128;  // up to so many tokens: tiles of 128 x 64, two blocks a CU
-constexpr uint64_t kGradBytes = 256ull << 20;  // a piece's D at most (or one vocabulary tile's)
 constexpr uint32_t kCus = 256;
 
 uint32_t ceil_div(uint64_t a, uint32_t b) { return static_cast<uint32_t>((a + b - 1) / b); }
@@ -1043,7 +1042,7 @@ struct Plan {
 };
 
 // `aligned`: the weight starts on a 16-byte boundary (bfloat16 weights of whole 16-byte pieces are then read in place).
-Plan plan_of(int vt, uint32_t n, uint32_t d, uint32_t vocab, bool aligned, bool gradients) {
+Plan plan_of(int vt, uint32_t n, uint32_t d, uint32_t vocab, bool aligned, bool gradients, uint64_t piece_bytes) {
     Plan p{};
     p.parts = vt == kBF16 ? 1 : 2;
     p.few = n <= kFewTokens;
@@ -1076,7 +1075,7 @@ Plan plan_of(int vt, uint32_t n, uint32_t d, uint32_t vocab, bool aligned, bool 
     p.weight = p.in_place ? 0 : take(2ull * p.parts * vocab * p.width);
     if (gradients) {
         const uint64_t per_row = 2ull * p.parts * p.n_pad;
-        const uint64_t most = kGradBytes / (per_row * kTile);
+        const uint64_t most = (piece_bytes == 0 ? kLossPieceBytes : piece_bytes) / (per_row * kTile);
         const uint32_t tiles = ceil_div(vocab, kTile), fit = most < 1 ? 1 : most < tiles ? static_cast<uint32_t>(most) : tiles;
         p.pieces = ceil_div(tiles, fit);
         p.piece = ceil_div(tiles, p.pieces) * kTile;
@@ -1109,7 +1108,7 @@ hipError_t product(const Plan& plan, const Product& p, hipStream_t stream) {
 template <typename T>
 hipError_t run(const LossCall& c, hipStream_t stream) {
     const bool gradients = c.gw != nullptr;
-    const Plan plan = plan_of(c.value_type, c.n, c.d, c.vocab, reinterpret_cast<uintptr_t>(c.weight) % 16 == 0, gradients);
+    const Plan plan = plan_of(c.value_type, c.n, c.d, c.vocab, reinterpret_cast<uintptr_t>(c.weight) % 16 == 0, gradients, c.piece_bytes);
     char* const work = static_cast<char*>(c.workspace);
     Meta* const meta = reinterpret_cast<Meta*>(work + plan.meta);
     int32_t *const rows = reinterpret_cast<int32_t*>(work + plan.rows), *const labels = reinterpret_cast<int32_t*>(work + plan.labels),
@@ -1248,8 +1247,8 @@ hipError_t run(const LossCall& c, hipStream_t stream) {
 
 }  // namespace
 
-uint64_t loss_workspace_bytes(int vt, uint32_t n, uint32_t d, uint32_t vocab, bool aligned, bool gradients) {
-    return plan_of(vt, n, d, vocab, aligned, gradients).bytes;
+uint64_t loss_workspace_bytes(int vt, uint32_t n, uint32_t d, uint32_t vocab, bool aligned, bool gradients, uint64_t piece_bytes) {
+    return plan_of(vt, n, d, vocab, aligned, gradients, piece_bytes).bytes;
 }
 
 hipError_t launch_loss(const LossCall& call, hipStream_t stream) {

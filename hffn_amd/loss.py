@@ -3,7 +3,8 @@ mean loss with the gradients of the hidden rows and of the head's weight (a trai
 
 For hidden rows ``x [N, d]``, a weight ``[V, d]`` and labels: ``l_t = log sum_v exp(x_t . w_v) - x_t . w_label(t)``; with
 ``p = softmax(x W^T)`` and ``D = (p - onehot) / counted``: ``gx = D W``, ``gw = D^T x``. Logits are computed in pieces of the
-vocabulary, once for the sums of exponentials and once more for the gradients; no [N, V] array is kept. Tokens whose label
+vocabulary and not kept: the sums of exponentials first, then piece by piece the softmax (16 bits an entry, float32: 32)
+and its two products. Tokens whose label
 is ``ignore_index`` take no part: their losses and rows of ``gx`` are zero whatever their rows of x hold, and the products
 run over the others alone.
 
@@ -16,23 +17,24 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .runtime import MAX_TOKENS, _device, _value_type
+from .runtime import MAX_TOKENS, _device, _value_type, current_stream
 
 REDUCTIONS = ("mean", "sum")
+PIECE_BYTES = 512 << 20
 MAX_WIDTH, MAX_VOCAB = 1 << 15, 1 << 24
 _LABEL_BYTES = {torch.int32: 4, torch.int64: 8}
 
 
-def rows_of(t: torch.Tensor, name: str, width: int, dtype: torch.dtype, device: torch.device) -> tuple[torch.Tensor, int]:
+def rows_of(t: torch.Tensor, name: str, width: int, dtype: torch.dtype) -> tuple[torch.Tensor, int]:
     """``t`` as rows of ``width`` entries the kernels read, and their stride: itself where a row's entries are adjacent and rows
     do not overlap, else a contiguous copy. Raises ``ValueError`` for another shape, type or device."""
-    if not (t.dim() == 2 and t.shape[1] == width and t.dtype == dtype and t.device == device):
-        raise ValueError(f"{name}: a {dtype} [N, {width}] tensor on {device} is required, not {t.dtype} {list(t.shape)} on {t.device}")
+    if t.dim() != 2 or t.dtype != dtype or t.get_device() != 0 or t.shape[1] != width:
+        raise ValueError(f"{name}: a {dtype} [N, {width}] tensor on cuda:0 is required, not {t.dtype} {list(t.shape)} on {t.device}")
     if t.shape[0] > MAX_TOKENS:
         raise ValueError(f"{name}: N={t.shape[0]} above {MAX_TOKENS}")
-    if t.shape[0] <= 1 and (width == 1 or t.stride(1) == 1):
+    if t.is_contiguous():
         return t, width
-    if (width == 1 or t.stride(1) == 1) and t.stride(0) >= width:
+    if t.stride(1) == 1 and t.stride(0) >= width:
         return t, t.stride(0)
     return t.contiguous(), width
 
@@ -42,7 +44,12 @@ class HeadLoss:
     call returns are views of them that the next call overwrites. Calls are queued on PyTorch's current stream; calls of one
     object on several streams have to be ordered by the caller."""
 
-    def __init__(self, weight: torch.Tensor, max_tokens: int = 1, ignore_index: int = -100, reduction: str = "mean") -> None:
+    def __init__(self, weight: torch.Tensor, max_tokens: int = 1, ignore_index: int = -100, reduction: str = "mean",
+                 piece_bytes: int = PIECE_BYTES) -> None:
+        """``max_tokens``: the calls the buffers are first sized for (``losses``; ``step``'s own come with its first call or
+        ``reserve``). ``piece_bytes``: what a piece of the vocabulary's softmax may take in ``step`` (N tokens times its rows, 2
+        bytes an entry in bfloat16, 4 in float32; 256 rows at least): the last piece's logits are computed once, the
+        others' twice."""
         self.device = _device(weight.device)
         if weight.dim() != 2 or not weight.is_contiguous() or weight.numel() == 0:
             raise ValueError(f"weight must be a contiguous, non-empty [V, d] tensor, not {list(weight.shape)}")
@@ -50,6 +57,9 @@ class HeadLoss:
             raise ValueError(f"weight of {list(weight.shape)}: at most [{MAX_VOCAB}, {MAX_WIDTH}]")
         if reduction not in REDUCTIONS:
             raise ValueError(f"reduction is one of {REDUCTIONS}, not {reduction!r}")
+        if piece_bytes < 1:
+            raise ValueError(f"piece_bytes={piece_bytes} must be positive")
+        self.piece_bytes = int(piece_bytes)
         self.value_type = _value_type(weight, "weight")
         self.weight, self.ignore_index, self.reduction = weight.detach(), int(ignore_index), reduction
         self.vocab, self.d_model = weight.shape
@@ -60,16 +70,19 @@ class HeadLoss:
         self._gx: torch.Tensor | None = None
         self._loss: torch.Tensor | None = None
         self.grad: torch.Tensor | None = None  # gw of the last step
-        self._stream: torch.cuda.Stream | None = None
+        self._stream: int | None = None
+        self._reserved = [0, 0]  # tokens the buffers hold, for losses and for step
         self.reserve(max_tokens, gradients=False)
 
     def _bytes(self, n: int, gradients: bool) -> int:
-        return _lib.query_bytes(self._lib.hffn_loss_workspace, self.value_type, n, self.d_model, self.vocab, self._aligned, int(gradients))
+        return _lib.query_bytes(self._lib.hffn_loss_workspace, self.value_type, n, self.d_model, self.vocab, self._aligned, int(gradients), self.piece_bytes)
 
     def reserve(self, n: int, gradients: bool = True) -> None:
         """Size the buffers for calls of up to ``n`` tokens (``gradients``: for ``step`` too); allocates what must grow."""
         if not 1 <= n <= MAX_TOKENS:
             raise ValueError(f"N={n} outside [1, {MAX_TOKENS}]")
+        if n <= self._reserved[gradients]:
+            return
         need = self._bytes(n, gradients)
         if self._workspace is None or self._workspace.numel() < need:
             self._workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
@@ -80,29 +93,30 @@ class HeadLoss:
         if gradients and self.grad is None:
             self.grad = torch.empty_like(self.weight)
             self._loss = torch.empty((), device=self.device)
+        self._reserved[gradients] = n
 
     def workspace_bytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in (self._workspace, self._losses, self._gx) if t is not None)
 
     def _call(self, x: torch.Tensor, labels: torch.Tensor, gradients: bool) -> tuple:
         """The checked arguments both entries share, and the stream; the buffers are sized."""
-        x, stride = rows_of(x, "x", self.d_model, self.weight.dtype, self.device)
+        x, stride = rows_of(x, "x", self.d_model, self.weight.dtype)
         n = x.shape[0]
-        if labels.dim() != 1 or labels.shape[0] != n or labels.dtype not in _LABEL_BYTES or labels.device != self.device:
+        if labels.dim() != 1 or labels.shape[0] != n or labels.dtype not in _LABEL_BYTES or labels.get_device() != 0:
             raise ValueError(f"labels: an int32 or int64 [{n}] tensor on {self.device} is required, not {labels.dtype} "
                              f"{list(labels.shape)} on {labels.device}")
-        stream = torch.cuda.current_stream(self.device)
-        if self._stream is not None and stream != self._stream:  # buffers of another stream's pool stay until this one is done
-            for t in (self._workspace, self._losses, self._gx, self._loss, self.grad):
-                if t is not None:
-                    t.record_stream(stream)
-        self._stream = stream
+        stream = current_stream(self.device)
+        if stream != self._stream:
+            if self._stream is not None:  # buffers of another stream's pool stay until this one is done with them
+                for t in (self._workspace, self._losses, self._gx, self._loss, self.grad):
+                    if t is not None:
+                        t.record_stream(torch.cuda.current_stream(self.device))
+            self._stream = stream
         if n:
             self.reserve(n, gradients)
         return x, (self.value_type, x.data_ptr(), stride, self.weight.data_ptr(), labels.data_ptr(), labels.stride(0) if n > 1 else 1,
-                   _LABEL_BYTES[labels.dtype], self.ignore_index), stream.cuda_stream
+                   _LABEL_BYTES[labels.dtype], self.ignore_index), stream
 
-    @torch.no_grad()
     def losses(self, x: torch.Tensor, labels: torch.Tensor) -> torch.Tensor:
         """float32 [N]: the negative log likelihood of every token's label; 0 where it is ``ignore_index``, NaN where it lies
         outside the vocabulary. ``x``: [N, d] of the weight's type, any row stride."""
@@ -113,7 +127,6 @@ class HeadLoss:
                                              self.d_model, self.vocab, n, stream), "losses")
         return self._losses[:n]
 
-    @torch.no_grad()
     def step(self, x: torch.Tensor, labels: torch.Tensor, scale: float = 1.0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """(loss, gx, gw): the mean (or sum) of the counted tokens' losses, float32 0-d, and the gradients of ``scale`` times it
         with respect to x ([N, d], zero rows for ignored tokens) and to the weight ([V, d], also ``self.grad``), both of the
@@ -123,7 +136,7 @@ class HeadLoss:
         if n == 0:
             self.reserve(1)
             return self._loss.zero_(), self._gx[:0], self.grad.zero_()
-        _lib.check(self._lib.hffn_loss_step(*args, int(self.reduction == "mean"), scale, self._loss.data_ptr(), self._gx.data_ptr(),
+        _lib.check(self._lib.hffn_loss_step(*args, int(self.reduction == "mean"), scale, self.piece_bytes, self._loss.data_ptr(), self._gx.data_ptr(),
                                             self.grad.data_ptr(), self._workspace.data_ptr(), self._workspace.numel(), self.d_model,
                                             self.vocab, n, stream), "loss step")
         return self._loss, self._gx[:n], self.grad

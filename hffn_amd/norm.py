@@ -15,15 +15,22 @@ between the calls.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
 from .loss import rows_of
-from .runtime import _device, _value_type
+from .runtime import _device, _value_type, current_stream
 
 KINDS = ("layer", "rms")
 PARAMETERS = ("weight", "bias", "gate", "post_weight", "post_bias")
 MAX_WIDTH = 16384
+
+
+@functools.lru_cache(maxsize=4096)
+def _backward_workspace(n: int, d_model: int) -> int:
+    return _lib.query_bytes(_lib.load().hffn_residual_norm_backward_workspace, n, d_model)
 
 
 def _pointer(t: torch.Tensor | None) -> int | None:
@@ -74,12 +81,11 @@ class ResidualNorm:
     def _rows(self, t: torch.Tensor | None, name: str, like: torch.Tensor) -> tuple[torch.Tensor | None, int]:
         if t is None:
             return None, 0
-        t, stride = rows_of(t, name, self.d_model, like.dtype, self.device)
+        t, stride = rows_of(t, name, self.d_model, like.dtype)
         if t.shape[0] != like.shape[0]:
             raise ValueError(f"{name}: {t.shape[0]} rows for {like.shape[0]}")
         return t, stride
 
-    @torch.no_grad()
     def forward(self, x: torch.Tensor, f: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
         """(r, h); without ``f`` (boundaries without gate and post norm) r is x itself."""
         value_type = _value_type(x, "x")
@@ -88,16 +94,15 @@ class ResidualNorm:
         x, x_stride = self._rows(x, "x", x)
         f, f_stride = self._rows(f, "f", x)
         n, p = x.shape[0], self._parameters
-        h = torch.empty(n, self.d_model, dtype=x.dtype, device=self.device)
+        h = torch.empty_like(x, memory_format=torch.contiguous_format)
         r = x if f is None else torch.empty_like(h)
         if n:
             _lib.check(self._lib.hffn_residual_norm(value_type, x.data_ptr(), x_stride, _pointer(f), f_stride,
                                                     *(_pointer(p.get(name)) for name in PARAMETERS), self.scale, self.eps,
                                                     int(self.kind == "layer"), None if f is None else r.data_ptr(), h.data_ptr(),
-                                                    self.d_model, n, torch.cuda.current_stream(self.device).cuda_stream), "residual norm")
+                                                    self.d_model, n, current_stream(self.device)), "residual norm")
         return r, h
 
-    @torch.no_grad()
     def backward(self, r: torch.Tensor, f: torch.Tensor | None, gr: torch.Tensor | None,
                  gh: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor | None]:
         """(gx, gf): the gradients of x and f for those of r (``None``: none but through h) and h, where r is the forward's (the
@@ -110,21 +115,20 @@ class ResidualNorm:
         gr, gr_stride = self._rows(gr, "gr", r)
         gh, gh_stride = self._rows(gh, "gh", r)
         n, d, p = r.shape[0], self.d_model, self._parameters
-        gx = torch.empty(n, d, dtype=r.dtype, device=self.device)
+        gx = torch.empty_like(r, memory_format=torch.contiguous_format)
         gf = None if f is None else torch.empty_like(gx)
-        for name, t in p.items():
-            if name not in self._gradients:
-                self._gradients[name] = torch.empty_like(t)
         g = self._gradients
+        if not g:
+            g.update((name, torch.empty_like(t)) for name, t in p.items())
         if n == 0:
             for t in g.values():
                 t.zero_()
             return gx, gf
-        bytes_ = _lib.query_bytes(self._lib.hffn_residual_norm_backward_workspace, n, d)
-        work = torch.empty(bytes_, dtype=torch.uint8, device=self.device)
+        bytes_ = _backward_workspace(n, d)
+        work = torch.empty(bytes_ // 4, device=self.device)
         _lib.check(self._lib.hffn_residual_norm_backward(
             value_type, r.data_ptr(), r_stride, _pointer(f), f_stride, _pointer(gr), gr_stride, gh.data_ptr(), gh_stride,
             p["weight"].data_ptr(), *(_pointer(p.get(name)) for name in PARAMETERS[2:]), self.scale, self.eps, int(self.kind == "layer"),
             gx.data_ptr(), _pointer(gf), *(_pointer(g.get(name)) for name in PARAMETERS), work.data_ptr(), bytes_, d, n,
-            torch.cuda.current_stream(self.device).cuda_stream), "residual norm backward")
+            current_stream(self.device)), "residual norm backward")
         return gx, gf

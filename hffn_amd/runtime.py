@@ -209,6 +209,14 @@ def _device(device: str | torch.device | None) -> torch.device:
     return torch.device("cuda", 0)
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def current_stream(device: torch.device) -> int:
+    """The handle of PyTorch's current stream of the device (1.7 us less than through its stream object)."""
+    return _raw_stream(device.index) if _raw_stream else torch.cuda.current_stream(device).cuda_stream
+
+
 def _value_type(tensor: torch.Tensor, name: str) -> int:
     try:
         return _VALUE_TYPES[tensor.dtype]

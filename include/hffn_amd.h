@@ -423,8 +423,8 @@ int hffn_residual_norm_backward(int value_type, const void* r, uint64_t r_stride
 /* The norm over all entries of `arrays` arrays (host arrays of device pointers, entry counts and value types; a pointer
  * aligned to an entry, at most 2^38 entries each): the 2-norm, or the largest magnitude (largest 1), in float64 and rounded
  * to *norm (a device float32). hffn_clip then scales every entry by min(1, limit / (norm + 1e-6)), in place (out NULL; with a
- * factor of one nothing is written) or into out[k] of out_types[k] (host arrays; apart from every p). A NaN norm makes
- * every scaled entry NaN. No two arrays may overlap. Workspace: hffn_clip_workspace bytes, any content, 8-byte aligned. */
+ * factor of one nothing is written) or into out[k] of out_types[k] (host arrays). A NaN norm makes every scaled entry NaN.
+ * hffn_clip refuses arrays that share memory. Workspace: hffn_clip_workspace bytes, any content, 8-byte aligned. */
 int hffn_clip_workspace(uint32_t arrays, uint64_t* bytes);
 int hffn_grad_norm(uint32_t arrays, const void* const* p, const uint64_t* counts, const int* types, int largest, void* workspace,
                    uint64_t workspace_bytes, float* norm, void* stream);
@@ -436,17 +436,21 @@ int hffn_clip(uint32_t arrays, void* const* p, void* const* out, const uint64_t*
  * losses[t] = log sum_v exp(x_t . w_v) - x_t . w_label, 0 for ignored tokens, NaN for a label outside the vocabulary.
  * hffn_loss_step: *loss, the mean (mean 1; 0 where every token is ignored) or the sum of the counted losses, and the
  * gradients of scale times it: gx [n, d_model] (zero rows for ignored tokens, whatever their x holds) and gw [vocab, d_model],
- * of the value type; a label outside the vocabulary makes all of them NaN. Logits are computed in pieces of the vocabulary and
- * not kept. Workspace: hffn_loss_workspace bytes (aligned: the weight starts on a 16-byte boundary; gradients: for
- * hffn_loss_step), any content, 256-byte aligned. Outputs may not overlap inputs. */
+ * of the value type; a label outside the vocabulary makes all of them NaN. Logits are not kept; the gradients are computed in
+ * pieces of the vocabulary whose softmax (16 bits an entry, float32: 32) takes at most piece_bytes (0:
+ * HFFN_LOSS_PIECE_BYTES; 256 vocabulary rows at least). The last piece's logits are computed once, the others' twice: a
+ * larger piece is faster. Workspace: hffn_loss_workspace bytes (aligned: the weight starts on a 16-byte boundary;
+ * gradients: for hffn_loss_step with this piece_bytes), any content, 256-byte aligned. Outputs may not overlap inputs. */
 #define HFFN_MAX_VOCAB (1u << 24)
-int hffn_loss_workspace(int value_type, uint32_t n, uint32_t d_model, uint32_t vocab, int aligned, int gradients, uint64_t* bytes);
+#define HFFN_LOSS_PIECE_BYTES (512ull << 20)
+int hffn_loss_workspace(int value_type, uint32_t n, uint32_t d_model, uint32_t vocab, int aligned, int gradients, uint64_t piece_bytes,
+                        uint64_t* bytes);
 int hffn_losses(int value_type, const void* x, uint64_t x_stride, const void* weight, const void* labels, int64_t labels_stride,
                 int label_bytes, int64_t ignore_index, float* losses, void* workspace, uint64_t workspace_bytes, uint32_t d_model,
                 uint32_t vocab, uint32_t n, void* stream);
 int hffn_loss_step(int value_type, const void* x, uint64_t x_stride, const void* weight, const void* labels, int64_t labels_stride,
-                   int label_bytes, int64_t ignore_index, int mean, float scale, float* loss, void* gx, void* gw, void* workspace,
-                   uint64_t workspace_bytes, uint32_t d_model, uint32_t vocab, uint32_t n, void* stream);
+                   int label_bytes, int64_t ignore_index, int mean, float scale, uint64_t piece_bytes, float* loss, void* gx, void* gw,
+                   void* workspace, uint64_t workspace_bytes, uint32_t d_model, uint32_t vocab, uint32_t n, void* stream);
 
 /* Measurement only, no counterpart in the reference: a plain streaming read of `bytes` (a nonzero multiple of 16 from
  * a 16-byte aligned pointer) by `blocks` blocks of 4 waves, each wave one contiguous span, one word per wave written to
