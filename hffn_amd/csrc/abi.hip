@@ -1008,7 +1008,7 @@ int hffn_residual_norm(int value_type, const void* x, uint64_t x_stride, const v
 int hffn_residual_norm_backward_workspace(uint32_t n, uint32_t d_model, uint64_t* bytes) {
     if (!bytes) return fail(HFFN_ERROR_ARGUMENT, "residual_norm_backward_workspace: null pointer");
     if (int status = check_norm(HFFN_VALUE_F32, n, d_model, {}, 0, false, 0.0f, "residual_norm_backward_workspace")) return status;
-    *bytes = static_cast<uint64_t>(hffn::kNormGrads) * hffn::norm_back_blocks(n, d_model) * d_model * sizeof(float);
+    *bytes = hffn::norm_back_workspace(n, d_model);
     return HFFN_OK;
 }
 
@@ -1029,8 +1029,8 @@ int hffn_residual_norm_backward(int value_type, const void* r, uint64_t r_stride
     if (int status = check_entries(value_type, {r, f, gr, gh, gx, gf},
                                    {weight, gate, post_weight, post_bias, g_weight, g_bias, g_gate, g_post_weight, g_post_bias, workspace}, what))
         return status;
-    uint64_t needed = 0;
-    if (int status = hffn_residual_norm_backward_workspace(n, d_model, &needed)) return status;
+    const uint64_t needed = hffn::norm_back_workspace(n, d_model);
+    if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return fail(HFFN_ERROR_ARGUMENT, "%s: the workspace must be 16-byte aligned", what);
     if (workspace_bytes < needed)
         return fail(HFFN_ERROR_ARGUMENT, "%s: workspace of %llu bytes, %llu needed", what, static_cast<unsigned long long>(workspace_bytes),
                     static_cast<unsigned long long>(needed));

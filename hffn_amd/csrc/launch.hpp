@@ -238,7 +238,8 @@ struct NormForward {
 };
 hipError_t launch_residual_norm(int vt, const NormForward& call, hipStream_t stream);
 // gx = gr + the gradient of r through h; gf that of f; the parameters' gradients (null where not wanted) in the order
-// weight, bias, gate, post_weight, post_bias, summed over the rows by way of partials [kNormGrads][norm_back_blocks][d].
+// weight, bias, gate, post_weight, post_bias, summed over the rows by way of partials (norm_back_workspace bytes,
+// 16-byte aligned).
 // gr null: none; gf null: not written (then f may be null).
 constexpr int kNormGrads = 5;
 struct NormBackward {
@@ -254,7 +255,7 @@ struct NormBackward {
 struct NormGradients {
     float* grad[kNormGrads];
 };
-uint32_t norm_back_blocks(uint32_t n, uint32_t d);
+uint64_t norm_back_workspace(uint32_t n, uint32_t d);
 hipError_t launch_residual_norm_backward(int vt, const NormBackward& call, const NormGradients& grads, hipStream_t stream);
 
 // The norm over many tensors and their scaling (clip.hip). An array is `count` entries of the value type at p (aligned to

@@ -412,7 +412,7 @@ int hffn_residual_norm(int value_type, const void* x, uint64_t x_stride, const v
 /* Its backward from r and f as the forward stored and read them: gx = gr + the gradient of r through h for gh (gr NULL:
  * none), the gradient of x; gf that of f (NULL: not wanted; needed with a gate or a post norm); float32[d_model] gradients
  * of the parameters, each summed over the rows in a fixed order (g_bias NULL: none; g_gate, g_post_weight and g_post_bias come
- * with gate, post_weight and post_bias). Workspace: hffn_residual_norm_backward_workspace bytes, any content. */
+ * with gate, post_weight and post_bias). Workspace: hffn_residual_norm_backward_workspace bytes, 16-byte aligned, any content. */
 int hffn_residual_norm_backward_workspace(uint32_t n, uint32_t d_model, uint64_t* bytes);
 int hffn_residual_norm_backward(int value_type, const void* r, uint64_t r_stride, const void* f, uint64_t f_stride, const void* gr,
                                 uint64_t gr_stride, const void* gh, uint64_t gh_stride, const float* weight, const float* gate,
