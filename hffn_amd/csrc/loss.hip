@@ -24,6 +24,11 @@ typedef __bf16 FragB __attribute__((ext_vector_type(8)));
 typedef _Float16 FragH __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) Quad* LdsQuad;
 typedef __attribute__((address_space(3))) const Frag* LdsFrag;
+typedef float Four __attribute__((ext_vector_type(4)));
+typedef float Eight __attribute__((ext_vector_type(8)));
+typedef uint32_t Words __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) const Four* LdsFour;
+typedef __attribute__((address_space(3))) const float* LdsFloat;
 
 constexpr int kLift = 10;      // the entry an operand's power of two is taken from lies in [2^9, 2^10) ...
 constexpr int kRoom = 5;       // ... and its largest up to kRoom binades above
@@ -68,7 +73,7 @@ __device__ __forceinline__ int64_t label_of(const void* labels, int64_t at, bool
 // What the preparing launches read and write: labels; the counted tokens in order (rows[i] the token of compact row i,
 // compact[i] its label or -1 where that lies outside the vocabulary, place[t] the compact row of token t or -1); the operand
 // rows of x's counted rows (zeros to the next multiple of 64) and, where it is not read in place, of the weight, as
-// [rows][width] bfloat16 or, per 32 entries, 32 hi and 32 lo halves; zeros from d on.
+// [rows][width] bfloat16, float32 (RAW) or, per 32 entries, 32 hi and 32 lo halves; zeros from d on.
 struct Prepare {
     const void *labels, *x, *weight;
     int64_t labels_stride, ignore;
@@ -170,8 +175,9 @@ __device__ __forceinline__ uint32_t sample_of(const Prepare& p, bool of_x, uint3
     return block_most(most, lds);
 }
 
-// One operand row by a wave, eight entries a lane and step; returns the largest finite magnitude that the lane saw.
-template <typename T>
+// One operand row by a wave, eight entries a lane and step; returns the largest finite magnitude that the lane saw. RAW:
+// float32 as they are.
+template <typename T, bool RAW>
 __device__ __forceinline__ uint32_t pack_row(const T* __restrict__ from, uint16_t* __restrict__ to, uint32_t d, uint32_t width, int e) {
     const uint32_t lane = threadIdx.x % kWave;
     const bool whole = reinterpret_cast<uintptr_t>(from) % 16 == 0;
@@ -184,6 +190,12 @@ __device__ __forceinline__ uint32_t pack_row(const T* __restrict__ from, uint16_
             } else {
 #pragma unroll
                 for (uint32_t k = 0; k < 8; ++k) v[k] = c + k < d ? from[c + k] : 0.0f;
+            }
+            if constexpr (RAW) {
+                float4* out = reinterpret_cast<float4*>(to + 2 * c);
+                out[0] = make_float4(v[0], v[1], v[2], v[3]);
+                out[1] = make_float4(v[4], v[5], v[6], v[7]);
+                continue;
             }
             uint32_t hi[4], lo[4];
 #pragma unroll
@@ -216,34 +228,35 @@ __device__ __forceinline__ uint32_t pack_row(const T* __restrict__ from, uint16_
 }
 
 // The weight's rows of block `block`; returns the thread's largest magnitude.
-template <typename T>
+template <typename T, bool RAW>
 __device__ __forceinline__ uint32_t pack_weight(const Prepare& p, uint32_t block, int e) {
     constexpr uint64_t kParts = sizeof(T) == 4 ? 2 : 1;
     uint32_t most = 0;
     for (uint32_t r = threadIdx.x / kWave; r < kWeightRows; r += kPrepWaves) {
         const uint64_t row = static_cast<uint64_t>(block) * kWeightRows + r;
-        if (row < p.vocab) most = max(most, pack_row(static_cast<const T*>(p.weight) + row * p.d, p.w_out + row * kParts * p.width, p.d, p.width, e));
+        if (row < p.vocab) most = max(most, pack_row<T, RAW>(static_cast<const T*>(p.weight) + row * p.d, p.w_out + row * kParts * p.width, p.d, p.width, e));
     }
     return most;
 }
 
 // A block per kPrepWaves tokens (a wave each, and the compact row of the same number where zeros belong) and, after those,
 // one per kWeightRows weight rows to pack.
-template <typename T>
+template <typename T, bool RAW>
 __global__ __launch_bounds__(kPrepThreads) void loss_prepare_kernel(Prepare p) {
     constexpr uint64_t kParts = sizeof(T) == 4 ? 2 : 1;
+    constexpr bool kScaled = sizeof(T) == 4 && !RAW;
     __shared__ uint32_t most_lds[kPrepWaves], sums[kPrepWaves][3];
     const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     if (blockIdx.x >= p.x_blocks) {
         const uint32_t block = blockIdx.x - p.x_blocks;
         int e = 0;
-        if constexpr (sizeof(T) == 4) {
+        if constexpr (kScaled) {
             const uint32_t sample = sample_of(p, false, most_lds);
             e = lift_of(sample);
             if (block == 0 && threadIdx.x == 0) p.meta->weight_sample = sample;
         }
-        const uint32_t most = pack_weight<T>(p, block, e);
-        if constexpr (sizeof(T) == 4) {
+        const uint32_t most = pack_weight<T, RAW>(p, block, e);
+        if constexpr (kScaled) {
             const uint32_t all = block_most(most, most_lds);
             if (threadIdx.x == 0) p.w_most[block] = all;
         }
@@ -301,18 +314,18 @@ __global__ __launch_bounds__(kPrepThreads) void loss_prepare_kernel(Prepare p) {
         }
     }
     int e = 0;
-    if constexpr (sizeof(T) == 4) {
+    if constexpr (kScaled) {
         const uint32_t sample = sample_of(p, true, most_lds);
         e = lift_of(sample);
         if (blockIdx.x == 0 && threadIdx.x == 0) p.meta->x_sample = sample;
     }
     uint32_t most = 0;
-    if (counted) most = pack_row(static_cast<const T*>(p.x) + i * p.x_stride, p.x_out + at * kParts * p.width, p.d, p.width, e);
+    if (counted) most = pack_row<T, RAW>(static_cast<const T*>(p.x) + i * p.x_stride, p.x_out + at * kParts * p.width, p.d, p.width, e);
     if (i >= valid && i < (valid + 63) / 64 * 64) {
         uint4* out = reinterpret_cast<uint4*>(p.x_out + i * kParts * p.width);
         for (uint32_t c = lane; c < kParts * p.width / 8; c += kWave) out[c] = make_uint4(0, 0, 0, 0);
     }
-    if constexpr (sizeof(T) == 4) {
+    if constexpr (kScaled) {
         const uint32_t all = block_most(most, most_lds);
         if (threadIdx.x == 0) p.x_most[blockIdx.x] = all;
     }
@@ -336,10 +349,10 @@ __global__ __launch_bounds__(kPrepThreads) void loss_settle_kernel(Prepare p) {
     }
     if (x_bits != x_sample)
         for (uint32_t i = blockIdx.x * kPrepWaves + threadIdx.x / kWave; i < valid; i += gridDim.x * kPrepWaves)
-            pack_row(static_cast<const float*>(p.x) + p.rows[i] * p.x_stride, p.x_out + static_cast<uint64_t>(i) * 2 * p.width, p.d, p.width,
+            pack_row<float, false>(static_cast<const float*>(p.x) + p.rows[i] * p.x_stride, p.x_out + static_cast<uint64_t>(i) * 2 * p.width, p.d, p.width,
                      lift_of(x_bits));
     if (w_bits != w_sample)
-        for (uint32_t block = blockIdx.x; block < p.w_blocks; block += gridDim.x) pack_weight<float>(p, block, lift_of(w_bits));
+        for (uint32_t block = blockIdx.x; block < p.w_blocks; block += gridDim.x) pack_weight<float, false>(p, block, lift_of(w_bits));
 }
 
 // --------------------------------------------------------------------------------------------------------- the product
@@ -351,10 +364,14 @@ __device__ __forceinline__ uint32_t permuted(uint32_t r) { return (r >> 2 & 1) *
 // An operand's tile in LDS, TILE indexes x 64 / PARTS k (128 bytes an index), 16-byte chunks swizzled so that the lanes of
 // a read touch every bank: index-major (memory rows are the operand's indexes, k contiguous; a row's 8 chunks) or k-major
 // (TR: memory rows are k, read through the LDS transpose reads). Transfers of 1 KB go straight from memory to LDS.
+// Entries in memory: PARTS 1 bfloat16; PARTS 2 fp16 hi and lo; PARTS 3 float32 as they are, split into three bfloat16 parts
+// by the wave that reads them (RAW; k-major tiles of these are read entry by entry).
 template <int PARTS, bool TR, int TILE, int WAVES>
 struct Operand {
+    static constexpr bool RAW = PARTS == 3;
+    static constexpr uint32_t kWords = PARTS == 1 ? 1 : 2;  // 16-bit words of an entry
     static constexpr uint32_t kBytes = TILE * 128, kPieces = kBytes / 1024, kPerWave = kPieces / WAVES;
-    static constexpr uint32_t kRow = TR ? TILE * 2 * PARTS : 128, kDepth = 64 / PARTS;
+    static constexpr uint32_t kRow = TR ? TILE * 2 * kWords : 128, kDepth = 64 / kWords;
     static_assert(kPieces % WAVES == 0, "every wave transfers as many pieces");
 
     const char* base;        // of the tile at k = 0 (index-major) or of its first column (k-major)
@@ -364,7 +381,8 @@ struct Operand {
     uint32_t row[kPerWave], last;  // k-major: the lane's k row of each piece (offset: its column); the last k row to read
 
     __device__ __forceinline__ static uint32_t swizzle(uint32_t r) {
-        if constexpr (TR) return (r & 1) * 4 + (r >> 1 & 1) * 9;
+        if constexpr (TR && RAW) return 0;
+        else if constexpr (TR) return (r & 1) * 4 + (r >> 1 & 1) * 9;
         else return ((r & 3) | (r >> 4 & 1) << 2) ^ (r >> 2 & 1);
     }
     // first: the tile's first index; indexes: memory rows (index-major) or columns, a multiple of 8 (k-major), there are; depth:
@@ -374,21 +392,21 @@ struct Operand {
         const uint32_t wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
         stride = row_entries * 2;
         last = depth - 1;
-        whole = depth * PARTS / 64;
+        whole = depth * kWords / 64;
         if (!TR && first >= indexes) first = indexes - 1;
-        if constexpr (TR) base = reinterpret_cast<const char*>(p) + static_cast<uint64_t>(first) * 2 * PARTS;
+        if constexpr (TR) base = reinterpret_cast<const char*>(p) + static_cast<uint64_t>(first) * 2 * kWords;
         else base = reinterpret_cast<const char*>(p) + first * stride;
 #pragma unroll
         for (uint32_t j = 0; j < kPerWave; ++j) {
             const uint32_t at = (wave * kPerWave + j) * 1024 + lane * 16, r = at / kRow, chunk = at % kRow / 16 ^ swizzle(r);
             if constexpr (TR) {
-                const uint32_t chunks = (indexes - first) * PARTS / 8;  // to the end of the memory row
+                const uint32_t chunks = (indexes - first) * kWords / 8;  // to the end of the memory row
                 row[j] = r;
                 offset[j] = (chunk < chunks ? chunk : chunks - 1) * 16;
             } else {
                 const uint32_t left = indexes - first - 1;  // clamped rows repeat the last
                 offset[j] = (r < left ? r : left) * static_cast<uint32_t>(stride) + chunk * 16;
-                back[j] = chunk * 16 >= depth * PARTS * 2 % 128 ? chunk * 16 : 0;
+                back[j] = chunk * 16 >= depth * kWords * 2 % 128 ? chunk * 16 : 0;
             }
         }
     }
@@ -412,19 +430,21 @@ struct Operand {
     // a lane's place in the tile for the 32-index blocks from `first` on
     __device__ __forceinline__ static uint32_t place(uint32_t first) {
         const uint32_t lane = threadIdx.x % kWave, half = lane / 32;
-        if constexpr (TR) {
+        if constexpr (TR && RAW) {
+            return half * 8 * kRow + (first + permuted(lane % 32)) * 4;
+        } else if constexpr (TR) {
             const uint32_t in = lane % 16, block = (lane / 16 & 1) * 4 + in % 4, k = in / 4;
-            const uint32_t column = first * 2 * PARTS + (block & 1) * 32 + (block >> 1) * 8;
+            const uint32_t column = first * 2 * kWords + (block & 1) * 32 + (block >> 1) * 8;
             return (half * 8 + k) * kRow + (column ^ swizzle(k) * 16);
         } else {
             const uint32_t r = first + permuted(lane % 32);
-            return r * 128 + (half ^ swizzle(r)) * 16;
+            return r * 128 + ((RAW ? 2 * half : half) ^ swizzle(r)) * 16;
         }
     }
     // entries k = 16 step + 8 (lane / 32) + 0..7 of index permuted(lane % 32) of block i
     __device__ __forceinline__ static Frag read(uint32_t tile, uint32_t place, int i, int step, int part) {
         if constexpr (TR) {
-            const uint32_t at = tile + (place ^ (i * 64 * PARTS + part * 64)) + step * 16 * kRow;
+            const uint32_t at = tile + (place ^ (i * 64 * kWords + part * 64)) + step * 16 * kRow;
             const Quad a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<LdsQuad>(at));
             const Quad b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<LdsQuad>(at + 4 * kRow));
             return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
@@ -432,18 +452,70 @@ struct Operand {
             return *reinterpret_cast<LdsFrag>(tile + i * 4096 + (place ^ (part * 64 + step * 32)));
         }
     }
+    __device__ __forceinline__ static Eight read_raw(uint32_t tile, uint32_t place, int i, int step) {
+        if constexpr (TR) {
+            Eight v;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = *reinterpret_cast<LdsFloat>(tile + place + i * 128 + (step * 16 + k) * kRow);
+            return v;
+        } else {
+            const Four a = *reinterpret_cast<LdsFour>(tile + i * 4096 + (place ^ (step * 64)));
+            const Four b = *reinterpret_cast<LdsFour>(tile + i * 4096 + (place ^ (step * 64 + 16)));
+            return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    }
+};
+
+// The same entries as `count` MFMA operands: the parts as read, or three bfloat16 ones whose sum is the float32 to 2^-24.
+template <int PARTS>
+struct Parts {
+    Frag part[PARTS];
+    template <typename OP>
+    __device__ __forceinline__ void read(uint32_t tile, uint32_t place, int i, int step) {
+#pragma unroll
+        for (int k = 0; k < PARTS; ++k) part[k] = OP::read(tile, place, i, step, k);
+    }
+    __device__ __forceinline__ const Parts& parts() const { return *this; }
+};
+struct Raw {
+    Eight value;
+    template <typename OP>
+    __device__ __forceinline__ void read(uint32_t tile, uint32_t place, int i, int step) {
+        value = OP::read_raw(tile, place, i, step);
+    }
+    __device__ __forceinline__ Parts<3> parts() const {
+        uint32_t words[3][4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            float low = value[2 * k], high = value[2 * k + 1];
+#pragma unroll
+            for (int p = 0; p < 3; ++p) {
+                const uint32_t pair = bf16_pair(low, high);
+                words[p][k] = pair;
+                low -= __uint_as_float(pair << 16);
+                high -= __uint_as_float(pair & 0xffff0000u);
+            }
+        }
+        Parts<3> out;
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+            const Words w{words[p][0], words[p][1], words[p][2], words[p][3]};
+            out.part[p] = __builtin_bit_cast(Frag, w);
+        }
+        return out;
+    }
 };
 
 template <int PARTS>
 __device__ __forceinline__ Acc multiply(Frag a, Frag b, Acc c) {
-    if constexpr (PARTS == 1) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(FragB, a), __builtin_bit_cast(FragB, b), c, 0, 0, 0);
+    if constexpr (PARTS != 2) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(FragB, a), __builtin_bit_cast(FragB, b), c, 0, 0, 0);
     else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(FragH, a), __builtin_bit_cast(FragH, b), c, 0, 0, 0);
 }
 
 // float32 calls keep the exponential's last bits; bfloat16 ones round it to 8.
 template <int PARTS>
 __device__ __forceinline__ float exponential(float v) {
-    if constexpr (PARTS == 2) return v < -150.0f ? 0.0f : exp_split(v);  // also -inf, of which exp_split makes a NaN
+    if constexpr (PARTS != 1) return v < -150.0f ? 0.0f : exp_split(v);  // also -inf, of which exp_split makes a NaN
     else return __expf(v);
 }
 
@@ -460,6 +532,7 @@ struct Product {
     uint32_t vocab;
     uint32_t k_tiles;             // all (GradX: of the piece)
     uint32_t a_tiles, b_tiles, splits;
+    uint32_t height, a_columns_out;  // vocabulary rows of a tile (Stats, Keep, Grad; kA at most), columns of D to write
     const Meta* meta;
     const int32_t* labels;        // compact
     const float* lse;             // Grad, compact
@@ -505,9 +578,9 @@ __device__ __forceinline__ TilePlace tile_place(uint32_t block, uint32_t inner, 
     return {group * kGroup + rest % width, rest / width};
 }
 
-// Where a tile's results lie.
+// Where a tile's results lie: a0 <= indexes of A < a_end, a_tile its whole tile along A.
 struct TileAt {
-    uint32_t a0, b0, split;
+    uint32_t a0, b0, split, a_tile, a_end;
 };
 
 // One tile: where it lies, its operands and its k-tiles.
@@ -528,13 +601,15 @@ struct Tile {
         at.split = index / per_split;
         const TilePlace tile = tile_place(index % per_split, kTokensFirst ? live_b : p.a_tiles, kTokensFirst ? p.a_tiles : live_b);
         constexpr uint32_t kPartsA = WHOLE::kA / S::kA;
-        at.a0 = (kTokensFirst ? tile.outer : tile.inner) * WHOLE::kA + part % kPartsA * S::kA;
+        at.a_tile = kTokensFirst ? tile.outer : tile.inner;
+        at.a0 = at.a_tile * (kTokensFirst ? p.height : WHOLE::kA) + part % kPartsA * S::kA;
+        at.a_end = kTokensFirst ? min((at.a_tile + 1) * p.height, p.a_columns_out) : p.a_count;
         at.b0 = (kTokensFirst ? tile.inner : tile.outer) * WHOLE::kB + part / kPartsA * S::kB;
         k_begin = 0;
         k_end = p.k_tiles;
         if constexpr (kTokensFirst) {
             if (at.b0 >= valid) return false;
-            a.begin(p.a, p.a_stride, p.a_first + at.a0, p.vocab, p.a_columns);
+            a.begin(p.a, p.a_stride, p.a_first + at.a0, min(p.vocab, p.a_first + at.a_end), p.a_columns);
             b.begin(p.b, p.b_stride, at.b0, p.n_pad, p.b_columns);
         } else if constexpr (USE == Use::GradX) {
             if (at.b0 >= valid || at.a0 >= p.a_columns) return false;
@@ -576,7 +651,7 @@ __device__ __forceinline__ void meet() {
 // others.
 template <typename S>
 __device__ __forceinline__ void accumulate(const Tile<S>& tile, const char* ring, Acc (&sums)[S::TA][S::TB]) {
-    constexpr int PARTS = S::PARTS, TA = S::TA, TB = S::TB, kSteps = 4 / PARTS, kTransfers = static_cast<int>(S::kTransfers);
+    constexpr int PARTS = S::PARTS, TA = S::TA, TB = S::TB, kSteps = PARTS == 1 ? 4 : 2, kTransfers = static_cast<int>(S::kTransfers);
     static_assert(kSteps % 2 == 0, "a k-tile's first step always reads into the same registers");
     const uint32_t wave = threadIdx.x / kWave, lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(ring));
     const uint32_t a_place = S::OpA::place(wave % S::WA * TA * 32), b_place = S::OpB::place(wave / S::WA * TB * 32);
@@ -586,27 +661,25 @@ __device__ __forceinline__ void accumulate(const Tile<S>& tile, const char* ring
 #pragma unroll
         for (int j = 0; j < TB; ++j) sums[i][j] = 0.0f;
     if (k_begin >= k_end) return;
-    Acc chain[PARTS == 2 ? TA : 1][PARTS == 2 ? TB : 1];
-    if constexpr (PARTS == 2) {
+    Acc chain[PARTS != 1 ? TA : 1][PARTS != 1 ? TB : 1];
+    if constexpr (PARTS != 1) {
 #pragma unroll
         for (int i = 0; i < TA; ++i)
 #pragma unroll
             for (int j = 0; j < TB; ++j) chain[i][j] = 0.0f;
     }
     const auto acc = [&](int i, int j) -> Acc& {
-        if constexpr (PARTS == 2) return chain[i][j];
+        if constexpr (PARTS != 1) return chain[i][j];
         else return sums[i][j];
     };
-    Frag fa[2][TA][PARTS], fb[2][TB][PARTS];
+    using Read = typename std::conditional<PARTS == 3, Raw, Parts<PARTS>>::type;
+    Read fa[2][TA], fb[2][TB];
     const auto read = [&](uint32_t kt, int step, int to) {
         const uint32_t tile_a = lds + (kt - k_begin) % S::kStages * S::kStage, tile_b = tile_a + S::OpA::kBytes;
 #pragma unroll
-        for (int part = 0; part < PARTS; ++part) {
+        for (int i = 0; i < TA; ++i) fa[to][i].template read<typename S::OpA>(tile_a, a_place, i, step);
 #pragma unroll
-            for (int i = 0; i < TA; ++i) fa[to][i][part] = S::OpA::read(tile_a, a_place, i, step, part);
-#pragma unroll
-            for (int j = 0; j < TB; ++j) fb[to][j][part] = S::OpB::read(tile_b, b_place, j, step, part);
-        }
+        for (int j = 0; j < TB; ++j) fb[to][j].template read<typename S::OpB>(tile_b, b_place, j, step);
     };
     if (k_end - k_begin >= static_cast<uint32_t>(S::kStages)) meet<kTransfers * (S::kStages - 1)>();
     else meet<0>();
@@ -623,18 +696,21 @@ __device__ __forceinline__ void accumulate(const Tile<S>& tile, const char* ring
                 if (kt + S::kStages < k_end) tile.fetch(kt + S::kStages, ring);
                 read(kt + 1, 0, 1 - now);
             }
+            Parts<PARTS> a[TA], b[TB];
+#pragma unroll
+            for (int i = 0; i < TA; ++i) a[i] = fa[now][i].parts();
+#pragma unroll
+            for (int j = 0; j < TB; ++j) b[j] = fb[now][j].parts();
 #pragma unroll
             for (int i = 0; i < TA; ++i)
 #pragma unroll
-                for (int j = 0; j < TB; ++j) {
-                    acc(i, j) = multiply<PARTS>(fa[now][i][0], fb[now][j][0], acc(i, j));
-                    if constexpr (PARTS == 2) {
-                        acc(i, j) = multiply<PARTS>(fa[now][i][0], fb[now][j][1], acc(i, j));
-                        acc(i, j) = multiply<PARTS>(fa[now][i][1], fb[now][j][0], acc(i, j));
-                    }
-                }
+                for (int j = 0; j < TB; ++j)
+#pragma unroll
+                    for (int k = 0; k < PARTS; ++k)  // the parts' products down to the last part's weight
+#pragma unroll
+                        for (int m = 0; k + m < PARTS; ++m) acc(i, j) = multiply<PARTS>(a[i].part[k], b[j].part[m], acc(i, j));
         }
-        if constexpr (PARTS == 2) {
+        if constexpr (PARTS != 1) {
             if ((kt - k_begin) % kChain == kChain - 1 || kt + 1 == k_end) {
 #pragma unroll
                 for (int i = 0; i < TA; ++i)
@@ -656,7 +732,7 @@ __device__ __forceinline__ void finish(const Product& p, const Meta& meta, const
     constexpr int PARTS = S::PARTS, WA = S::WA, TA = S::TA, TB = S::TB;
     constexpr Use USE = S::USE;
     const uint32_t wave = threadIdx.x / kWave, wa = wave % WA, wb = wave / WA, lane = threadIdx.x % kWave, half = lane / 32;
-    const uint32_t a0 = tile.a0, b0 = tile.b0, split_at = tile.split, a_lane = a0 + wa * TA * 32 + 16 * half;
+    const uint32_t a0 = tile.a0, b0 = tile.b0, split_at = tile.split, a_end = tile.a_end, a_lane = a0 + wa * TA * 32 + 16 * half;
     float power = 1.0f;
     if constexpr (PARTS == 2) {
         const int ew = lift_of(meta.weight_bits), ex = lift_of(meta.x_bits);
@@ -671,26 +747,29 @@ __device__ __forceinline__ void finish(const Product& p, const Meta& meta, const
         }
     }
     const auto result = [&](int i, int j, int r) -> float { return sums[i][j][r]; };
-    // 16 consecutive 16-bit entries of a lane (float32: hi and lo) into row t of D, from its block i on
+    // 16 consecutive entries of a lane into row t of D, from its block i on: 16-bit ones (PARTS 2: hi and lo), or the bits of
+    // 16 float32 (PARTS 3: eight and eight)
     const auto store = [&](uint32_t t, int i, const uint32_t (&hi)[8], const uint32_t (&lo)[8]) {
-        uint16_t* to = p.grad + t * p.grad_stride + (a_lane - 16 * half + i * 32) * PARTS + 16 * half;
+        if (a_lane + i * 32 >= a_end) return;
+        uint16_t* to = p.grad + t * p.grad_stride + (a_lane - 16 * half + i * 32) * (PARTS == 1 ? 1 : 2) + (PARTS == 3 ? 32 : 16) * half;
         *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
         *reinterpret_cast<uint4*>(to + 8) = make_uint4(hi[4], hi[5], hi[6], hi[7]);
-        if constexpr (PARTS == 2) {
-            *reinterpret_cast<uint4*>(to + 32) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-            *reinterpret_cast<uint4*>(to + 40) = make_uint4(lo[4], lo[5], lo[6], lo[7]);
+        constexpr int kLow = PARTS == 3 ? 16 : 32;
+        if constexpr (PARTS != 1) {
+            *reinterpret_cast<uint4*>(to + kLow) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            *reinterpret_cast<uint4*>(to + kLow + 8) = make_uint4(lo[4], lo[5], lo[6], lo[7]);
         }
     };
     if constexpr (USE == Use::Stats || USE == Use::Keep) {
         constexpr uint32_t kFill = SLICES * S::kA / (WHOLE_A * WA);  // slices a wave fills
-        const uint32_t slice = p.slice_first + a0 / WHOLE_A * SLICES + (a0 % WHOLE_A / (WA * TA * 32) * WA + wa) * kFill;
-        const uint32_t first = p.a_first + a_lane;  // vocabulary row of the lane's first result
-        if (p.a_first + a0 + S::kA > p.vocab) {     // the last vocabulary tile: what lies beyond adds nothing
+        const uint32_t slice = p.slice_first + tile.a_tile * SLICES + ((a0 - tile.a_tile * p.height) / (WA * TA * 32) * WA + wa) * kFill;
+        const uint32_t first = p.a_first + a_lane, end = min(p.vocab, p.a_first + a_end);  // vocabulary rows: the lane's first, the tile's end
+        if (p.a_first + a0 + S::kA > end) {  // what lies beyond adds nothing
 #pragma unroll
             for (int i = 0; i < TA; ++i)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    if (first + i * 32 + r >= p.vocab)
+                    if (first + i * 32 + r >= end)
 #pragma unroll
                         for (int j = 0; j < S::TB; ++j) sums[i][j][r] = -__builtin_huge_valf();
         }
@@ -706,7 +785,7 @@ __device__ __forceinline__ void finish(const Product& p, const Meta& meta, const
             const float shift = most == -__builtin_huge_valf() ? 0.0f : most;
             float sum = 0.0f;
             const uint32_t label = t < meta.valid ? static_cast<uint32_t>(p.labels[t]) - first : 0xffffffffu;  // outside: far from every lane
-            if (label < TA * 32 && (label & 16) == 0) {
+            if (label < TA * 32 && (label & 16) == 0 && first + label < end) {
                 float logit = 0.0f;
 #pragma unroll
                 for (int i = 0; i < TA; ++i)
@@ -724,6 +803,10 @@ __device__ __forceinline__ void finish(const Product& p, const Meta& meta, const
                     sum += e[1];
                     if constexpr (USE == Use::Keep && PARTS == 1) {
                         hi[r / 2] = kept_bits(e[0]) | kept_bits(e[1]) << 16;
+                    } else if constexpr (USE == Use::Keep && PARTS == 3) {
+                        uint32_t* const to = r < 8 ? hi : lo;
+                        to[r % 8] = __float_as_uint(e[0]);
+                        to[r % 8 + 1] = __float_as_uint(e[1]);
                     } else if constexpr (USE == Use::Keep) {
                         uint16_t h[2], l[2];
                         split(e[0] * (1 << kGradLift), h[0], l[0]);
@@ -761,6 +844,10 @@ __device__ __forceinline__ void finish(const Product& p, const Meta& meta, const
                     }
                     if constexpr (PARTS == 1) {
                         hi[r / 2] = bf16_pair(v[0], v[1]);
+                    } else if constexpr (PARTS == 3) {
+                        uint32_t* const to = r < 8 ? hi : lo;
+                        to[r % 8] = __float_as_uint(v[0]);
+                        to[r % 8 + 1] = __float_as_uint(v[1]);
                     } else {
                         uint16_t h[2], l[2];
                         split(v[0] * (1 << kGradLift), h[0], l[0]);
@@ -886,34 +973,42 @@ __global__ __launch_bounds__(WA* WB* kWave) __attribute__((amdgpu_waves_per_eu(2
 // ------------------------------------------------------------------------------------------- the sums over the vocabulary
 
 // lse and loss of every counted token from the slices: TOKENS tokens a block, 1024 / TOKENS threads each over the slices.
-constexpr uint32_t kLseThreads = 1024;
+constexpr uint32_t kLseThreads = 1024, kLseWaves = kLseThreads / kWave;
+__device__ __forceinline__ float2 joined(float2 a, float2 b) {
+    const float most = fmaxf(a.x, b.x);
+    if (most == -__builtin_huge_valf()) return make_float2(most, a.y + b.y);
+    return make_float2(most, a.y * exponential<2>(a.x - most) + b.y * exponential<2>(b.x - most));
+}
+template <uint32_t TOKENS>
+__device__ __forceinline__ float2 joined_lanes(float2 v) {  // over the lanes of a wave that share a token
+#pragma unroll
+    for (uint32_t step = TOKENS; step < kWave; step *= 2) v = joined(v, make_float2(__shfl_xor(v.x, step), __shfl_xor(v.y, step)));
+    return v;
+}
 template <uint32_t TOKENS>
 __global__ __launch_bounds__(kLseThreads) void loss_lse_kernel(const float2* __restrict__ slices, uint32_t count, uint32_t n_pad,
                                                               const float* __restrict__ picked, const int32_t* __restrict__ rows,
                                                               const int32_t* __restrict__ labels, const Meta* __restrict__ meta,
                                                               float* __restrict__ lse, float* __restrict__ losses) {
     constexpr uint32_t kLanes = kLseThreads / TOKENS;
-    __shared__ float2 lds[kLanes][TOKENS];
-    const uint32_t in = threadIdx.x % TOKENS, first = threadIdx.x / TOKENS, t = blockIdx.x * TOKENS + in, valid = meta->valid;
+    __shared__ float2 lds[kLseWaves * TOKENS];
+    const uint32_t in = threadIdx.x % TOKENS, t = blockIdx.x * TOKENS + in, valid = meta->valid, lane = threadIdx.x % kWave;
     if (blockIdx.x * TOKENS >= valid) return;
-    const auto join = [](float2 a, float2 b) {
-        const float most = fmaxf(a.x, b.x);
-        if (most == -__builtin_huge_valf()) return make_float2(most, a.y + b.y);
-        return make_float2(most, a.y * expf(a.x - most) + b.y * expf(b.x - most));
-    };
     float2 all = make_float2(-__builtin_huge_valf(), 0.0f);
     if (t < valid)
 #pragma unroll 4
-        for (uint32_t s = first; s < count; s += kLanes) all = join(all, slices[static_cast<uint64_t>(s) * n_pad + t]);
-    lds[first][in] = all;
+        for (uint32_t s = threadIdx.x / TOKENS; s < count; s += kLanes) all = joined(all, slices[static_cast<uint64_t>(s) * n_pad + t]);
+    all = joined_lanes<TOKENS>(all);
+    if (lane < TOKENS) lds[threadIdx.x / kWave * TOKENS + in] = all;
     __syncthreads();
-    for (uint32_t step = kLanes / 2; step > 0; step /= 2) {
-        if (first < step) lds[first][in] = join(lds[first][in], lds[first + step][in]);
-        __syncthreads();
-    }
-    if (first != 0 || t >= valid) return;
-    const float2 total = lds[0][in];
-    const float value = total.x + logf(total.y);
+    if (threadIdx.x >= kWave) return;
+    all = make_float2(-__builtin_huge_valf(), 0.0f);
+#pragma unroll
+    for (uint32_t k = 0; k < kLseWaves * TOKENS; k += kWave)
+        if (k + lane < kLseWaves * TOKENS) all = joined(all, lds[k + lane]);  // a multiple of TOKENS apart: the lane's token
+    all = joined_lanes<TOKENS>(all);
+    if (lane >= TOKENS || t >= valid) return;
+    const float value = all.x + logf(all.y);
     lse[t] = value;
     losses[rows[t]] = labels[t] < 0 ? __uint_as_float(0x7fc00000u) : value - picked[t];
 }
@@ -925,33 +1020,40 @@ __global__ __launch_bounds__(kLseThreads) void loss_lse_kernel(const float2* __r
 // against 222 us.
 constexpr uint32_t kTurnThreads = 256;
 template <int PARTS>
-__global__ __launch_bounds__(kTurnThreads) void loss_turn_kernel(uint16_t* __restrict__ grad, uint64_t stride, uint32_t first, uint32_t count, uint32_t across,
-                                                                const float2* __restrict__ slices, uint32_t slice_rows, uint32_t n_pad,
+__global__ __launch_bounds__(kTurnThreads) void loss_turn_kernel(uint16_t* __restrict__ grad, uint64_t stride, uint32_t first, uint32_t count,
+                                                                uint32_t across, const float2* __restrict__ slices, uint32_t height,
+                                                                uint32_t per_tile, uint32_t slice_rows, uint32_t n_pad,
                                                                 const float* __restrict__ lse, const int32_t* __restrict__ labels,
                                                                 const Meta* __restrict__ meta) {
     const uint32_t t = blockIdx.x / across, valid = meta->valid, c = (blockIdx.x % across * kTurnThreads + threadIdx.x) * 8;
     if (t >= (valid + 63) / 64 * 64 || c >= count) return;
-    uint4* const at = reinterpret_cast<uint4*>(grad + t * stride + (PARTS == 2 ? c / 32 * 64 + c % 32 : c));
-    uint4* const low = at + 4;  // the lo halves
+    uint4* const at = reinterpret_cast<uint4*>(grad + t * stride + (PARTS == 1 ? c : PARTS == 2 ? c / 32 * 64 + c % 32 : 2 * c));
+    uint4* const low = at + (PARTS == 2 ? 4 : 1);  // PARTS 2: the lo halves, 3: the last four
     if (t >= valid) {
         *at = make_uint4(0, 0, 0, 0);
-        if constexpr (PARTS == 2) *low = make_uint4(0, 0, 0, 0);
+        if constexpr (PARTS != 1) *low = make_uint4(0, 0, 0, 0);
         return;
     }
-    const float most = slices[static_cast<uint64_t>(c / slice_rows) * n_pad + t].x;
+    const float most = slices[static_cast<uint64_t>(c / height * per_tile + c % height / slice_rows) * n_pad + t].x;
     const float factor = exponential<2>(most - lse[t]) * (PARTS == 2 ? 1.0f / (1 << kGradLift) : 1.0f);
     const uint32_t label = static_cast<uint32_t>(labels[t]) - first - c;
-    const uint4 kept = *at, rest = PARTS == 2 ? *low : make_uint4(0, 0, 0, 0);
+    const uint4 kept = *at, rest = PARTS != 1 ? *low : make_uint4(0, 0, 0, 0);
     const uint32_t hi[4] = {kept.x, kept.y, kept.z, kept.w}, lo[4] = {rest.x, rest.y, rest.z, rest.w};
     float v[8];
 #pragma unroll
     for (uint32_t k = 0; k < 8; ++k) {
         const uint32_t shift = 16 * (k % 2);
-        const float e = PARTS == 1 ? kept_value(hi[k / 2] >> shift) : half_value(hi[k / 2] >> shift) + half_value(lo[k / 2] >> shift);
+        float e;
+        if constexpr (PARTS == 1) e = kept_value(hi[k / 2] >> shift);
+        else if constexpr (PARTS == 2) e = half_value(hi[k / 2] >> shift) + half_value(lo[k / 2] >> shift);
+        else e = __uint_as_float(k < 4 ? hi[k] : lo[k - 4]);
         v[k] = e * factor - (label == k ? 1.0f : 0.0f);
     }
     if constexpr (PARTS == 1) {
         *at = make_uint4(bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]), bf16_pair(v[4], v[5]), bf16_pair(v[6], v[7]));
+    } else if constexpr (PARTS == 3) {
+        *reinterpret_cast<float4*>(at) = make_float4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<float4*>(low) = make_float4(v[4], v[5], v[6], v[7]);
     } else {
         uint32_t h[4], l[4];
 #pragma unroll
@@ -1028,31 +1130,55 @@ __global__ __launch_bounds__(kFinishThreads) void loss_finish_kernel(const float
 
 // ------------------------------------------------------------------------------------------------------------ the host
 
-constexpr uint32_t kTile = 256;                // vocabulary rows and width of a tile
+constexpr uint32_t kTile = 256;                      // vocabulary rows and width of a tile
 constexpr uint32_t kFewTokens = 64, kFewTile = 128;  // up to so many tokens: tiles of 128 x 64, two blocks a CU
 constexpr uint32_t kCus = 256;
 
 uint32_t ceil_div(uint64_t a, uint32_t b) { return static_cast<uint32_t>((a + b - 1) / b); }
 uint32_t padded(uint32_t v, uint32_t to) { return ceil_div(v, to) * to; }
 
+// How a call runs. parts: 1 bfloat16, 2 float32 as fp16 hi + lo, 3 float32 as three bfloat16 parts split where they are
+// multiplied. A few tokens wait for the weight, not for the matrix unit: packing it would read and write it once more.
 struct Plan {
-    uint32_t parts, n_pad, width, vocab_tile, token_tile, per_tile, slices, piece, pieces, splits;
-    bool few, in_place;
+    uint32_t parts, words, n_pad, width, vocab_tile, token_tile, height, per_tile, slices, piece, pieces, last, stats_tiles, keep_tiles, splits;
+    bool few, in_place, keeps;
     uint64_t meta, rows, labels, place, lse, picked, losses, slice_sums, x_most, w_most, x, weight, grad, partial, bytes;
 };
 
-// `aligned`: the weight starts on a 16-byte boundary (bfloat16 weights of whole 16-byte pieces are then read in place).
+// `aligned`: the weight starts on a 16-byte boundary (weights of whole 16-byte pieces are then read in place, but for parts 2).
 Plan plan_of(int vt, uint32_t n, uint32_t d, uint32_t vocab, bool aligned, bool gradients, uint64_t piece_bytes) {
     Plan p{};
-    p.parts = vt == kBF16 ? 1 : 2;
     p.few = n <= kFewTokens;
+    p.parts = vt == kBF16 ? 1 : p.few ? 3 : 2;
+    p.words = p.parts == 1 ? 1 : 2;
     p.vocab_tile = p.few ? kFewTile : kTile;
     p.token_tile = p.few ? kFewTokens : p.parts == 1 ? 256 : 128;
     p.n_pad = padded(n, p.few ? kFewTokens : 256);
-    p.width = padded(d, 64 / p.parts);
-    p.in_place = p.parts == 1 && d % 8 == 0 && aligned;
-    p.per_tile = !p.few && p.parts == 2 ? 8 : 4;  // slices: as many as waves of quarter tiles along the vocabulary
-    p.slices = padded(vocab, kTile) / p.vocab_tile * p.per_tile;
+    p.width = padded(d, 64 / p.words);
+    p.in_place = p.parts != 2 && d % (8 / p.words) == 0 && aligned;
+    p.per_tile = p.parts == 2 ? 8 : 4;  // slices: as many as waves of quarter tiles (few: of tiles) along the vocabulary
+    p.pieces = 1;
+    p.piece = padded(vocab, kTile);
+    if (gradients) {
+        const uint64_t most = (piece_bytes == 0 ? kLossPieceBytes : piece_bytes) / (2ull * p.words * p.n_pad * kTile);
+        const uint32_t tiles = ceil_div(vocab, kTile), fit = most < 1 ? 1 : most < tiles ? static_cast<uint32_t>(most) : tiles;
+        p.piece = ceil_div(tiles, ceil_div(tiles, fit)) * kTile;
+        p.pieces = ceil_div(vocab, p.piece);
+    }
+    // The last piece's exponentials stay where its D belongs. Not those of a few bfloat16 tokens, whose products wait for the
+    // weight and whose gradients may come from a single entry of D: it is rounded once.
+    p.keeps = gradients && !(p.few && p.parts == 1);
+    p.last = p.keeps ? (p.pieces - 1) * p.piece : vocab;
+    // A few tokens' vocabulary tiles share the rows evenly between the blocks that the CUs hold (50304 rows: 99 or 112 of 128
+    // a block, 512 blocks, where whole tiles would be 393); their results go out in sixteens where D is written.
+    p.height = p.vocab_tile;
+    if (p.few) {
+        const uint32_t blocks = 2 * kCus, even = ceil_div(vocab, blocks * ceil_div(vocab, blocks * kFewTile));
+        p.height = gradients ? padded(even, 16) : even < 16 ? 16 : even;
+    }
+    p.stats_tiles = ceil_div(p.last, p.height);
+    p.keep_tiles = p.keeps ? ceil_div(padded(vocab - p.last, kTile), p.height) : 0;
+    p.slices = (p.stats_tiles + p.keep_tiles) * p.per_tile;
     uint64_t at = 0;
     const auto take = [&](uint64_t bytes) {
         const uint64_t here = at;
@@ -1071,20 +1197,14 @@ Plan plan_of(int vt, uint32_t n, uint32_t d, uint32_t vocab, bool aligned, bool 
         p.x_most = take(4ull * ceil_div(p.n_pad, kPrepWaves));
         p.w_most = take(4ull * ceil_div(vocab, kWeightRows));
     }
-    p.x = take(2ull * p.parts * p.n_pad * p.width);
-    p.weight = p.in_place ? 0 : take(2ull * p.parts * vocab * p.width);
+    p.x = take(2ull * p.words * p.n_pad * p.width);
+    p.weight = p.in_place ? 0 : take(2ull * p.words * vocab * p.width);
     if (gradients) {
-        const uint64_t per_row = 2ull * p.parts * p.n_pad;
-        const uint64_t most = (piece_bytes == 0 ? kLossPieceBytes : piece_bytes) / (per_row * kTile);
-        const uint32_t tiles = ceil_div(vocab, kTile), fit = most < 1 ? 1 : most < tiles ? static_cast<uint32_t>(most) : tiles;
-        p.pieces = ceil_div(tiles, fit);
-        p.piece = ceil_div(tiles, p.pieces) * kTile;
-        p.pieces = ceil_div(vocab, p.piece);
         // splits of the vocabulary that give every CU a block (few tokens: two), each of 8 k-tiles at least
-        const uint32_t blocks = ceil_div(p.width, p.vocab_tile) * (p.n_pad / p.token_tile), k_tiles = p.piece / (64 / p.parts);
+        const uint32_t blocks = ceil_div(p.width, p.vocab_tile) * (p.n_pad / p.token_tile), k_tiles = p.piece / (64 / p.words);
         const uint32_t fill = ceil_div(p.few ? 2 * kCus : kCus, blocks), limit = k_tiles / 8 < 1 ? 1 : k_tiles / 8;
         p.splits = fill < limit ? fill : limit;
-        p.grad = take(per_row * p.piece);
+        p.grad = take(2ull * p.words * p.n_pad * p.piece);
         p.partial = take(4ull * p.splits * p.n_pad * p.width);
     }
     p.bytes = at;
@@ -1100,8 +1220,9 @@ hipError_t launch_product(const Product& p, hipStream_t stream) {
 
 template <Use USE>
 hipError_t product(const Plan& plan, const Product& p, hipStream_t stream) {
-    if constexpr (USE != Use::GradW)
-        if (plan.few) return plan.parts == 1 ? launch_product<1, USE, 4, 1, 1, 2>(p, stream) : launch_product<2, USE, 4, 1, 1, 2>(p, stream);
+    if (plan.parts == 3) return launch_product<3, USE, 4, 1, 1, 2>(p, stream);
+    if constexpr (USE != Use::GradW && USE != Use::Keep)
+        if (plan.few) return launch_product<1, USE, 4, 1, 1, 2>(p, stream);
     return plan.parts == 1 ? launch_product<1, USE, 2, 4, 4, 2>(p, stream) : launch_product<2, USE, 4, 2, 2, 2>(p, stream);
 }
 
@@ -1117,8 +1238,8 @@ hipError_t run(const LossCall& c, hipStream_t stream) {
     float* const losses = c.losses != nullptr ? c.losses : reinterpret_cast<float*>(work + plan.losses);
     uint16_t* const x = reinterpret_cast<uint16_t*>(work + plan.x);
     const uint16_t* const weight = plan.in_place ? static_cast<const uint16_t*>(c.weight) : reinterpret_cast<const uint16_t*>(work + plan.weight);
-    const uint64_t x_row = static_cast<uint64_t>(plan.width) * plan.parts, w_row = plan.in_place ? c.d : x_row;
-    const uint32_t w_columns = plan.in_place ? c.d : plan.width, depth = 64 / plan.parts;
+    const uint32_t w_columns = plan.in_place ? c.d : plan.width, depth = 64 / plan.words;
+    const uint64_t x_row = static_cast<uint64_t>(plan.width) * plan.words, w_row = static_cast<uint64_t>(w_columns) * plan.words;
     const auto failed = [](hipError_t& status) { return (status = hipGetLastError()) != hipSuccess; };
     hipError_t status;
 
@@ -1130,12 +1251,16 @@ hipError_t run(const LossCall& c, hipStream_t stream) {
         hipLaunchKernelGGL(loss_scan_kernel, dim3(1), dim3(kScanThreads), 0, stream, prepare);
         if (failed(status)) return status;
     }
-    hipLaunchKernelGGL(loss_prepare_kernel<T>, dim3(prepare.x_blocks + prepare.w_blocks), dim3(kPrepThreads), 0, stream, prepare);
-    if (failed(status)) return status;
+    const dim3 prepare_grid(prepare.x_blocks + prepare.w_blocks);
     if constexpr (sizeof(T) == 4) {
-        hipLaunchKernelGGL(loss_settle_kernel, dim3(2 * kCus), dim3(kPrepThreads), 0, stream, prepare);
+        if (plan.parts == 3) hipLaunchKernelGGL((loss_prepare_kernel<T, true>), prepare_grid, dim3(kPrepThreads), 0, stream, prepare);
+        else hipLaunchKernelGGL((loss_prepare_kernel<T, false>), prepare_grid, dim3(kPrepThreads), 0, stream, prepare);
         if (failed(status)) return status;
+        if (plan.parts == 2) hipLaunchKernelGGL(loss_settle_kernel, dim3(2 * kCus), dim3(kPrepThreads), 0, stream, prepare);
+    } else {
+        hipLaunchKernelGGL((loss_prepare_kernel<T, false>), prepare_grid, dim3(kPrepThreads), 0, stream, prepare);
     }
+    if (failed(status)) return status;
 
     Product p{};
     p.meta = meta;
@@ -1156,25 +1281,21 @@ hipError_t run(const LossCall& c, hipStream_t stream) {
     stats.b_stride = x_row;
     stats.b_columns = plan.width;
     stats.k_tiles = plan.width / depth;
-    stats.a_tiles = padded(c.vocab, kTile) / plan.vocab_tile;
+    stats.a_tiles = plan.stats_tiles;
     stats.b_tiles = token_tiles;
+    stats.height = plan.height;
+    stats.a_columns_out = plan.last;
     stats.picked = picked;
     stats.slices = reinterpret_cast<float2*>(work + plan.slice_sums);
-    // The last piece's exponentials stay where its D belongs. Not those of a few bfloat16 tokens, whose products wait for the
-    // weight and whose gradients may come from a single entry of D: it is rounded once.
-    const bool keeps = gradients && (plan.parts == 2 || !plan.few);
-    const uint32_t last = keeps ? (plan.pieces - 1) * plan.piece : c.vocab;
     Product keep = stats;
-    if (keeps) {
-        keep.a_first = last;
-        keep.a_tiles = padded(c.vocab - last, kTile) / plan.vocab_tile;
-        keep.slice_first = last / plan.vocab_tile * plan.per_tile;
-        stats.a_tiles = last / plan.vocab_tile;
-    }
+    keep.a_first = plan.last;
+    keep.a_tiles = plan.keep_tiles;
+    keep.a_columns_out = plan.keeps ? padded(c.vocab - plan.last, kTile) : 0;
+    keep.slice_first = plan.stats_tiles * plan.per_tile;
     keep.grad = reinterpret_cast<uint16_t*>(work + plan.grad);
-    keep.grad_stride = static_cast<uint64_t>(plan.piece) * plan.parts;
+    keep.grad_stride = static_cast<uint64_t>(plan.piece) * plan.words;
     if (stats.a_tiles != 0 && (status = product<Use::Stats>(plan, stats, stream)) != hipSuccess) return status;
-    if (keeps && (status = product<Use::Keep>(plan, keep, stream)) != hipSuccess) return status;
+    if (plan.keeps && (status = product<Use::Keep>(plan, keep, stream)) != hipSuccess) return status;
     const auto lse_of = [&](auto tokens) {
         constexpr uint32_t kTokens = decltype(tokens)::value;
         hipLaunchKernelGGL(loss_lse_kernel<kTokens>, dim3(ceil_div(c.n, kTokens)), dim3(kLseThreads), 0, stream, stats.slices, plan.slices, plan.n_pad,
@@ -1188,19 +1309,26 @@ hipError_t run(const LossCall& c, hipStream_t stream) {
     if (failed(status)) return status;
     if (!gradients) return hipSuccess;
 
+    const uint32_t gw_tile = plan.parts == 3 ? kFewTile : kTile, gw_rows = plan.parts == 1 ? 256 : plan.parts == 2 ? 128 : 64;
     for (uint32_t piece = plan.pieces; piece-- > 0;) {
         const uint32_t first = piece * plan.piece, count = c.vocab - first < plan.piece ? c.vocab - first : plan.piece;
         Product grad = keep;
-        if (first == last) {
-            const uint32_t columns = padded(count, kTile), slice_rows = plan.vocab_tile / plan.per_tile, across = ceil_div(columns, 8 * kTurnThreads);
-            const dim3 grid(across * padded(c.n, 64));
+        if (first == plan.last) {
+            const uint32_t columns = padded(count, kTile), across = ceil_div(columns, 8 * kTurnThreads), slice_rows = plan.vocab_tile / plan.per_tile;
             const float2* slices = stats.slices + static_cast<uint64_t>(keep.slice_first) * plan.n_pad;
-            if (plan.parts == 1) hipLaunchKernelGGL(loss_turn_kernel<1>, grid, dim3(kTurnThreads), 0, stream, grad.grad, grad.grad_stride, first, columns, across, slices, slice_rows, plan.n_pad, lse, labels, meta);
-            else hipLaunchKernelGGL(loss_turn_kernel<2>, grid, dim3(kTurnThreads), 0, stream, grad.grad, grad.grad_stride, first, columns, across, slices, slice_rows, plan.n_pad, lse, labels, meta);
+            const auto turn = [&](auto parts) {
+                constexpr int kParts = decltype(parts)::value;
+                hipLaunchKernelGGL(loss_turn_kernel<kParts>, dim3(across * padded(c.n, 64)), dim3(kTurnThreads), 0, stream, grad.grad, grad.grad_stride,
+                                   first, columns, across, slices, plan.height, plan.per_tile, slice_rows, plan.n_pad, lse, labels, meta);
+            };
+            if (plan.parts == 1) turn(std::integral_constant<int, 1>{});
+            else if (plan.parts == 2) turn(std::integral_constant<int, 2>{});
+            else turn(std::integral_constant<int, 3>{});
             if (failed(status)) return status;
         } else {
             grad.a_first = first;
-            grad.a_tiles = padded(count, kTile) / plan.vocab_tile;
+            grad.a_columns_out = padded(count, kTile);
+            grad.a_tiles = ceil_div(grad.a_columns_out, plan.height);
             if ((status = product<Use::Grad>(plan, grad, stream)) != hipSuccess) return status;
         }
 
@@ -1231,8 +1359,8 @@ hipError_t run(const LossCall& c, hipStream_t stream) {
         gw.b_columns = plan.piece;
         gw.a_count = c.d;
         gw.b_count = count;
-        gw.a_tiles = ceil_div(c.d, kTile);
-        gw.b_tiles = ceil_div(count, plan.parts == 1 ? 256 : 128);
+        gw.a_tiles = ceil_div(c.d, gw_tile);
+        gw.b_tiles = ceil_div(count, gw_rows);
         gw.out = static_cast<T*>(c.gw) + static_cast<uint64_t>(first) * c.d;
         gw.out_stride = c.d;
         gw.out_whole = c.d % (16 / sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(c.gw) % 16 == 0;

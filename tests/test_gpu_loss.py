@@ -108,6 +108,25 @@ def test_a_vocabulary_in_pieces():
 
 
 @pytest.mark.parametrize("dtype", (BF16, F32))
+@pytest.mark.parametrize("n,vocab", [(7, 1500), (64, 2049), (65, 1500), (300, 2300), (600, 1281)])
+def test_small_pieces(n, vocab, dtype):
+    """Pieces of 256 and of 512 vocabulary rows: the same losses, the same gradients within their bounds."""
+    x, weight, labels = make(n, 136, vocab, dtype, ignored=0.2, seed=14)
+    ref = reference(x, weight, labels)
+    rows = -(-n // 64) * 64 if n <= 64 else -(-n // 256) * 256
+    for piece in (1, 512 * rows * (2 if dtype == BF16 else 4)):
+        head = HeadLoss(weight, piece_bytes=piece)
+        check_step(head.step(x, labels), ref, x, weight, int((labels != IGNORE).sum()))
+        assert head.workspace_bytes() < HeadLoss(weight, max_tokens=n).workspace_bytes() + 64 * rows * 136 * 4 + 512 * rows * 8 + (1 << 16)
+
+
+@pytest.mark.parametrize("n,d,vocab", [(1, 1024, 50304), (3, 36, 513), (64, 2052, 700), (33, 30, 90), (17, 96, 66000)])
+def test_a_few_float32_tokens(n, d, vocab):
+    """Float32 weights read as they are (rows of whole 16-byte pieces) or from a padded copy."""
+    run_both(n, d, vocab, F32, seed=15)
+
+
+@pytest.mark.parametrize("dtype", (BF16, F32))
 def test_every_token_ignored(dtype):
     x, weight, _ = make(70, 96, 500, dtype)
     labels = torch.full((70,), IGNORE, device="cuda")
@@ -281,6 +300,6 @@ def test_refusals(device):
                 call(bad, at)
     for make_head, match in ((lambda: HeadLoss(weight.T), "contiguous"), (lambda: HeadLoss(weight[:0]), "non-empty"),
                              (lambda: HeadLoss(weight.half()), "float32 or bfloat16"), (lambda: HeadLoss(weight, reduction="none"), "reduction"),
-                             (lambda: HeadLoss(weight, max_tokens=0), "N=0"), (lambda: HeadLoss(weight[0]), "contiguous")):
+                             (lambda: HeadLoss(weight, max_tokens=0), "N=0"), (lambda: HeadLoss(weight, piece_bytes=0), "piece_bytes"), (lambda: HeadLoss(weight[0]), "contiguous")):
         with pytest.raises(ValueError, match=match):
             make_head()
