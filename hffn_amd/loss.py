@@ -3,10 +3,9 @@ mean loss with the gradients of the hidden rows and of the head's weight (a trai
 
 For hidden rows ``x [N, d]``, a weight ``[V, d]`` and labels: ``l_t = log sum_v exp(x_t . w_v) - x_t . w_label(t)``; with
 ``p = softmax(x W^T)`` and ``D = (p - onehot) / counted``: ``gx = D W``, ``gw = D^T x``. Logits are computed in pieces of the
-vocabulary and not kept: the sums of exponentials first, then piece by piece the softmax (16 bits an entry, float32: 32)
-and its two products. Tokens whose label
-is ``ignore_index`` take no part: their losses and rows of ``gx`` are zero whatever their rows of x hold, and the products
-run over the others alone.
+vocabulary and not kept: the sums of exponentials first, then piece by piece the softmax (16 bits an entry,
+float32: 32) and its two products. Tokens whose label is ``ignore_index`` take no part: their losses and rows of ``gx``
+are zero whatever their rows of x hold, and the products run over the others alone.
 
     head = HeadLoss(weight, max_tokens=2048)          # weight [V, d] float32 or bfloat16 on the GPU, read at every call
     losses = head.losses(x, labels)                   # float32 [N]
@@ -40,7 +39,7 @@ def rows_of(t: torch.Tensor, name: str, width: int, dtype: torch.dtype) -> tuple
 
 
 class HeadLoss:
-    """The loss of one head (see the module docstring). Buffers are the object's own, sized for the largest N seen; what a
+    """The loss of one head (see the module docstring). Buffers are the object's own and grow with the calls; what a
     call returns are views of them that the next call overwrites. Calls are queued on PyTorch's current stream; calls of one
     object on several streams have to be ordered by the caller."""
 
@@ -71,17 +70,17 @@ class HeadLoss:
         self._loss: torch.Tensor | None = None
         self.grad: torch.Tensor | None = None  # gw of the last step
         self._stream: int | None = None
-        self._reserved = [0, 0]  # tokens the buffers hold, for losses and for step
+        self._sized = [0, 0]  # tokens the buffers were last sized for, for losses and for step (more may need less: fewer pieces)
         self.reserve(max_tokens, gradients=False)
 
     def _bytes(self, n: int, gradients: bool) -> int:
         return _lib.query_bytes(self._lib.hffn_loss_workspace, self.value_type, n, self.d_model, self.vocab, self._aligned, int(gradients), self.piece_bytes)
 
     def reserve(self, n: int, gradients: bool = True) -> None:
-        """Size the buffers for calls of up to ``n`` tokens (``gradients``: for ``step`` too); allocates what must grow."""
+        """Size the buffers for calls of ``n`` tokens (``gradients``: for ``step`` too); allocates what must grow."""
         if not 1 <= n <= MAX_TOKENS:
             raise ValueError(f"N={n} outside [1, {MAX_TOKENS}]")
-        if n <= self._reserved[gradients]:
+        if n == self._sized[gradients]:
             return
         need = self._bytes(n, gradients)
         if self._workspace is None or self._workspace.numel() < need:
@@ -93,7 +92,7 @@ class HeadLoss:
         if gradients and self.grad is None:
             self.grad = torch.empty_like(self.weight)
             self._loss = torch.empty((), device=self.device)
-        self._reserved[gradients] = n
+        self._sized[gradients] = n
 
     def workspace_bytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in (self._workspace, self._losses, self._gx) if t is not None)

@@ -120,6 +120,18 @@ def test_small_pieces(n, vocab, dtype):
         assert head.workspace_bytes() < HeadLoss(weight, max_tokens=n).workspace_bytes() + 64 * rows * 136 * 4 + 512 * rows * 8 + (1 << 16)
 
 
+@pytest.mark.parametrize("dtype", (BF16, F32))
+def test_fewer_tokens_may_need_more_workspace(dtype):
+    """Fewer tokens run in fewer, larger pieces: calls of any order on one object, each with the workspace it needs."""
+    x, weight, labels = make(900, 64, 2000, dtype, seed=21)
+    head = HeadLoss(weight, piece_bytes=800000)
+    bytes_of = []
+    for n in (300, 65, 64, 900, 700):
+        bytes_of.append(head._bytes(n, True))
+        check_step(head.step(x[:n], labels[:n]), reference(x[:n], weight, labels[:n]), x[:n], weight, n)
+    assert bytes_of[1] < bytes_of[2] or bytes_of[3] < bytes_of[4]
+
+
 @pytest.mark.parametrize("n,d,vocab", [(1, 1024, 50304), (3, 36, 513), (64, 2052, 700), (33, 30, 90), (17, 96, 66000)])
 def test_a_few_float32_tokens(n, d, vocab):
     """Float32 weights read as they are (rows of whole 16-byte pieces) or from a padded copy."""
