@@ -1069,14 +1069,15 @@ __global__ __launch_bounds__(kTurnThreads) void loss_turn_kernel(uint16_t* __res
     }
 }
 
-// gx of every token: the splits' sums in order times the factor; zeros for tokens that do not count. A wave per token,
-// four entries a lane and step (the partials' rows are padded to whole steps' quarters). The last block: the loss, the
-// tokens' losses added in a fixed order.
-constexpr uint32_t kFinishThreads = 256, kFinishRows = kFinishThreads / kWave;
-template <typename T>
+// gx of every token: the splits' sums in order times the factor; zeros for tokens that do not count. A wave per token and 256
+// columns, four a lane; from kFinishWaves splits on a block, each wave every fourth of the splits (ways), the waves' sums added
+// in order (one token, 64 splits of 1024 columns: 5 us, 35 by one wave). The last block: the loss, the tokens' losses added
+// in a fixed order.
+constexpr uint32_t kFinishThreads = 256, kFinishWaves = kFinishThreads / kWave, kFinishColumns = 4 * kWave;
+template <typename T, uint32_t WAYS>
 __global__ __launch_bounds__(kFinishThreads) void loss_finish_kernel(const float* __restrict__ partial, uint32_t splits, uint32_t n_pad, uint32_t width,
-                                                                    const int32_t* __restrict__ place, const Meta* __restrict__ meta, uint32_t n,
-                                                                    uint32_t d, float scale, bool mean, const float* __restrict__ losses,
+                                                                    const int32_t* __restrict__ place, const Meta* __restrict__ meta,
+                                                                    uint32_t n, uint32_t d, float scale, bool mean, const float* __restrict__ losses,
                                                                     float* __restrict__ loss, T* __restrict__ gx, bool whole) {
     const Meta m = *meta;
     if (blockIdx.x == gridDim.x - 1) {
@@ -1093,38 +1094,39 @@ __global__ __launch_bounds__(kFinishThreads) void loss_finish_kernel(const float
         if (threadIdx.x == 0) *loss = static_cast<float>(mean && m.valid != 0 ? lds[0] / m.valid : lds[0]);
         return;
     }
-    const uint32_t t = blockIdx.x * kFinishRows + threadIdx.x / kWave;
-    if (t >= n) return;
-    const int32_t row = place[t];
+    __shared__ Four sums[kFinishWaves][kWave];
+    const uint32_t lane = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave), across = (d + kFinishColumns - 1) / kFinishColumns;
+    const uint32_t unit = blockIdx.x * (kFinishWaves / WAYS) + wave / WAYS, t = unit / across, c = unit % across * kFinishColumns + 4 * lane;
+    const int32_t row = t < n ? place[t] : -1;
     const float factor = grad_factor(m, scale, mean);
-    const float* from = partial + static_cast<uint64_t>(row < 0 ? 0 : row) * width;
-    const uint64_t next = static_cast<uint64_t>(n_pad) * width;
-    T* to = gx + static_cast<uint64_t>(t) * d;
-    for (uint32_t c = 4 * (threadIdx.x % kWave); c < d; c += 4 * kWave) {
-        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (row >= 0) {
+    Four v = 0.0f;
+    if (row >= 0 && c < d) {
+        const float* from = partial + static_cast<uint64_t>(row) * width + c;
+        const uint64_t next = static_cast<uint64_t>(n_pad) * width;
 #pragma unroll 4
-            for (uint32_t s = 0; s < splits; ++s) {
-                const float4 part = *reinterpret_cast<const float4*>(from + s * next + c);
-                v[0] += part.x; v[1] += part.y; v[2] += part.z; v[3] += part.w;
+        for (uint32_t s = wave % WAYS; s < splits; s += WAYS) v += *reinterpret_cast<const Four*>(from + s * next);
+    }
+    if constexpr (WAYS != 1) {
+        sums[wave][lane] = v;
+        __syncthreads();
+        if (wave != 0) return;
+#pragma unroll
+        for (uint32_t w = 1; w < kFinishWaves; ++w) v += sums[w][lane];
+    }
+    if (t >= n || c >= d) return;
+    if (row >= 0) v *= factor;
+    else if (m.invalid != 0) v = factor;  // NaN: a label was outside the vocabulary
+    T* to = gx + static_cast<uint64_t>(t) * d + c;
+    if (whole) {
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<Four*>(to) = v;
+        else *reinterpret_cast<uint2*>(to) = make_uint2(bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]));
+    } else {
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k)
+            if (c + k < d) {
+                if constexpr (sizeof(T) == 4) to[k] = v[k];
+                else to[k] = bf16_bits(v[k]);
             }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] *= factor;
-        } else if (m.invalid != 0) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] = factor;  // NaN: a label was outside the vocabulary
-        }
-        if (whole) {
-            if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(to + c) = make_float4(v[0], v[1], v[2], v[3]);
-            else *reinterpret_cast<uint2*>(to + c) = make_uint2(bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]));
-        } else {
-#pragma unroll
-            for (uint32_t k = 0; k < 4; ++k)
-                if (c + k < d) {
-                    if constexpr (sizeof(T) == 4) to[c + k] = v[k];
-                    else to[c + k] = bf16_bits(v[k]);
-                }
-        }
     }
 }
 
@@ -1367,9 +1369,15 @@ hipError_t run(const LossCall& c, hipStream_t stream) {
         if ((status = product<Use::GradW>(plan, gw, stream)) != hipSuccess) return status;
     }
     const bool whole = c.d % 4 == 0 && reinterpret_cast<uintptr_t>(c.gx) % 16 == 0;
-    hipLaunchKernelGGL(loss_finish_kernel<T>, dim3(ceil_div(c.n, kFinishRows) + 1), dim3(kFinishThreads), 0, stream,
-                       reinterpret_cast<const float*>(work + plan.partial), plan.splits, plan.n_pad, plan.width, place, meta, c.n, c.d, c.scale, c.mean,
-                       losses, c.loss, static_cast<T*>(c.gx), whole);
+    const auto finish = [&](auto ways) {
+        constexpr uint32_t kWays = decltype(ways)::value;
+        const uint32_t blocks = ceil_div(static_cast<uint64_t>(c.n) * ceil_div(c.d, kFinishColumns), kFinishWaves / kWays);
+        hipLaunchKernelGGL((loss_finish_kernel<T, kWays>), dim3(blocks + 1), dim3(kFinishThreads), 0, stream,
+                           reinterpret_cast<const float*>(work + plan.partial), plan.splits, plan.n_pad, plan.width, place, meta, c.n, c.d, c.scale, c.mean,
+                           losses, c.loss, static_cast<T*>(c.gx), whole);
+    };
+    if (plan.splits < kFinishWaves) finish(std::integral_constant<uint32_t, 1>{});
+    else finish(std::integral_constant<uint32_t, kFinishWaves>{});
     return hipGetLastError();
 }
 
