@@ -83,7 +83,7 @@ struct Prepare {
     int32_t *rows, *compact, *place;
     float* losses;
     Meta* meta;
-    uint16_t *x_out, *w_out;
+    uint16_t *x_out, *w_out, *x_split;  // x_split: RAW, the counted rows of x as per 32 entries 3 x 32 bfloat16 parts
     uint32_t *x_most, *w_most;  // float32: largest finite magnitude of each block's rows, bits
     uint32_t x_blocks, w_blocks;
 };
@@ -175,10 +175,21 @@ __device__ __forceinline__ uint32_t sample_of(const Prepare& p, bool of_x, uint3
     return block_most(most, lds);
 }
 
+// A float32 as three bfloat16 parts whose sum it is to 2^-24: the pair (low, high)'s into words[0..2].
+__device__ __forceinline__ void split_pair(float low, float high, uint32_t (&words)[3]) {
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+        words[p] = bf16_pair(low, high);
+        low -= __uint_as_float(words[p] << 16);
+        high -= __uint_as_float(words[p] & 0xffff0000u);
+    }
+}
+
 // One operand row by a wave, eight entries a lane and step; returns the largest finite magnitude that the lane saw. RAW:
-// float32 as they are.
+// float32 as they are, and where `split_to` is given their parts there.
 template <typename T, bool RAW>
-__device__ __forceinline__ uint32_t pack_row(const T* __restrict__ from, uint16_t* __restrict__ to, uint32_t d, uint32_t width, int e) {
+__device__ __forceinline__ uint32_t pack_row(const T* __restrict__ from, uint16_t* __restrict__ to, uint32_t d, uint32_t width, int e,
+                                             uint16_t* __restrict__ split_to = nullptr) {
     const uint32_t lane = threadIdx.x % kWave;
     const bool whole = reinterpret_cast<uintptr_t>(from) % 16 == 0;
     uint32_t most = 0;
@@ -195,6 +206,14 @@ __device__ __forceinline__ uint32_t pack_row(const T* __restrict__ from, uint16_
                 float4* out = reinterpret_cast<float4*>(to + 2 * c);
                 out[0] = make_float4(v[0], v[1], v[2], v[3]);
                 out[1] = make_float4(v[4], v[5], v[6], v[7]);
+                if (split_to == nullptr) continue;
+                uint32_t words[4][3];
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k) split_pair(v[2 * k], v[2 * k + 1], words[k]);
+#pragma unroll
+                for (uint32_t part = 0; part < 3; ++part)
+                    *reinterpret_cast<uint4*>(split_to + c / 32 * 96 + part * 32 + c % 32) =
+                        make_uint4(words[0][part], words[1][part], words[2][part], words[3][part]);
                 continue;
             }
             uint32_t hi[4], lo[4];
@@ -320,10 +339,17 @@ __global__ __launch_bounds__(kPrepThreads) void loss_prepare_kernel(Prepare p) {
         if (blockIdx.x == 0 && threadIdx.x == 0) p.meta->x_sample = sample;
     }
     uint32_t most = 0;
-    if (counted) most = pack_row<T, RAW>(static_cast<const T*>(p.x) + i * p.x_stride, p.x_out + at * kParts * p.width, p.d, p.width, e);
+    uint16_t* const split_rows = RAW ? p.x_split : nullptr;
+    if (counted)
+        most = pack_row<T, RAW>(static_cast<const T*>(p.x) + i * p.x_stride, p.x_out + at * kParts * p.width, p.d, p.width, e,
+                                RAW ? split_rows + static_cast<uint64_t>(at) * 3 * p.width : nullptr);
     if (i >= valid && i < (valid + 63) / 64 * 64) {
         uint4* out = reinterpret_cast<uint4*>(p.x_out + i * kParts * p.width);
         for (uint32_t c = lane; c < kParts * p.width / 8; c += kWave) out[c] = make_uint4(0, 0, 0, 0);
+        if constexpr (RAW) {
+            uint4* parts = reinterpret_cast<uint4*>(split_rows + static_cast<uint64_t>(i) * 3 * p.width);
+            for (uint32_t c = lane; c < 3 * p.width / 8; c += kWave) parts[c] = make_uint4(0, 0, 0, 0);
+        }
     }
     if constexpr (kScaled) {
         const uint32_t all = block_most(most, most_lds);
@@ -466,6 +492,42 @@ struct Operand {
     }
 };
 
+// float32 entries already split into three bfloat16 parts (memory: per 32 entries 3 x 32), index-major, in LDS as a plane of
+// TILE x 64 bytes a part: x's rows for the weight's products, which every wave of a block reads (splitting them where they are
+// read took four waves' time: one token, 6400 rows of 1024: a call of 61 us).
+template <int TILE, int WAVES>
+struct SplitOperand {
+    static constexpr uint32_t kPlane = TILE * 64, kBytes = 3 * kPlane, kPieces = kBytes / 1024, kPerWave = kPieces / WAVES, kDepth = 32;
+    static_assert(kPieces % WAVES == 0 && kPlane % 1024 == 0, "every wave transfers as many pieces, each of one plane");
+
+    const char* base;
+    uint32_t offset[kPerWave];
+
+    __device__ __forceinline__ static uint32_t swizzle(uint32_t r) { return ((r >> 1 ^ r >> 2) & 1) | (r >> 4 & 1) << 1; }
+    __device__ __forceinline__ void begin(const uint16_t* p, uint64_t row_entries, uint32_t first, uint32_t indexes, uint32_t) {
+        const uint32_t wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, left = indexes - first - 1;
+        base = reinterpret_cast<const char*>(p) + first * row_entries * 2;
+#pragma unroll
+        for (uint32_t j = 0; j < kPerWave; ++j) {
+            const uint32_t at = (wave * kPerWave + j) * 1024 + lane * 16, part = at / kPlane, r = at % kPlane / 64, chunk = at % 64 / 16 ^ swizzle(r);
+            offset[j] = min(r, left) * static_cast<uint32_t>(row_entries * 2) + part * 64 + chunk * 16;
+        }
+    }
+    __device__ __forceinline__ void fetch(uint32_t kt, const char* lds) const {
+        const uint32_t wave = uniform(threadIdx.x / kWave);
+        const char* from = base + kt * 192;
+#pragma unroll
+        for (uint32_t j = 0; j < kPerWave; ++j) dma16(from, offset[j], lds + (wave * kPerWave + j) * 1024);
+    }
+    __device__ __forceinline__ static uint32_t place(uint32_t first) {
+        const uint32_t lane = threadIdx.x % kWave, r = first + permuted(lane % 32);
+        return r * 64 + (lane / 32 ^ swizzle(r)) * 16;
+    }
+    __device__ __forceinline__ static Frag read(uint32_t tile, uint32_t place, int i, int step, int part) {
+        return *reinterpret_cast<LdsFrag>(tile + part * kPlane + i * 2048 + (place ^ (step * 32)));
+    }
+};
+
 // The same entries as `count` MFMA operands: the parts as read, or three bfloat16 ones whose sum is the float32 to 2^-24.
 template <int PARTS>
 struct Parts {
@@ -484,22 +546,13 @@ struct Raw {
         value = OP::read_raw(tile, place, i, step);
     }
     __device__ __forceinline__ Parts<3> parts() const {
-        uint32_t words[3][4];
+        uint32_t words[4][3];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            float low = value[2 * k], high = value[2 * k + 1];
-#pragma unroll
-            for (int p = 0; p < 3; ++p) {
-                const uint32_t pair = bf16_pair(low, high);
-                words[p][k] = pair;
-                low -= __uint_as_float(pair << 16);
-                high -= __uint_as_float(pair & 0xffff0000u);
-            }
-        }
+        for (int k = 0; k < 4; ++k) split_pair(value[2 * k], value[2 * k + 1], words[k]);
         Parts<3> out;
 #pragma unroll
         for (int p = 0; p < 3; ++p) {
-            const Words w{words[p][0], words[p][1], words[p][2], words[p][3]};
+            const Words w{words[0][p], words[1][p], words[2][p], words[3][p]};
             out.part[p] = __builtin_bit_cast(Frag, w);
         }
         return out;
@@ -558,9 +611,11 @@ struct Shape {
     static constexpr bool kATr = USE == Use::GradX || USE == Use::GradW, kBTr = USE == Use::GradW;
     static constexpr int kA = WA * TA * 32, kB = WB * TB * 32, kWaves = WA * WB;
     using OpA = Operand<PARTS, kATr, kA, kWaves>;
-    using OpB = Operand<PARTS, kBTr, kB, kWaves>;
+    // float32 as it is: x's rows come split, D's do not
+    static constexpr bool kBSplit = PARTS == 3 && USE != Use::GradX && USE != Use::GradW;
+    using OpB = typename std::conditional<kBSplit, SplitOperand<kB, kWaves>, Operand<PARTS, kBTr, kB, kWaves>>::type;
     static constexpr uint32_t kStage = OpA::kBytes + OpB::kBytes, kTransfers = OpA::kPerWave + OpB::kPerWave;
-    static constexpr int kStages = kWaves == 4 ? 3 : 163840 / kStage < 4 ? 163840 / kStage : 4;  // 4 waves: two blocks a CU
+    static constexpr int kStages = kWaves == 4 ? 81920 / kStage : 163840 / kStage < 4 ? 163840 / kStage : 4;  // 4 waves: two blocks a CU
     static constexpr uint32_t kLds = kStage * kStages;
     static_assert(kStages >= 2, "two stages at least");
 };
@@ -672,8 +727,8 @@ __device__ __forceinline__ void accumulate(const Tile<S>& tile, const char* ring
         if constexpr (PARTS != 1) return chain[i][j];
         else return sums[i][j];
     };
-    using Read = typename std::conditional<PARTS == 3, Raw, Parts<PARTS>>::type;
-    Read fa[2][TA], fb[2][TB];
+    typename std::conditional<PARTS == 3, Raw, Parts<PARTS>>::type fa[2][TA];
+    typename std::conditional<PARTS == 3 && !S::kBSplit, Raw, Parts<PARTS>>::type fb[2][TB];
     const auto read = [&](uint32_t kt, int step, int to) {
         const uint32_t tile_a = lds + (kt - k_begin) % S::kStages * S::kStage, tile_b = tile_a + S::OpA::kBytes;
 #pragma unroll
@@ -1144,7 +1199,7 @@ uint32_t padded(uint32_t v, uint32_t to) { return ceil_div(v, to) * to; }
 struct Plan {
     uint32_t parts, words, n_pad, width, vocab_tile, token_tile, height, per_tile, slices, piece, pieces, last, stats_tiles, keep_tiles, splits;
     bool few, in_place, keeps;
-    uint64_t meta, rows, labels, place, lse, picked, losses, slice_sums, x_most, w_most, x, weight, grad, partial, bytes;
+    uint64_t meta, rows, labels, place, lse, picked, losses, slice_sums, x_most, w_most, x, x_split, weight, grad, partial, bytes;
 };
 
 // `aligned`: the weight starts on a 16-byte boundary (weights of whole 16-byte pieces are then read in place, but for parts 2).
@@ -1200,6 +1255,7 @@ Plan plan_of(int vt, uint32_t n, uint32_t d, uint32_t vocab, bool aligned, bool 
         p.w_most = take(4ull * ceil_div(vocab, kWeightRows));
     }
     p.x = take(2ull * p.words * p.n_pad * p.width);
+    p.x_split = p.parts == 3 ? take(6ull * p.n_pad * p.width) : 0;
     p.weight = p.in_place ? 0 : take(2ull * p.words * vocab * p.width);
     if (gradients) {
         // splits of the vocabulary that give every CU a block (few tokens: two), each of 8 k-tiles at least
@@ -1246,7 +1302,7 @@ hipError_t run(const LossCall& c, hipStream_t stream) {
     hipError_t status;
 
     const Prepare prepare{c.labels, c.x, c.weight, c.labels_stride, c.ignore, c.x_stride, c.wide_labels, c.n, c.d, plan.width, c.vocab, rows, labels,
-                          place, losses, meta, x, reinterpret_cast<uint16_t*>(work + plan.weight),
+                          place, losses, meta, x, reinterpret_cast<uint16_t*>(work + plan.weight), reinterpret_cast<uint16_t*>(work + plan.x_split),
                           reinterpret_cast<uint32_t*>(work + plan.x_most), reinterpret_cast<uint32_t*>(work + plan.w_most),
                           ceil_div(padded(c.n, 64), kPrepWaves), plan.in_place ? 0 : ceil_div(c.vocab, kWeightRows)};
     if (c.n > kScanTokens) {
@@ -1279,8 +1335,8 @@ hipError_t run(const LossCall& c, hipStream_t stream) {
     stats.a = weight;
     stats.a_stride = w_row;
     stats.a_columns = w_columns;
-    stats.b = x;
-    stats.b_stride = x_row;
+    stats.b = plan.parts == 3 ? reinterpret_cast<const uint16_t*>(work + plan.x_split) : x;
+    stats.b_stride = plan.parts == 3 ? 3ull * plan.width : x_row;
     stats.b_columns = plan.width;
     stats.k_tiles = plan.width / depth;
     stats.a_tiles = plan.stats_tiles;
