@@ -186,7 +186,7 @@ __device__ __forceinline__ void split_pair(float low, float high, uint32_t (&wor
 }
 
 // One operand row by a wave, eight entries a lane and step; returns the largest finite magnitude that the lane saw. RAW:
-// float32 as they are, and where `split_to` is given their parts there.
+// float32 as they are, and their parts to `split_to`.
 template <typename T, bool RAW>
 __device__ __forceinline__ uint32_t pack_row(const T* __restrict__ from, uint16_t* __restrict__ to, uint32_t d, uint32_t width, int e,
                                              uint16_t* __restrict__ split_to = nullptr) {
@@ -206,7 +206,6 @@ __device__ __forceinline__ uint32_t pack_row(const T* __restrict__ from, uint16_
                 float4* out = reinterpret_cast<float4*>(to + 2 * c);
                 out[0] = make_float4(v[0], v[1], v[2], v[3]);
                 out[1] = make_float4(v[4], v[5], v[6], v[7]);
-                if (split_to == nullptr) continue;
                 uint32_t words[4][3];
 #pragma unroll
                 for (uint32_t k = 0; k < 4; ++k) split_pair(v[2 * k], v[2 * k + 1], words[k]);
@@ -247,13 +246,13 @@ __device__ __forceinline__ uint32_t pack_row(const T* __restrict__ from, uint16_
 }
 
 // The weight's rows of block `block`; returns the thread's largest magnitude.
-template <typename T, bool RAW>
+template <typename T>
 __device__ __forceinline__ uint32_t pack_weight(const Prepare& p, uint32_t block, int e) {
     constexpr uint64_t kParts = sizeof(T) == 4 ? 2 : 1;
     uint32_t most = 0;
     for (uint32_t r = threadIdx.x / kWave; r < kWeightRows; r += kPrepWaves) {
         const uint64_t row = static_cast<uint64_t>(block) * kWeightRows + r;
-        if (row < p.vocab) most = max(most, pack_row<T, RAW>(static_cast<const T*>(p.weight) + row * p.d, p.w_out + row * kParts * p.width, p.d, p.width, e));
+        if (row < p.vocab) most = max(most, pack_row<T, false>(static_cast<const T*>(p.weight) + row * p.d, p.w_out + row * kParts * p.width, p.d, p.width, e));
     }
     return most;
 }
@@ -266,7 +265,7 @@ __global__ __launch_bounds__(kPrepThreads) void loss_prepare_kernel(Prepare p) {
     constexpr bool kScaled = sizeof(T) == 4 && !RAW;
     __shared__ uint32_t most_lds[kPrepWaves], sums[kPrepWaves][3];
     const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    if (blockIdx.x >= p.x_blocks) {
+    if (!RAW && blockIdx.x >= p.x_blocks) {
         const uint32_t block = blockIdx.x - p.x_blocks;
         int e = 0;
         if constexpr (kScaled) {
@@ -274,7 +273,7 @@ __global__ __launch_bounds__(kPrepThreads) void loss_prepare_kernel(Prepare p) {
             e = lift_of(sample);
             if (block == 0 && threadIdx.x == 0) p.meta->weight_sample = sample;
         }
-        const uint32_t most = pack_weight<T, RAW>(p, block, e);
+        const uint32_t most = pack_weight<T>(p, block, e);
         if constexpr (kScaled) {
             const uint32_t all = block_most(most, most_lds);
             if (threadIdx.x == 0) p.w_most[block] = all;
@@ -378,7 +377,7 @@ __global__ __launch_bounds__(kPrepThreads) void loss_settle_kernel(Prepare p) {
             pack_row<float, false>(static_cast<const float*>(p.x) + p.rows[i] * p.x_stride, p.x_out + static_cast<uint64_t>(i) * 2 * p.width, p.d, p.width,
                      lift_of(x_bits));
     if (w_bits != w_sample)
-        for (uint32_t block = blockIdx.x; block < p.w_blocks; block += gridDim.x) pack_weight<float, false>(p, block, lift_of(w_bits));
+        for (uint32_t block = blockIdx.x; block < p.w_blocks; block += gridDim.x) pack_weight<float>(p, block, lift_of(w_bits));
 }
 
 // --------------------------------------------------------------------------------------------------------- the product
@@ -1188,14 +1187,19 @@ __global__ __launch_bounds__(kFinishThreads) void loss_finish_kernel(const float
 // ------------------------------------------------------------------------------------------------------------ the host
 
 constexpr uint32_t kTile = 256;                      // vocabulary rows and width of a tile
-constexpr uint32_t kFewTokens = 64, kFewTile = 128;  // up to so many tokens: tiles of 128 x 64, two blocks a CU
+constexpr uint32_t kFewTokens = 64, kFewTile = 128;  // a few tokens: tiles of 128 x 64, two blocks a CU
+constexpr uint32_t kFewRows = 16384;                 // float32: vocabulary rows from which reading them as they are pays
 constexpr uint32_t kCus = 256;
 
 uint32_t ceil_div(uint64_t a, uint32_t b) { return static_cast<uint32_t>((a + b - 1) / b); }
 uint32_t padded(uint32_t v, uint32_t to) { return ceil_div(v, to) * to; }
 
 // How a call runs. parts: 1 bfloat16, 2 float32 as fp16 hi + lo, 3 float32 as three bfloat16 parts split where they are
-// multiplied. A few tokens wait for the weight, not for the matrix unit: packing it would read and write it once more.
+// multiplied. A few tokens wait for the weight, not for the matrix unit, and packing it reads and writes it once more: float32
+// calls then read it as it is (it has to be made of whole 16-byte pieces). Losses, width 1024, as it is against packed: 1
+// token of 50304 rows 67 against 161 us, 128 tokens 110 / 159, 192 156 / 195, 256 202 / 202; of 32768 rows 128 tokens 107 /
+// 115, 192 151 / 126; of 16384 rows 64 tokens 58 / 62, 128 102 / 64; of 10000 rows 64 tokens 57 / 48. Steps gain less (their
+// products with D split what they read): 64 tokens of 50304 rows 229 / 324 us, 128 362 / 350.
 struct Plan {
     uint32_t parts, words, n_pad, width, vocab_tile, token_tile, height, per_tile, slices, piece, pieces, last, stats_tiles, keep_tiles, splits;
     bool few, in_place, keeps;
@@ -1205,14 +1209,16 @@ struct Plan {
 // `aligned`: the weight starts on a 16-byte boundary (weights of whole 16-byte pieces are then read in place, but for parts 2).
 Plan plan_of(int vt, uint32_t n, uint32_t d, uint32_t vocab, bool aligned, bool gradients, uint64_t piece_bytes) {
     Plan p{};
-    p.few = n <= kFewTokens;
+    p.words = vt == kBF16 ? 1 : 2;
+    const bool whole = d % (8 / p.words) == 0 && aligned;
+    if (vt == kBF16) p.few = n <= kFewTokens;
+    else p.few = whole && (gradients ? n <= kFewTokens && vocab >= kFewRows : n <= 3 * kFewTokens && vocab >= ceil_div(n, kFewTokens) * kFewRows);
     p.parts = vt == kBF16 ? 1 : p.few ? 3 : 2;
-    p.words = p.parts == 1 ? 1 : 2;
     p.vocab_tile = p.few ? kFewTile : kTile;
     p.token_tile = p.few ? kFewTokens : p.parts == 1 ? 256 : 128;
     p.n_pad = padded(n, p.few ? kFewTokens : 256);
     p.width = padded(d, 64 / p.words);
-    p.in_place = p.parts != 2 && d % (8 / p.words) == 0 && aligned;
+    p.in_place = p.parts != 2 && whole;
     p.per_tile = p.parts == 2 ? 8 : 4;  // slices: as many as waves of quarter tiles (few: of tiles) along the vocabulary
     p.pieces = 1;
     p.piece = padded(vocab, kTile);

@@ -138,6 +138,24 @@ def test_a_few_float32_tokens(n, d, vocab):
     run_both(n, d, vocab, F32, seed=15)
 
 
+@pytest.mark.parametrize("ignored", (0.0, 0.4))
+@pytest.mark.parametrize("n,d,vocab", [(1, 4, 16384), (3, 36, 16385), (64, 2052, 16400), (33, 28, 20001), (64, 37, 16400), (65, 36, 33000),
+                                       (128, 100, 32768), (128, 100, 32767), (150, 64, 50304), (192, 8, 49152), (193, 8, 65536)])
+def test_float32_weights_read_as_they_are(n, d, vocab, ignored):
+    """Sizes on both sides of the rule that reads a float32 weight without packing it, with tiles that end anywhere."""
+    run_both(n, d, vocab, F32, ignored=ignored, seed=22)
+
+
+@pytest.mark.parametrize("rows", (256, 4096, 16384))
+def test_pieces_of_a_float32_weight_read_as_it_is(rows):
+    x, weight, labels = make(50, 136, 17000, F32, ignored=0.2, seed=23)
+    head = HeadLoss(weight, piece_bytes=rows * 64 * 4)
+    check_step(head.step(x, labels), reference(x, weight, labels), x, weight, int((labels != IGNORE).sum()))
+    labels.fill_(IGNORE)
+    loss, gx, gw = head.step(x, labels)
+    assert float(loss) == 0.0 and not gx.any() and not gw.any() and not head.losses(x, labels).any()
+
+
 @pytest.mark.parametrize("dtype", (BF16, F32))
 def test_every_token_ignored(dtype):
     x, weight, _ = make(70, 96, 500, dtype)
