@@ -27,6 +27,10 @@ typedef __attribute__((address_space(3))) const Frag* LdsFrag;
 typedef float Four __attribute__((ext_vector_type(4)));
 typedef float Eight __attribute__((ext_vector_type(8)));
 typedef uint32_t Words __attribute__((ext_vector_type(4)));
+// The same 16 bytes where rows start on their entries' boundaries only; the hardware takes these in one access.
+typedef float FourAnywhere __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t WordsAnywhere __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t HalvesAnywhere __attribute__((ext_vector_type(2), aligned(2)));
 typedef __attribute__((address_space(3))) const Four* LdsFour;
 typedef __attribute__((address_space(3))) const float* LdsFloat;
 
@@ -191,13 +195,16 @@ template <typename T, bool RAW>
 __device__ __forceinline__ uint32_t pack_row(const T* __restrict__ from, uint16_t* __restrict__ to, uint32_t d, uint32_t width, int e,
                                              uint16_t* __restrict__ split_to = nullptr) {
     const uint32_t lane = threadIdx.x % kWave;
-    const bool whole = reinterpret_cast<uintptr_t>(from) % 16 == 0;
     uint32_t most = 0;
     for (uint32_t c = 8 * lane; c < width; c += 8 * kWave) {
         if constexpr (sizeof(T) == 4) {
             float v[8];
-            if (whole && c + 8 <= d) {
-                load_vec<8>(from + c, v);
+            if (c + 8 <= d) {
+#pragma unroll
+                for (uint32_t k = 0; k < 8; k += 4) {
+                    const FourAnywhere part = *reinterpret_cast<const FourAnywhere*>(from + c + k);
+                    v[k] = part[0], v[k + 1] = part[1], v[k + 2] = part[2], v[k + 3] = part[3];
+                }
             } else {
 #pragma unroll
                 for (uint32_t k = 0; k < 8; ++k) v[k] = c + k < d ? from[c + k] : 0.0f;
@@ -229,17 +236,17 @@ __device__ __forceinline__ uint32_t pack_row(const T* __restrict__ from, uint16_
             *reinterpret_cast<uint4*>(out) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
             *reinterpret_cast<uint4*>(out + 32) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         } else {
-            uint4 v;
-            if (whole && c + 8 <= d) {
-                v = *reinterpret_cast<const uint4*>(from + c);
+            WordsAnywhere v;
+            if (c + 8 <= d) {
+                v = *reinterpret_cast<const WordsAnywhere*>(from + c);
             } else {
                 uint32_t words[4];
 #pragma unroll
                 for (uint32_t k = 0; k < 8; k += 2)
                     words[k / 2] = (c + k < d ? from[c + k] : 0u) | (c + k + 1 < d ? static_cast<uint32_t>(from[c + k + 1]) : 0u) << 16;
-                v = make_uint4(words[0], words[1], words[2], words[3]);
+                v = WordsAnywhere{words[0], words[1], words[2], words[3]};
             }
-            *reinterpret_cast<uint4*>(to + c) = v;
+            *reinterpret_cast<uint4*>(to + c) = make_uint4(v[0], v[1], v[2], v[3]);
         }
     }
     return most;
@@ -599,7 +606,7 @@ struct Product {
     void* out;                    // GradW: [V, d]
     uint64_t out_stride;
     float scale;
-    bool mean, out_bf16, out_whole;  // out_whole: rows of the output start on 16-byte boundaries and hold whole 16-byte pieces
+    bool mean, out_bf16;
 };
 
 // WA x WB waves of TA x TB 32 x 32 results each; k-tiles go through a ring of kStages tile pairs.
@@ -941,17 +948,15 @@ __device__ __forceinline__ void finish(const Product& p, const Meta& meta, const
                     float v[16];
 #pragma unroll
                     for (int r = 0; r < 16; ++r) v[r] = factor * result(i, j, r);
-                    if (p.out_whole && p.out_bf16) {
+                    if (at_a + 16 <= p.a_count && p.out_bf16) {
 #pragma unroll
                         for (int r = 0; r < 16; r += 8)
-                            if (at_a + r < p.a_count)
-                                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + to + r) =
-                                    make_uint4(bf16_pair(v[r], v[r + 1]), bf16_pair(v[r + 2], v[r + 3]), bf16_pair(v[r + 4], v[r + 5]), bf16_pair(v[r + 6], v[r + 7]));
-                    } else if (p.out_whole) {
+                            *reinterpret_cast<WordsAnywhere*>(static_cast<uint16_t*>(p.out) + to + r) =
+                                WordsAnywhere{bf16_pair(v[r], v[r + 1]), bf16_pair(v[r + 2], v[r + 3]), bf16_pair(v[r + 4], v[r + 5]), bf16_pair(v[r + 6], v[r + 7])};
+                    } else if (at_a + 16 <= p.a_count) {
 #pragma unroll
                         for (int r = 0; r < 16; r += 4)
-                            if (at_a + r < p.a_count)
-                                *reinterpret_cast<float4*>(static_cast<float*>(p.out) + to + r) = make_float4(v[r], v[r + 1], v[r + 2], v[r + 3]);
+                            *reinterpret_cast<FourAnywhere*>(static_cast<float*>(p.out) + to + r) = FourAnywhere{v[r], v[r + 1], v[r + 2], v[r + 3]};
                     } else {
 #pragma unroll
                         for (int r = 0; r < 16; ++r) {
@@ -1132,7 +1137,7 @@ template <typename T, uint32_t WAYS>
 __global__ __launch_bounds__(kFinishThreads) void loss_finish_kernel(const float* __restrict__ partial, uint32_t splits, uint32_t n_pad, uint32_t width,
                                                                     const int32_t* __restrict__ place, const Meta* __restrict__ meta,
                                                                     uint32_t n, uint32_t d, float scale, bool mean, const float* __restrict__ losses,
-                                                                    float* __restrict__ loss, T* __restrict__ gx, bool whole) {
+                                                                    float* __restrict__ loss, T* __restrict__ gx) {
     const Meta m = *meta;
     if (blockIdx.x == gridDim.x - 1) {
         __shared__ double lds[kFinishThreads];
@@ -1171,9 +1176,9 @@ __global__ __launch_bounds__(kFinishThreads) void loss_finish_kernel(const float
     if (row >= 0) v *= factor;
     else if (m.invalid != 0) v = factor;  // NaN: a label was outside the vocabulary
     T* to = gx + static_cast<uint64_t>(t) * d + c;
-    if (whole) {
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<Four*>(to) = v;
-        else *reinterpret_cast<uint2*>(to) = make_uint2(bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]));
+    if (c + 4 <= d) {
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<FourAnywhere*>(to) = v;
+        else *reinterpret_cast<HalvesAnywhere*>(to) = HalvesAnywhere{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3])};
     } else {
 #pragma unroll
         for (uint32_t k = 0; k < 4; ++k)
@@ -1427,16 +1432,14 @@ hipError_t run(const LossCall& c, hipStream_t stream) {
         gw.b_tiles = ceil_div(count, gw_rows);
         gw.out = static_cast<T*>(c.gw) + static_cast<uint64_t>(first) * c.d;
         gw.out_stride = c.d;
-        gw.out_whole = c.d % (16 / sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(c.gw) % 16 == 0;
         if ((status = product<Use::GradW>(plan, gw, stream)) != hipSuccess) return status;
     }
-    const bool whole = c.d % 4 == 0 && reinterpret_cast<uintptr_t>(c.gx) % 16 == 0;
     const auto finish = [&](auto ways) {
         constexpr uint32_t kWays = decltype(ways)::value;
         const uint32_t blocks = ceil_div(static_cast<uint64_t>(c.n) * ceil_div(c.d, kFinishColumns), kFinishWaves / kWays);
         hipLaunchKernelGGL((loss_finish_kernel<T, kWays>), dim3(blocks + 1), dim3(kFinishThreads), 0, stream,
                            reinterpret_cast<const float*>(work + plan.partial), plan.splits, plan.n_pad, plan.width, place, meta, c.n, c.d, c.scale, c.mean,
-                           losses, c.loss, static_cast<T*>(c.gx), whole);
+                           losses, c.loss, static_cast<T*>(c.gx));
     };
     if (plan.splits < kFinishWaves) finish(std::integral_constant<uint32_t, 1>{});
     else finish(std::integral_constant<uint32_t, kFinishWaves>{});
