@@ -4,5 +4,9 @@
 * ``hffn_amd.parity``   - forced-pair parity check (as ``hffn_cuda.parity``)
 * ``hffn_amd.ffn``      - ``cuda_layer``/``hip_layer`` for compact test layers (as ``hffn_ffn_cuda``)
 * ``hffn_amd.synth``    - the seeded compact layers and inputs (test layers of the reference, workload layers)
+* ``hffn_amd.loss``     - ``HeadLoss``: a language-model head's loss and its gradients
+* ``hffn_amd.norm``     - ``ResidualNorm``: residual, gate, post norm and norm between two blocks, forward and backward
+* ``hffn_amd.clip``     - ``grad_norm``, ``clip_grad_norm_``
+* ``hffn_amd.train_lm`` - a small language model trained with these around the layers
 * ``hffn_amd.pythia``   - the Pythia two-arm loader and ``HFFNMLP`` hook (as ``hffn_pythia_cuda``)
 """

@@ -1,6 +1,9 @@
 // The global norm over many tensors and the clipping of their entries to it: two launches per table of kClipArrays arrays.
 // The first leaves one float64 partial per block; every block of the second adds the partials up again (8 KB a table out
 // of L2), so that no block waits for another, and scales its share.
+//
+// Bound by memory: 152 million entries in 98 tensors (506 MB; two tables) take 93 us for the norm, 5.4 TB/s, and 217 us scaled into 609 MB
+// of others, 5.1 TB/s, a copy's rate. 24 tensors of 5 MB: 5.2 and 3.3 us, less than the host's part of the calls (22 us).
 #include <vector>
 
 #include "common.hpp"
@@ -169,8 +172,9 @@ __device__ __forceinline__ void scale_chunk(const T* p, U* out, uint64_t count, 
     for (uint32_t i = before + pieces * V + threadIdx.x; i < all; i += kThreads) put(out + i, factor * widen(p[i]));
 }
 
-// The arrays of one table scaled, last entries first: they were read last and lie in the caches. `count` partials are all tables'. In place with a factor of one nothing is written:
-// every entry would be itself.
+// The arrays of one table scaled, last entries first: they were read last and lie in the caches. What goes to other tensors is
+// stored past the caches (331 -> 311 us of the call above). `count` partials are all tables'. In place with a factor of one
+// nothing is written: every entry would be itself.
 template <bool LARGEST>
 __global__ __launch_bounds__(kThreads) void clip_kernel(Table table, const double* __restrict__ partials, uint32_t count, double limit,
                                                        bool in_place, float* __restrict__ norm) {

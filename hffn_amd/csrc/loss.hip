@@ -2,13 +2,22 @@
 // vocabulary and without keeping the logits:
 //   l_t = log sum_v exp(x_t . w_v) - x_t . w_label(t),   D = softmax - onehot(label),   gx = f D W,   gw = f D^T x,
 // f the gradient's factor (1 / counted tokens for the mean). The forward leaves, per slice of the vocabulary and token, the
-// maximum and the sum of exponentials of its logits; the backward computes a piece's logits again, turns them into D
-// (16 bits) and multiplies D by the weight's rows and by x.
+// maximum and the sum of exponentials of its logits, and of the last piece (of the only one, mostly) the exponentials
+// themselves, where D belongs; the backward turns those into D, computes the other pieces' logits again, and multiplies D
+// by the weight's rows and by x.
 //
 // Every product is out[b][a] = sum_k A[a, k] B[b, k] on 16-bit MFMA operands with float32 sums. bfloat16 calls multiply
 // their entries as they are (D rounded to bfloat16: 2^-8 of an entry, as the gradients themselves are rounded). float32
 // calls hold every operand as fp16 hi + lo of the entry times a power of two of its tensor (22 bits down to 2^-12 of the
-// largest entry) and take hi hi + hi lo + lo hi.
+// largest entry) and take hi hi + hi lo + lo hi; those of a few tokens, which wait for the weight's bytes, read it as it is
+// and split it where it is multiplied into three bfloat16 parts (no power of two to know first), of whose nine products the six
+// down to 2^-16 count.
+//
+// What bounds it: many tokens, the matrix units and their power. 8192 bfloat16 tokens of 2048 x 50304: five products per half of
+// the vocabulary (844 GFLOP each) of 720 to 850 us, 1.0 to 1.17 PFLOP/s; the forward's over the whole vocabulary takes 1508 us, at
+// 1.97 GHz with the units busy 54 % of the time, a library product of the same operands 1472 us, at 1.56 GHz and 71 %.
+// 2048 tokens of 1024: 232 to 274 us a product (211 GFLOP). 512 float32 tokens of 1024: 184 to 245 us (158 GFLOP in fp16), and 95 us
+// that pack the weight (412 MB). One bfloat16 token of 2048: 49 us for the weight's 206 MB, 4.2 TB/s.
 #include <type_traits>
 
 #include "common.hpp"
@@ -500,7 +509,7 @@ struct Operand {
 
 // float32 entries already split into three bfloat16 parts (memory: per 32 entries 3 x 32), index-major, in LDS as a plane of
 // TILE x 64 bytes a part: x's rows for the weight's products, which every wave of a block reads (splitting them where they are
-// read took four waves' time: one token, 6400 rows of 1024: a call of 61 us).
+// read took four waves' time: losses of 64 tokens of 2048 x 50304 143 us, 123 so).
 template <int TILE, int WAVES>
 struct SplitOperand {
     static constexpr uint32_t kPlane = TILE * 64, kBytes = 3 * kPlane, kPieces = kBytes / 1024, kPerWave = kPieces / WAVES, kDepth = 32;
@@ -984,7 +993,8 @@ __device__ __forceinline__ void take_part(const Product& p, const Meta& meta, ui
 
 // A launch's blocks stay: block b, on XCD b % 8, takes every (blocks / 8)-th tile of the XCD's share and requests a tile's
 // first k-tiles before it finishes the tile before. Tiles that would leave most CUs idle in a last round are cut into halves
-// or quarters, one a block (1 / 2 or 1 / 4 of the whole shape): 788 tiles of 256 blocks take 3.1 rounds, not 4.
+// or quarters, one a block (1 / 2 or 1 / 4 of the whole shape): 788 tiles of 256 blocks take 3.25 rounds, not 4. bfloat16 tiles
+// are of 8 waves of 128 x 64 results (4 of 128 x 128: the forward's product of 8192 tokens of 2048 1540 -> 1780 us).
 constexpr int kXcds = 8;
 template <int PARTS, Use USE, int WA, int WB, int TA, int TB>
 __global__ __launch_bounds__(WA* WB* kWave) __attribute__((amdgpu_waves_per_eu(2, 2))) void loss_product_kernel(Product p) {
