@@ -406,19 +406,21 @@ __device__ __forceinline__ uint32_t permuted(uint32_t r) { return (r >> 2 & 1) *
 // a read touch every bank: index-major (memory rows are the operand's indexes, k contiguous; a row's 8 chunks) or k-major
 // (TR: memory rows are k, read through the LDS transpose reads). Transfers of 1 KB go straight from memory to LDS.
 // Entries in memory: PARTS 1 bfloat16; PARTS 2 fp16 hi and lo; PARTS 3 float32 as they are, split into three bfloat16 parts
-// by the wave that reads them (RAW; k-major tiles of these are read entry by entry).
-template <int PARTS, bool TR, int TILE, int WAVES>
+// by the wave that reads them (RAW; k-major tiles of these are read entry by entry). GRAIN: bytes a lane transfers at a time, 4 for
+// index-major rows that start on 4-byte boundaries.
+template <int PARTS, bool TR, int TILE, int WAVES, uint32_t GRAIN = 16>
 struct Operand {
     static constexpr bool RAW = PARTS == 3;
     static constexpr uint32_t kWords = PARTS == 1 ? 1 : 2;  // 16-bit words of an entry
-    static constexpr uint32_t kBytes = TILE * 128, kPieces = kBytes / 1024, kPerWave = kPieces / WAVES;
+    static constexpr uint32_t kBytes = TILE * 128, kPiece = GRAIN * kWave, kPieces = kBytes / kPiece, kPerWave = kPieces / WAVES;
     static constexpr uint32_t kRow = TR ? TILE * 2 * kWords : 128, kDepth = 64 / kWords;
     static_assert(kPieces % WAVES == 0, "every wave transfers as many pieces");
+    static_assert(GRAIN == 16 || (GRAIN == 4 && !TR && RAW), "16-byte transfers, or single float32");
 
     const char* base;        // of the tile at k = 0 (index-major) or of its first column (k-major)
     uint64_t stride;         // bytes of a memory row
     uint32_t offset[kPerWave];  // index-major: a lane's byte offset of each piece
-    uint32_t back[kPerWave], whole;  // index-major: bytes back to the row's first chunk where k-tile `whole`, the last, has no more
+    uint32_t back[kPerWave], whole;  // index-major: bytes back to the tile's first chunk where k-tile `whole`, the last, has no more
     uint32_t row[kPerWave], last;  // k-major: the lane's k row of each piece (offset: its column); the last k row to read
 
     __device__ __forceinline__ static uint32_t swizzle(uint32_t r) {
@@ -439,15 +441,16 @@ struct Operand {
         else base = reinterpret_cast<const char*>(p) + first * stride;
 #pragma unroll
         for (uint32_t j = 0; j < kPerWave; ++j) {
-            const uint32_t at = (wave * kPerWave + j) * 1024 + lane * 16, r = at / kRow, chunk = at % kRow / 16 ^ swizzle(r);
+            const uint32_t at = (wave * kPerWave + j) * kPiece + lane * GRAIN, r = at / kRow, chunk = at % kRow / 16 ^ swizzle(r);
             if constexpr (TR) {
                 const uint32_t chunks = (indexes - first) * kWords / 8;  // to the end of the memory row
                 row[j] = r;
                 offset[j] = (chunk < chunks ? chunk : chunks - 1) * 16;
             } else {
                 const uint32_t left = indexes - first - 1;  // clamped rows repeat the last
-                offset[j] = (r < left ? r : left) * static_cast<uint32_t>(stride) + chunk * 16;
-                back[j] = chunk * 16 >= depth * kWords * 2 % 128 ? chunk * 16 : 0;
+                const uint32_t byte = chunk * 16 + at % 16;
+                offset[j] = (r < left ? r : left) * static_cast<uint32_t>(stride) + byte;
+                back[j] = byte >= depth * kWords * 2 % 128 ? byte : 0;
             }
         }
     }
@@ -465,7 +468,11 @@ struct Operand {
         } else {
             const char* from = base + kt * 128;
 #pragma unroll
-            for (uint32_t j = 0; j < kPerWave; ++j) dma16(from, kt == whole ? offset[j] - back[j] : offset[j], lds + (wave * kPerWave + j) * 1024);
+            for (uint32_t j = 0; j < kPerWave; ++j) {
+                const uint32_t at = kt == whole ? offset[j] - back[j] : offset[j];
+                if constexpr (GRAIN == 16) dma16(from, at, lds + (wave * kPerWave + j) * kPiece);
+                else dma4(from, at, lds + (wave * kPerWave + j) * kPiece);
+            }
         }
     }
     // a lane's place in the tile for the 32-index blocks from `first` on
@@ -619,13 +626,13 @@ struct Product {
 };
 
 // WA x WB waves of TA x TB 32 x 32 results each; k-tiles go through a ring of kStages tile pairs.
-template <int PARTS_, Use USE_, int WA_, int WB_, int TA_, int TB_>
+template <int PARTS_, Use USE_, int WA_, int WB_, int TA_, int TB_, uint32_t GRAIN = 16>
 struct Shape {
     static constexpr int PARTS = PARTS_, WA = WA_, WB = WB_, TA = TA_, TB = TB_;
     static constexpr Use USE = USE_;
     static constexpr bool kATr = USE == Use::GradX || USE == Use::GradW, kBTr = USE == Use::GradW;
     static constexpr int kA = WA * TA * 32, kB = WB * TB * 32, kWaves = WA * WB;
-    using OpA = Operand<PARTS, kATr, kA, kWaves>;
+    using OpA = Operand<PARTS, kATr, kA, kWaves, GRAIN>;
     // float32 as it is: x's rows come split, D's do not
     static constexpr bool kBSplit = PARTS == 3 && USE != Use::GradX && USE != Use::GradW;
     using OpB = typename std::conditional<kBSplit, SplitOperand<kB, kWaves>, Operand<PARTS, kBTr, kB, kWaves>>::type;
@@ -996,12 +1003,12 @@ __device__ __forceinline__ void take_part(const Product& p, const Meta& meta, ui
 // or quarters, one a block (1 / 2 or 1 / 4 of the whole shape): 788 tiles of 256 blocks take 3.25 rounds, not 4. bfloat16 tiles
 // are of 8 waves of 128 x 64 results (4 of 128 x 128: the forward's product of 8192 tokens of 2048 1540 -> 1780 us).
 constexpr int kXcds = 8;
-template <int PARTS, Use USE, int WA, int WB, int TA, int TB>
+template <int PARTS, Use USE, int WA, int WB, int TA, int TB, uint32_t GRAIN>
 __global__ __launch_bounds__(WA* WB* kWave) __attribute__((amdgpu_waves_per_eu(2, 2))) void loss_product_kernel(Product p) {
     constexpr bool kCut = TA % 2 == 0 && TB % 2 == 0;
-    using Whole = Shape<PARTS, USE, WA, WB, TA, TB>;
-    using Half = Shape<PARTS, USE, WA, WB, TA, kCut ? TB / 2 : TB>;
-    using Quarter = Shape<PARTS, USE, WA, WB, kCut ? TA / 2 : TA, kCut ? TB / 2 : TB>;
+    using Whole = Shape<PARTS, USE, WA, WB, TA, TB, GRAIN>;
+    using Half = Shape<PARTS, USE, WA, WB, TA, kCut ? TB / 2 : TB, GRAIN>;
+    using Quarter = Shape<PARTS, USE, WA, WB, kCut ? TA / 2 : TA, kCut ? TB / 2 : TB, GRAIN>;
     constexpr uint32_t kSlices = kCut ? 2 * WA : WA;
     constexpr uint32_t kLds = Whole::kLds > Quarter::kLds ? (Whole::kLds > Half::kLds ? Whole::kLds : Half::kLds)
                                                           : (Quarter::kLds > Half::kLds ? Quarter::kLds : Half::kLds);
@@ -1211,29 +1218,31 @@ uint32_t padded(uint32_t v, uint32_t to) { return ceil_div(v, to) * to; }
 
 // How a call runs. parts: 1 bfloat16, 2 float32 as fp16 hi + lo, 3 float32 as three bfloat16 parts split where they are
 // multiplied. A few tokens wait for the weight, not for the matrix unit, and packing it reads and writes it once more: float32
-// calls then read it as it is (it has to be made of whole 16-byte pieces). Losses, width 1024, as it is against packed: 1
+// calls then read it as it is (steps: where its rows are made of whole 16-byte pieces; losses: in 4-byte transfers else, one token
+// of 1001 x 50304 in 69 us, packed 164). Losses, width 1024, as it is against packed: 1
 // token of 50304 rows 67 against 161 us, 128 tokens 110 / 159, 192 156 / 195, 256 202 / 202; of 32768 rows 128 tokens 107 /
 // 115, 192 151 / 126; of 16384 rows 64 tokens 58 / 62, 128 102 / 64; of 10000 rows 64 tokens 57 / 48. Steps gain less (their
 // products with D split what they read): 64 tokens of 50304 rows 229 / 324 us, 128 362 / 350.
 struct Plan {
     uint32_t parts, words, n_pad, width, vocab_tile, token_tile, height, per_tile, slices, piece, pieces, last, stats_tiles, keep_tiles, splits;
-    bool few, in_place, keeps;
+    bool whole, few, in_place, keeps;  // whole: the weight's rows are made of whole 16-byte pieces
     uint64_t meta, rows, labels, place, lse, picked, losses, slice_sums, x_most, w_most, x, x_split, weight, grad, partial, bytes;
 };
 
-// `aligned`: the weight starts on a 16-byte boundary (weights of whole 16-byte pieces are then read in place, but for parts 2).
+// `aligned`: the weight starts on a 16-byte boundary.
 Plan plan_of(int vt, uint32_t n, uint32_t d, uint32_t vocab, bool aligned, bool gradients, uint64_t piece_bytes) {
     Plan p{};
     p.words = vt == kBF16 ? 1 : 2;
-    const bool whole = d % (8 / p.words) == 0 && aligned;
+    p.whole = d % (8 / p.words) == 0 && aligned;
     if (vt == kBF16) p.few = n <= kFewTokens;
-    else p.few = whole && (gradients ? n <= kFewTokens && vocab >= kFewRows : n <= 3 * kFewTokens && vocab >= ceil_div(n, kFewTokens) * kFewRows);
+    else if (gradients) p.few = p.whole && n <= kFewTokens && vocab >= kFewRows;
+    else p.few = n <= 3 * kFewTokens && vocab >= ceil_div(n, kFewTokens) * kFewRows;
     p.parts = vt == kBF16 ? 1 : p.few ? 3 : 2;
     p.vocab_tile = p.few ? kFewTile : kTile;
     p.token_tile = p.few ? kFewTokens : p.parts == 1 ? 256 : 128;
     p.n_pad = padded(n, p.few ? kFewTokens : 256);
     p.width = padded(d, 64 / p.words);
-    p.in_place = p.parts != 2 && whole;
+    p.in_place = p.parts == 3 || (p.parts == 1 && p.whole);
     p.per_tile = p.parts == 2 ? 8 : 4;  // slices: as many as waves of quarter tiles (few: of tiles) along the vocabulary
     p.pieces = 1;
     p.piece = padded(vocab, kTile);
@@ -1290,15 +1299,17 @@ Plan plan_of(int vt, uint32_t n, uint32_t d, uint32_t vocab, bool aligned, bool 
     return p;
 }
 
-template <int PARTS, Use USE, int WA, int WB, int TA, int TB>
+template <int PARTS, Use USE, int WA, int WB, int TA, int TB, uint32_t GRAIN = 16>
 hipError_t launch_product(const Product& p, hipStream_t stream) {
     constexpr uint32_t kBlocks = WA * WB == 4 ? 2 * kCus : kCus;  // as many as the CUs hold
-    hipLaunchKernelGGL((loss_product_kernel<PARTS, USE, WA, WB, TA, TB>), dim3(kBlocks), dim3(WA * WB * kWave), 0, stream, p);
+    hipLaunchKernelGGL((loss_product_kernel<PARTS, USE, WA, WB, TA, TB, GRAIN>), dim3(kBlocks), dim3(WA * WB * kWave), 0, stream, p);
     return hipGetLastError();
 }
 
 template <Use USE>
 hipError_t product(const Plan& plan, const Product& p, hipStream_t stream) {
+    if constexpr (USE == Use::Stats)
+        if (plan.parts == 3 && !plan.whole) return launch_product<3, USE, 4, 1, 1, 2, 4>(p, stream);
     if (plan.parts == 3) return launch_product<3, USE, 4, 1, 1, 2>(p, stream);
     if constexpr (USE != Use::GradW && USE != Use::Keep)
         if (plan.few) return launch_product<1, USE, 4, 1, 1, 2>(p, stream);

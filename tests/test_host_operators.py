@@ -74,7 +74,7 @@ def test_loss_workspace_sizes():
     # a float32 weight is read as it is for a few tokens of a large vocabulary, packed otherwise
     weight = 4 * 50304 * 1024
     assert loss_bytes(F32, 8, 1024, 50304, gradients=0) < weight < loss_bytes(F32, 512, 1024, 50304, gradients=0)
-    assert loss_bytes(F32, 8, 1024, 50304, aligned=0, gradients=0) > weight
+    assert loss_bytes(F32, 8, 1024, 50304, aligned=0) > weight > loss_bytes(F32, 8, 1024, 50304, aligned=0, gradients=0)
     # the largest call the entries take is a finite number of bytes
     assert 0 < loss_bytes(F32, 1 << 18, 32768, 1 << 24) < 1 << 50
 
