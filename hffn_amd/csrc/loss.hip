@@ -1312,6 +1312,9 @@ hipError_t product(const Plan& plan, const Product& p, hipStream_t stream) {
     if constexpr (USE == Use::Stats)
         if (plan.parts == 3 && !plan.whole) return launch_product<3, USE, 4, 1, 1, 2, 4>(p, stream);
     if (plan.parts == 3) return launch_product<3, USE, 4, 1, 1, 2>(p, stream);
+    // gw of a few bfloat16 tokens, one k-tile a tile: 128 x 128, two blocks a CU (1 token of 1024 x 50304: a step of 113 us, 107 so)
+    if constexpr (USE == Use::GradW)
+        if (plan.few) return launch_product<1, USE, 4, 1, 1, 4>(p, stream);
     if constexpr (USE != Use::GradW && USE != Use::Keep)
         if (plan.few) return launch_product<1, USE, 4, 1, 1, 2>(p, stream);
     return plan.parts == 1 ? launch_product<1, USE, 2, 4, 4, 2>(p, stream) : launch_product<2, USE, 4, 2, 2, 2>(p, stream);
@@ -1403,7 +1406,7 @@ hipError_t run(const LossCall& c, hipStream_t stream) {
     if (failed(status)) return status;
     if (!gradients) return hipSuccess;
 
-    const uint32_t gw_tile = plan.parts == 3 ? kFewTile : kTile, gw_rows = plan.parts == 1 ? 256 : plan.parts == 2 ? 128 : 64;
+    const uint32_t gw_tile = plan.few ? kFewTile : kTile, gw_rows = plan.parts == 3 ? 64 : plan.few || plan.parts == 2 ? 128 : 256;
     for (uint32_t piece = plan.pieces; piece-- > 0;) {
         const uint32_t first = piece * plan.piece, count = c.vocab - first < plan.piece ? c.vocab - first : plan.piece;
         Product grad = keep;
