@@ -407,7 +407,7 @@ __device__ __forceinline__ uint32_t permuted(uint32_t r) { return (r >> 2 & 1) *
 // (TR: memory rows are k, read through the LDS transpose reads). Transfers of 1 KB go straight from memory to LDS.
 // Entries in memory: PARTS 1 bfloat16; PARTS 2 fp16 hi and lo; PARTS 3 float32 as they are, split into three bfloat16 parts
 // by the wave that reads them (RAW; k-major tiles of these are read entry by entry). GRAIN: bytes a lane transfers at a time, 4 for
-// index-major rows that start on 4-byte boundaries.
+// rows of float32 that start on their own boundaries only.
 template <int PARTS, bool TR, int TILE, int WAVES, uint32_t GRAIN = 16>
 struct Operand {
     static constexpr bool RAW = PARTS == 3;
@@ -415,7 +415,7 @@ struct Operand {
     static constexpr uint32_t kBytes = TILE * 128, kPiece = GRAIN * kWave, kPieces = kBytes / kPiece, kPerWave = kPieces / WAVES;
     static constexpr uint32_t kRow = TR ? TILE * 2 * kWords : 128, kDepth = 64 / kWords;
     static_assert(kPieces % WAVES == 0, "every wave transfers as many pieces");
-    static_assert(GRAIN == 16 || (GRAIN == 4 && !TR && RAW), "16-byte transfers, or single float32");
+    static_assert(GRAIN == 16 || (GRAIN == 4 && RAW), "16-byte transfers, or single float32");
 
     const char* base;        // of the tile at k = 0 (index-major) or of its first column (k-major)
     uint64_t stride;         // bytes of a memory row
@@ -443,9 +443,9 @@ struct Operand {
         for (uint32_t j = 0; j < kPerWave; ++j) {
             const uint32_t at = (wave * kPerWave + j) * kPiece + lane * GRAIN, r = at / kRow, chunk = at % kRow / 16 ^ swizzle(r);
             if constexpr (TR) {
-                const uint32_t chunks = (indexes - first) * kWords / 8;  // to the end of the memory row
+                const uint32_t byte = chunk * 16 + at % 16, end = (indexes - first) * kWords * 2;  // of the memory row
                 row[j] = r;
-                offset[j] = (chunk < chunks ? chunk : chunks - 1) * 16;
+                offset[j] = byte < end ? byte : end - GRAIN;
             } else {
                 const uint32_t left = indexes - first - 1;  // clamped rows repeat the last
                 const uint32_t byte = chunk * 16 + at % 16;
@@ -453,6 +453,10 @@ struct Operand {
                 back[j] = byte >= depth * kWords * 2 % 128 ? byte : 0;
             }
         }
+    }
+    __device__ __forceinline__ static void transfer(const char* from, uint32_t at, const char* lds) {
+        if constexpr (GRAIN == 16) dma16(from, at, lds);
+        else dma4(from, at, lds);
     }
     // the tile of k-tile kt into LDS
     __device__ __forceinline__ void fetch(uint32_t kt, const char* lds) const {
@@ -463,16 +467,12 @@ struct Operand {
 #pragma unroll
             for (uint32_t j = 0; j < kPerWave; ++j) {
                 const uint32_t r = k0 + row[j] <= last ? row[j] : last - k0;  // beyond: the other operand holds zeros
-                dma16(from, r * static_cast<uint32_t>(stride) + offset[j], lds + (wave * kPerWave + j) * 1024);
+                transfer(from, r * static_cast<uint32_t>(stride) + offset[j], lds + (wave * kPerWave + j) * kPiece);
             }
         } else {
             const char* from = base + kt * 128;
 #pragma unroll
-            for (uint32_t j = 0; j < kPerWave; ++j) {
-                const uint32_t at = kt == whole ? offset[j] - back[j] : offset[j];
-                if constexpr (GRAIN == 16) dma16(from, at, lds + (wave * kPerWave + j) * kPiece);
-                else dma4(from, at, lds + (wave * kPerWave + j) * kPiece);
-            }
+            for (uint32_t j = 0; j < kPerWave; ++j) transfer(from, kt == whole ? offset[j] - back[j] : offset[j], lds + (wave * kPerWave + j) * kPiece);
         }
     }
     // a lane's place in the tile for the 32-index blocks from `first` on
@@ -1219,7 +1219,7 @@ uint32_t padded(uint32_t v, uint32_t to) { return ceil_div(v, to) * to; }
 
 // How a call runs. parts: 1 bfloat16, 2 float32 as fp16 hi + lo, 3 float32 as three bfloat16 parts split where they are
 // multiplied. A few tokens wait for the weight, not for the matrix unit, and packing it reads and writes it once more: float32
-// calls then read it as it is (steps: where its rows are made of whole 16-byte pieces; losses: in 4-byte transfers else, one token
+// calls then read it as it is (in 4-byte transfers where its rows are not made of whole 16-byte pieces: losses of one token
 // of 1001 x 50304 in 69 us, packed 164). Losses, width 1024, as it is against packed: 1
 // token of 50304 rows 67 against 161 us, 128 tokens 110 / 159, 192 156 / 195, 256 202 / 202; of 32768 rows 128 tokens 107 /
 // 115, 192 151 / 126; of 16384 rows 64 tokens 58 / 62, 128 102 / 64; of 10000 rows 64 tokens 57 / 48. Steps gain less (their
@@ -1236,8 +1236,7 @@ Plan plan_of(int vt, uint32_t n, uint32_t d, uint32_t vocab, bool aligned, bool 
     p.words = vt == kBF16 ? 1 : 2;
     p.whole = d % (8 / p.words) == 0 && aligned;
     if (vt == kBF16) p.few = n <= kFewTokens;
-    else if (gradients) p.few = p.whole && n <= kFewTokens && vocab >= kFewRows;
-    else p.few = n <= 3 * kFewTokens && vocab >= ceil_div(n, kFewTokens) * kFewRows;
+    else p.few = n <= (gradients ? 1 : 3) * kFewTokens && vocab >= ceil_div(n, kFewTokens) * kFewRows;
     p.parts = vt == kBF16 ? 1 : p.few ? 3 : 2;
     p.vocab_tile = p.few ? kFewTile : kTile;
     p.token_tile = p.few ? kFewTokens : p.parts == 1 ? 256 : 128;
@@ -1309,7 +1308,7 @@ hipError_t launch_product(const Product& p, hipStream_t stream) {
 
 template <Use USE>
 hipError_t product(const Plan& plan, const Product& p, hipStream_t stream) {
-    if constexpr (USE == Use::Stats)
+    if constexpr (USE != Use::GradW)  // which does not read the weight
         if (plan.parts == 3 && !plan.whole) return launch_product<3, USE, 4, 1, 1, 2, 4>(p, stream);
     if (plan.parts == 3) return launch_product<3, USE, 4, 1, 1, 2>(p, stream);
     // gw of a few bfloat16 tokens, one k-tile a tile: 128 x 128, two blocks a CU (1 token of 1024 x 50304: a step of 113 us, 107 so)

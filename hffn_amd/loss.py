@@ -41,7 +41,8 @@ def rows_of(t: torch.Tensor, name: str, width: int, dtype: torch.dtype) -> tuple
 class HeadLoss:
     """The loss of one head (see the module docstring). Buffers are the object's own and grow with the calls; what a
     call returns are views of them that the next call overwrites. Calls are queued on PyTorch's current stream; calls of one
-    object on several streams have to be ordered by the caller."""
+    object on several streams have to be ordered by the caller. A captured graph holds the buffers of its capture: ``reserve``
+    the sizes that later calls will have before it, so that none of these replaces them."""
 
     def __init__(self, weight: torch.Tensor, max_tokens: int = 1, ignore_index: int = -100, reduction: str = "mean",
                  piece_bytes: int = PIECE_BYTES) -> None:

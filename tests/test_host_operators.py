@@ -54,8 +54,9 @@ def test_loss_entries_refuse_bad_arguments():
         refused(step(**{name: None}), "null")
     need = loss_bytes(F32, 5, 64, 100)
     refused(step(bytes=need - 1), f"{need} needed")
-    odd = loss_bytes(F32, 5, 64, 100, aligned=0)  # a weight that is not 16-byte aligned is never read in place
-    refused(step(bytes=odd - 1, w=ctypes.c_void_p(4100)), f"{odd} needed")
+    odd = loss_bytes(BF16, 5, 64, 100, aligned=0)  # a bfloat16 weight that is not 16-byte aligned is packed
+    assert odd > loss_bytes(BF16, 5, 64, 100)
+    refused(step(vt=BF16, bytes=odd - 1, w=ctypes.c_void_p(4098)), f"{odd} needed")
 
 
 def test_loss_workspace_sizes():
@@ -74,7 +75,8 @@ def test_loss_workspace_sizes():
     # a float32 weight is read as it is for a few tokens of a large vocabulary, packed otherwise
     weight = 4 * 50304 * 1024
     assert loss_bytes(F32, 8, 1024, 50304, gradients=0) < weight < loss_bytes(F32, 512, 1024, 50304, gradients=0)
-    assert loss_bytes(F32, 8, 1024, 50304, aligned=0) > weight > loss_bytes(F32, 8, 1024, 50304, aligned=0, gradients=0)
+    assert loss_bytes(F32, 8, 1024, 50304, aligned=0, gradients=0) < weight
+    assert loss_bytes(BF16, 8, 1024, 50304, gradients=0) < weight // 2 < loss_bytes(BF16, 8, 1024, 50304, aligned=0, gradients=0)
     # the largest call the entries take is a finite number of bytes
     assert 0 < loss_bytes(F32, 1 << 18, 32768, 1 << 24) < 1 << 50
 
