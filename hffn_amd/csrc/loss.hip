@@ -594,6 +594,13 @@ __device__ __forceinline__ float exponential(float v) {
     else return __expf(v);
 }
 
+// Where a slice's maximum and sum of token t lie: a few tokens' slices token by token, which one block a token reads in whole
+// lines (losses of 1 token 2.4 us of 31 or 57 less), many tokens' slice by slice.
+template <bool FEW>
+__device__ __forceinline__ uint64_t slice_at(uint32_t slice, uint32_t t, uint32_t pitch) {
+    return FEW ? static_cast<uint64_t>(t) * pitch + slice : static_cast<uint64_t>(slice) * pitch + t;
+}
+
 // Stats: slices' maxima and sums; Keep: those, and the exponentials kept where D belongs; Grad: D.
 enum class Use { Stats, Keep, Grad, GradX, GradW };
 
@@ -613,7 +620,7 @@ struct Product {
     const float* lse;             // Grad, compact
     float* picked;                // Stats, Keep: the label's logit, compact
     float2* slices;               // Stats, Keep: a slice's maximum and sum of exponentials per token
-    uint32_t slice_step, token_step;  // float2 from one slice, one token to the next
+    uint32_t slice_pitch;         // slices of many tokens [slice][n_pad]; of a few [n_pad][slice]: n_pad, or the slices there are
     uint32_t slice_first;         // the piece's first
     uint16_t* grad;               // Grad: D, [n_pad][piece]; Keep: the exponentials
     uint64_t grad_stride;
@@ -899,7 +906,7 @@ __device__ __forceinline__ void finish(const Product& p, const Meta& meta, const
             sum += __shfl_xor(sum, 32);
             if (t >= meta.valid || half != 0) continue;
 #pragma unroll
-            for (uint32_t k = 0; k < kFill; ++k) p.slices[static_cast<uint64_t>(slice + k) * p.slice_step + static_cast<uint64_t>(t) * p.token_step] = make_float2(most, k == 0 ? sum : 0.0f);
+            for (uint32_t k = 0; k < kFill; ++k) p.slices[slice_at<S::kWaves == 4>(slice + k, t, p.slice_pitch)] = make_float2(most, k == 0 ? sum : 0.0f);
         }
     } else if constexpr (USE == Use::Grad) {
 #pragma unroll
@@ -1063,7 +1070,7 @@ __device__ __forceinline__ float2 joined_lanes(float2 v) {  // over the lanes of
     return v;
 }
 template <uint32_t TOKENS>
-__global__ __launch_bounds__(kLseThreads) void loss_lse_kernel(const float2* __restrict__ slices, uint32_t count, uint32_t slice_step, uint32_t token_step,
+__global__ __launch_bounds__(kLseThreads) void loss_lse_kernel(const float2* __restrict__ slices, uint32_t count, uint32_t pitch,
                                                               const float* __restrict__ picked, const int32_t* __restrict__ rows,
                                                               const int32_t* __restrict__ labels, const Meta* __restrict__ meta,
                                                               float* __restrict__ lse, float* __restrict__ losses) {
@@ -1074,7 +1081,7 @@ __global__ __launch_bounds__(kLseThreads) void loss_lse_kernel(const float2* __r
     float2 all = make_float2(-__builtin_huge_valf(), 0.0f);
     if (t < valid)
 #pragma unroll 4
-        for (uint32_t s = threadIdx.x / TOKENS; s < count; s += kLanes) all = joined(all, slices[static_cast<uint64_t>(s) * slice_step + static_cast<uint64_t>(t) * token_step]);
+        for (uint32_t s = threadIdx.x / TOKENS; s < count; s += kLanes) all = joined(all, slices[slice_at<TOKENS == 1>(s, t, pitch)]);
     all = joined_lanes<TOKENS>(all);
     if (lane < TOKENS) lds[threadIdx.x / kWave * TOKENS + in] = all;
     __syncthreads();
@@ -1099,7 +1106,7 @@ constexpr uint32_t kTurnThreads = 256;
 template <int PARTS>
 __global__ __launch_bounds__(kTurnThreads) void loss_turn_kernel(uint16_t* __restrict__ grad, uint64_t stride, uint32_t first, uint32_t count,
                                                                 uint32_t across, const float2* __restrict__ slices, uint32_t height,
-                                                                uint32_t per_tile, uint32_t slice_rows, uint32_t slice_step, uint32_t token_step,
+                                                                uint32_t per_tile, uint32_t slice_rows, uint32_t pitch,
                                                                 const float* __restrict__ lse, const int32_t* __restrict__ labels,
                                                                 const Meta* __restrict__ meta) {
     const uint32_t t = blockIdx.x / across, valid = meta->valid, c = (blockIdx.x % across * kTurnThreads + threadIdx.x) * 8;
@@ -1111,7 +1118,7 @@ __global__ __launch_bounds__(kTurnThreads) void loss_turn_kernel(uint16_t* __res
         if constexpr (PARTS != 1) *low = make_uint4(0, 0, 0, 0);
         return;
     }
-    const float most = slices[static_cast<uint64_t>(c / height * per_tile + c % height / slice_rows) * slice_step + static_cast<uint64_t>(t) * token_step].x;
+    const float most = slices[slice_at<PARTS == 3>(c / height * per_tile + c % height / slice_rows, t, pitch)].x;
     const float factor = exponential<2>(most - lse[t]) * (PARTS == 2 ? 1.0f / (1 << kGradLift) : 1.0f);
     const uint32_t label = static_cast<uint32_t>(labels[t]) - first - c;
     const uint4 kept = *at, rest = PARTS != 1 ? *low : make_uint4(0, 0, 0, 0);
@@ -1380,9 +1387,7 @@ hipError_t run(const LossCall& c, hipStream_t stream) {
     stats.a_columns_out = plan.last;
     stats.picked = picked;
     stats.slices = reinterpret_cast<float2*>(work + plan.slice_sums);
-    // many tokens: [slice][n_pad]; a few: [n_pad][slice], which one block a token reads in whole lines (1 token: 2.4 us of 31 or 57 less)
-    stats.slice_step = plan.few ? 1 : plan.n_pad;
-    stats.token_step = plan.few ? plan.slices : 1;
+    stats.slice_pitch = plan.few ? plan.slices : plan.n_pad;
     Product keep = stats;
     keep.a_first = plan.last;
     keep.a_tiles = plan.keep_tiles;
@@ -1394,7 +1399,7 @@ hipError_t run(const LossCall& c, hipStream_t stream) {
     if (plan.keeps && (status = product<Use::Keep>(plan, keep, stream)) != hipSuccess) return status;
     const auto lse_of = [&](auto tokens) {
         constexpr uint32_t kTokens = decltype(tokens)::value;
-        hipLaunchKernelGGL(loss_lse_kernel<kTokens>, dim3(ceil_div(c.n, kTokens)), dim3(kLseThreads), 0, stream, stats.slices, plan.slices, stats.slice_step, stats.token_step,
+        hipLaunchKernelGGL(loss_lse_kernel<kTokens>, dim3(ceil_div(c.n, kTokens)), dim3(kLseThreads), 0, stream, stats.slices, plan.slices, stats.slice_pitch,
                            picked, rows, labels, meta, lse, losses);
     };
     // tokens a block: one where few are all there are, more where that still fills the CUs (runs of 128 bytes of a slice; 8192
@@ -1411,11 +1416,11 @@ hipError_t run(const LossCall& c, hipStream_t stream) {
         Product grad = keep;
         if (first == plan.last) {
             const uint32_t columns = padded(count, kTile), across = ceil_div(columns, 8 * kTurnThreads), slice_rows = plan.vocab_tile / plan.per_tile;
-            const float2* slices = stats.slices + static_cast<uint64_t>(keep.slice_first) * stats.slice_step;
+            const float2* slices = stats.slices + static_cast<uint64_t>(keep.slice_first) * (plan.few ? 1 : stats.slice_pitch);
             const auto turn = [&](auto parts) {
                 constexpr int kParts = decltype(parts)::value;
                 hipLaunchKernelGGL(loss_turn_kernel<kParts>, dim3(across * padded(c.n, 64)), dim3(kTurnThreads), 0, stream, grad.grad, grad.grad_stride,
-                                   first, columns, across, slices, plan.height, plan.per_tile, slice_rows, stats.slice_step, stats.token_step, lse, labels, meta);
+                                   first, columns, across, slices, plan.height, plan.per_tile, slice_rows, stats.slice_pitch, lse, labels, meta);
             };
             if (plan.parts == 1) turn(std::integral_constant<int, 1>{});
             else if (plan.parts == 2) turn(std::integral_constant<int, 2>{});
