@@ -2,8 +2,8 @@
 // The first leaves one float64 partial per block; every block of the second adds the partials up again (8 KB a table out
 // of L2), so that no block waits for another, and scales its share.
 //
-// Bound by memory: 152 million entries in 98 tensors (506 MB; two tables) take 93 us for the norm, 5.4 TB/s, and 217 us scaled into 609 MB
-// of others, 5.1 TB/s, a copy's rate. 24 tensors of 5 MB: 5.2 and 3.3 us, less than the host's part of the calls (22 us).
+// Bound by memory: 152 million entries in 145 tensors (506 MB; two tables) take 93 us for the norm, 5.4 TB/s, and 217 us scaled into 609 MB
+// of others, 5.1 TB/s, a copy's rate. 36 tensors of 10 MB: 5.2 and 3.3 us, less than the host's part of the calls (22 us).
 #include <vector>
 
 #include "common.hpp"
