@@ -57,15 +57,16 @@ def _at(values: array) -> int:
 
 
 @functools.lru_cache(maxsize=None)
-def _workspace_floats(count: int) -> int:
-    return _lib.query_bytes(_lib.load().hffn_clip_workspace, count) // 4
+def _workspace_bytes(count: int) -> int:
+    return _lib.query_bytes(_lib.load().hffn_clip_workspace, count)
 
 
 def _buffers(count: int, norm_type: float) -> tuple:
     if norm_type not in NORM_TYPES:
         raise ValueError(f"norm_type is 2 or inf, not {norm_type!r}")
     device = _device(None) if count == 0 else _CUDA  # the tensors lie there
-    return torch.empty(_workspace_floats(count), device=device), torch.empty((), device=device), current_stream(device)
+    work = torch.empty(_workspace_bytes(count), dtype=torch.uint8, device=device)
+    return work, torch.empty((), dtype=torch.float32, device=device), current_stream(device)
 
 
 def grad_norm(tensors: Iterable[torch.Tensor], norm_type: float = 2.0) -> torch.Tensor:
@@ -74,7 +75,7 @@ def grad_norm(tensors: Iterable[torch.Tensor], norm_type: float = 2.0) -> torch.
     tensors, pointers, counts, types, _ = _table(tensors, "tensors")
     work, norm, stream = _buffers(len(tensors), norm_type)
     _lib.check(_lib.load().hffn_grad_norm(len(tensors), _at(pointers), _at(counts), _at(types), int(norm_type == math.inf), work.data_ptr(),
-                                          4 * work.numel(), norm.data_ptr(), stream), "gradient norm")
+                                          work.numel(), norm.data_ptr(), stream), "gradient norm")
     return norm
 
 
@@ -97,5 +98,5 @@ def clip_grad_norm_(tensors: Iterable[torch.Tensor], max_norm: float, norm_type:
         to = (_at(to_pointers), _at(to_types))
     work, norm, stream = _buffers(len(tensors), norm_type)
     _lib.check(_lib.load().hffn_clip(len(tensors), _at(pointers), to[0], _at(counts), _at(types), to[1], int(norm_type == math.inf), max_norm,
-                                     work.data_ptr(), 4 * work.numel(), norm.data_ptr(), stream), "clip")
+                                     work.data_ptr(), work.numel(), norm.data_ptr(), stream), "clip")
     return norm

@@ -87,12 +87,12 @@ class HeadLoss:
         if self._workspace is None or self._workspace.numel() < need:
             self._workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
         if self._losses is None or self._losses.numel() < n:
-            self._losses = torch.empty(n, device=self.device)
+            self._losses = torch.empty(n, dtype=torch.float32, device=self.device)
         if gradients and (self._gx is None or self._gx.shape[0] < n):
             self._gx = torch.empty(n, self.d_model, dtype=self.weight.dtype, device=self.device)
         if gradients and self.grad is None:
             self.grad = torch.empty_like(self.weight)
-            self._loss = torch.empty((), device=self.device)
+            self._loss = torch.empty((), dtype=torch.float32, device=self.device)
         self._sized[gradients] = n
 
     def workspace_bytes(self) -> int:

@@ -124,11 +124,10 @@ class ResidualNorm:
             for t in g.values():
                 t.zero_()
             return gx, gf
-        bytes_ = _backward_workspace(n, d)
-        work = torch.empty(bytes_ // 4, device=self.device)
+        work = torch.empty(_backward_workspace(n, d), dtype=torch.uint8, device=self.device)
         _lib.check(self._lib.hffn_residual_norm_backward(
             value_type, r.data_ptr(), r_stride, _pointer(f), f_stride, _pointer(gr), gr_stride, gh.data_ptr(), gh_stride,
             p["weight"].data_ptr(), *(_pointer(p.get(name)) for name in PARAMETERS[2:]), self.scale, self.eps, int(self.kind == "layer"),
-            gx.data_ptr(), _pointer(gf), *(_pointer(g.get(name)) for name in PARAMETERS), work.data_ptr(), bytes_, d, n,
+            gx.data_ptr(), _pointer(gf), *(_pointer(g.get(name)) for name in PARAMETERS), work.data_ptr(), work.numel(), d, n,
             current_stream(self.device)), "residual norm backward")
         return gx, gf

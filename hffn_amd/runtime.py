@@ -354,17 +354,17 @@ class HFFNRuntime:
         self._stale: set[int] = set()   # layers whose values changed since their planes were built
         self._tiles_stale: set[int] = set()  # ... since their tiled stores were built
         self._tiles: list[dict] | None = None
-        self._tiles_work = torch.empty(1, device=self.device)
+        self._tiles_work = torch.empty(1, dtype=torch.float32, device=self.device)
         if self._tiles_eligible():
             self._tiles = [self._tiles_build(tensors) for tensors in self._tensors]
             words = max(_lib.query_bytes(self._lib.hffn_tiles_workspace, args[0], TILES_MAX_TOKENS, self.d_model, self.d_ff,
                                          *nnz) for args, nnz in zip(self._args, self._nnz)) // 4
-            self._tiles_work = torch.empty(words, device=self.device)  # the per-chunk partial sums
-        self._gemv_work = torch.empty(1, device=self.device)
+            self._tiles_work = torch.empty(words, dtype=torch.float32, device=self.device)  # the per-chunk partial sums
+        self._gemv_work = torch.empty(1, dtype=torch.float32, device=self.device)
         if (dense or (dense is None and self.density >= MFMA_MIN_DENSITY)) and self._mfma_eligible():
             self._planes = [self._densify(tensors) for tensors in self._tensors]
             words = (_lib.query_bytes(self._lib.hffn_gemv_workspace, self.d_model, self.d_ff) + 3) // 4
-            self._gemv_work = torch.empty(words, device=self.device)  # the decode GEMVs' k-split partial sums
+            self._gemv_work = torch.empty(words, dtype=torch.float32, device=self.device)  # the decode GEMVs' k-split partial sums
         self._policy: dict[int, tuple[str, str]] = {}  # N -> the policy's (up, down)
         self._transient_allowed = dense is not False and self._tiles is not None
         longest = [torch.stack([tensors[name].diff().max() for tensors in self._tensors]).max() for name in ("up_offsets", "out_offsets")]
@@ -498,10 +498,10 @@ class HFFNRuntime:
     def _reserve(self, n: int) -> None:
         self._tokens = n
         ld = leading_dim(n)
-        self._x_t = torch.empty(self.d_model * ld, device=self.device)   # [d_model, ld]
-        self._act = torch.empty(self.d_ff * ld, device=self.device)      # [d_ff, ld]
-        self._y_t = torch.empty(self.d_model * ld, device=self.device)   # [d_model, ld]
-        self._y = torch.empty(n, self.d_model, device=self.device)
+        self._x_t = torch.empty(self.d_model * ld, dtype=torch.float32, device=self.device)   # [d_model, ld]
+        self._act = torch.empty(self.d_ff * ld, dtype=torch.float32, device=self.device)      # [d_ff, ld]
+        self._y_t = torch.empty(self.d_model * ld, dtype=torch.float32, device=self.device)   # [d_model, ld]
+        self._y = torch.empty(n, self.d_model, dtype=torch.float32, device=self.device)
         words = 1
         if self._planes is not None:
             words = (_lib.query_bytes(self._lib.hffn_mfma_workspace, n, self.d_model, self.d_ff) + 3) // 4

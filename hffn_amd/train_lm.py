@@ -43,9 +43,9 @@ class LMTrainer:
         device, d = self.train.runtime.device, self.train.d_model
         self.device, self.max_norm, self.steps = device, float(max_norm), 0
         g = torch.Generator(device).manual_seed(seed)
-        self.embedding = torch.randn(vocab, d, generator=g, device=device)
-        self.head = HeadLoss(torch.randn(vocab, d, generator=g, device=device) / math.sqrt(d), max_tokens, IGNORE)
-        vector = lambda value: torch.full((d,), value, device=device)  # noqa: E731
+        self.embedding = torch.randn(vocab, d, generator=g, dtype=torch.float32, device=device)
+        self.head = HeadLoss(torch.randn(vocab, d, generator=g, dtype=torch.float32, device=device) / math.sqrt(d), max_tokens, IGNORE)
+        vector = lambda value: torch.full((d,), value, dtype=torch.float32, device=device)  # noqa: E731
         self.boundaries = [ResidualNorm(vector(1.0), vector(0.0), gate=vector(1.0 / math.sqrt(len(layers))) if i else None)
                            for i in range(len(layers) + 1)]
         self._embedding_grad = torch.zeros_like(self.embedding)
@@ -86,7 +86,7 @@ class LMTrainer:
             raise ValueError("no tokens")
         entries = self.train.d_ff * leading_dim(n)
         if self._z is None or self._z.numel() < entries:
-            self._z = torch.empty(entries, device=self.device)
+            self._z = torch.empty(entries, dtype=torch.float32, device=self.device)
         rs, hs = self.forward(ids)
         loss, gh, _ = self.head.step(hs[-1], labels)
         gr = None

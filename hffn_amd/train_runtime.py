@@ -149,9 +149,9 @@ class HFFNTrainRuntime:
         if n > self._tokens:
             ld = leading_dim(n)
             device = runtime.device
-            self._z, self._gz = (torch.empty(self.d_ff * ld, device=device) for _ in range(2))
-            self._gy_t, self._gx_t = (torch.empty(self.d_model * ld, device=device) for _ in range(2))
-            self._gx = torch.empty(n, self.d_model, device=device)
+            self._z, self._gz = (torch.empty(self.d_ff * ld, dtype=torch.float32, device=device) for _ in range(2))
+            self._gy_t, self._gx_t = (torch.empty(self.d_model * ld, dtype=torch.float32, device=device) for _ in range(2))
+            self._gx = torch.empty(n, self.d_model, dtype=torch.float32, device=device)
             self._tokens = n
             self._last_forward = None
             self.growths += 1
@@ -182,7 +182,7 @@ class HFFNTrainRuntime:
         width = max(state.columns[3] for state in self._layers)
         if tiles * width >= 1 << 32:
             raise ValueError(f"{tiles} token tiles x {width} partial columns do not fit the kernels' 32-bit offsets")
-        self._partials = torch.empty(tiles * width, device=self.runtime.device)
+        self._partials = torch.empty(tiles * width, dtype=torch.float32, device=self.runtime.device)
         self._tiles = tiles
         self.growths += 1
 
