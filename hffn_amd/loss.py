@@ -16,7 +16,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .runtime import MAX_TOKENS, _device, _value_type, current_stream
+from .runtime import MAX_TOKENS, StreamUses, _device, _value_type, current_stream
 
 REDUCTIONS = ("mean", "sum")
 PIECE_BYTES = 512 << 20
@@ -70,12 +70,16 @@ class HeadLoss:
         self._gx: torch.Tensor | None = None
         self._loss: torch.Tensor | None = None
         self.grad: torch.Tensor | None = None  # gw of the last step
-        self._stream: int | None = None
+        self._streams = StreamUses()
         self._sized = [0, 0]  # tokens the buffers were last sized for, for losses and for step (more may need less: fewer pieces)
         self.reserve(max_tokens, gradients=False)
 
     def _bytes(self, n: int, gradients: bool) -> int:
         return _lib.query_bytes(self._lib.hffn_loss_workspace, self.value_type, n, self.d_model, self.vocab, self._aligned, int(gradients), self.piece_bytes)
+
+    def _new(self, *shape: int, dtype: torch.dtype) -> torch.Tensor:
+        self._streams.allocated()
+        return torch.empty(shape, dtype=dtype, device=self.device)
 
     def reserve(self, n: int, gradients: bool = True) -> None:
         """Size the buffers for calls of ``n`` tokens (``gradients``: for ``step`` too); allocates what must grow."""
@@ -85,14 +89,14 @@ class HeadLoss:
             return
         need = self._bytes(n, gradients)
         if self._workspace is None or self._workspace.numel() < need:
-            self._workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
+            self._workspace = self._new(need, dtype=torch.uint8)
         if self._losses is None or self._losses.numel() < n:
-            self._losses = torch.empty(n, dtype=torch.float32, device=self.device)
+            self._losses = self._new(n, dtype=torch.float32)
         if gradients and (self._gx is None or self._gx.shape[0] < n):
-            self._gx = torch.empty(n, self.d_model, dtype=self.weight.dtype, device=self.device)
+            self._gx = self._new(n, self.d_model, dtype=self.weight.dtype)
         if gradients and self.grad is None:
-            self.grad = torch.empty_like(self.weight)
-            self._loss = torch.empty((), dtype=torch.float32, device=self.device)
+            self.grad = self._new(self.vocab, self.d_model, dtype=self.weight.dtype)
+            self._loss = self._new(dtype=torch.float32)
         self._sized[gradients] = n
 
     def workspace_bytes(self) -> int:
@@ -106,14 +110,8 @@ class HeadLoss:
             raise ValueError(f"labels: an int32 or int64 [{n}] tensor on {self.device} is required, not {labels.dtype} "
                              f"{list(labels.shape)} on {labels.device}")
         stream = current_stream(self.device)
-        if stream != self._stream:
-            if self._stream is not None:  # buffers of another stream's pool stay until this one is done with them
-                for t in (self._workspace, self._losses, self._gx, self._loss, self.grad):
-                    if t is not None:
-                        t.record_stream(torch.cuda.current_stream(self.device))
-            self._stream = stream
-        if n:
-            self.reserve(n, gradients)
+        self.reserve(max(n, 1), gradients)
+        self._streams.use(stream, self.device, (self._workspace, self._losses, self._gx, self._loss, self.grad))
         return x, (self.value_type, x.data_ptr(), stride, self.weight.data_ptr(), labels.data_ptr(), labels.stride(0) if n > 1 else 1,
                    _LABEL_BYTES[labels.dtype], self.ignore_index), stream
 
@@ -134,7 +132,6 @@ class HeadLoss:
         x, args, stream = self._call(x, labels, True)
         n = x.shape[0]
         if n == 0:
-            self.reserve(1)
             return self._loss.zero_(), self._gx[:0], self.grad.zero_()
         _lib.check(self._lib.hffn_loss_step(*args, int(self.reduction == "mean"), scale, self.piece_bytes, self._loss.data_ptr(), self._gx.data_ptr(),
                                             self.grad.data_ptr(), self._workspace.data_ptr(), self._workspace.numel(), self.d_model,

@@ -21,7 +21,7 @@ import torch
 
 from . import _lib
 from .loss import rows_of
-from .runtime import _device, _value_type, current_stream
+from .runtime import StreamUses, _device, _value_type, current_stream
 
 KINDS = ("layer", "rms")
 PARAMETERS = ("weight", "bias", "gate", "post_weight", "post_bias")
@@ -66,6 +66,7 @@ class ResidualNorm:
                 raise ValueError(f"{name} must be a contiguous float32 [{self.d_model}] tensor on {self.device}")
             self._parameters[name] = t.detach()
         self._gradients: dict[str, torch.Tensor] = {}
+        self._streams = StreamUses()
         self._lib = _lib.load()
 
     def parameters(self) -> dict[str, torch.Tensor]:
@@ -120,6 +121,8 @@ class ResidualNorm:
         g = self._gradients
         if not g:
             g.update((name, torch.empty_like(t)) for name, t in p.items())
+        stream = current_stream(self.device)
+        self._streams.use(stream, self.device, g.values())
         if n == 0:
             for t in g.values():
                 t.zero_()
@@ -128,6 +131,6 @@ class ResidualNorm:
         _lib.check(self._lib.hffn_residual_norm_backward(
             value_type, r.data_ptr(), r_stride, _pointer(f), f_stride, _pointer(gr), gr_stride, gh.data_ptr(), gh_stride,
             p["weight"].data_ptr(), *(_pointer(p.get(name)) for name in PARAMETERS[2:]), self.scale, self.eps, int(self.kind == "layer"),
-            gx.data_ptr(), _pointer(gf), *(_pointer(g.get(name)) for name in PARAMETERS), work.data_ptr(), work.numel(), d, n,
-            current_stream(self.device)), "residual norm backward")
+            gx.data_ptr(), _pointer(gf), *(_pointer(g.get(name)) for name in PARAMETERS), work.data_ptr(), work.numel(), d, n, stream),
+                   "residual norm backward")
         return gx, gf

@@ -45,6 +45,7 @@ from __future__ import annotations
 import ctypes
 import math
 from collections import Counter
+from collections.abc import Iterable
 from dataclasses import dataclass
 
 import torch
@@ -215,6 +216,29 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 def current_stream(device: torch.device) -> int:
     """The handle of PyTorch's current stream of the device (1.7 us less than through its stream object)."""
     return _raw_stream(device.index) if _raw_stream else torch.cuda.current_stream(device).cuda_stream
+
+
+class StreamUses:
+    """The streams that an object's own buffers are known to be used on. A buffer belongs to the stream current at its
+    allocation; the allocator gives its memory to that stream's next tensors as soon as it is dropped, unless it was told of
+    the other streams whose queued work still uses it."""
+
+    def __init__(self) -> None:
+        self._known: set[int] = set()
+
+    def allocated(self) -> None:
+        """A buffer is new: on any stream that comes next, buffers are made known again."""
+        self._known.clear()
+
+    def use(self, stream: int, device: torch.device, buffers: Iterable[torch.Tensor | None]) -> None:
+        """The buffers are used on ``stream``, the current one."""
+        if stream in self._known:
+            return
+        current = torch.cuda.current_stream(device)
+        for t in buffers:
+            if t is not None:
+                t.record_stream(current)
+        self._known.add(stream)
 
 
 def _value_type(tensor: torch.Tensor, name: str) -> int:
