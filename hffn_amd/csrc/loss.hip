@@ -1254,7 +1254,9 @@ Plan plan_of(int vt, uint32_t n, uint32_t d, uint32_t vocab, bool aligned, bool 
     p.pieces = 1;
     p.piece = padded(vocab, kTile);
     if (gradients) {
-        const uint64_t most = (piece_bytes == 0 ? kLossPieceBytes : piece_bytes) / (2ull * p.words * p.n_pad * kTile);
+        // A tile of D's rows is read by 32-bit byte offsets from its first (Operand::begin), which its last row must not pass.
+        const uint64_t reach = ((1ull << 32) - 256) / (2ull * p.words * (p.token_tile - 1) * kTile);
+        const uint64_t asked = (piece_bytes == 0 ? kLossPieceBytes : piece_bytes) / (2ull * p.words * p.n_pad * kTile), most = asked < reach ? asked : reach;
         const uint32_t tiles = ceil_div(vocab, kTile), fit = most < 1 ? 1 : most < tiles ? static_cast<uint32_t>(most) : tiles;
         p.piece = ceil_div(tiles, ceil_div(tiles, fit)) * kTile;
         p.pieces = ceil_div(vocab, p.piece);

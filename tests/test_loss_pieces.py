@@ -1,0 +1,22 @@
+"""How large a piece of the vocabulary may be, by the workspace it takes, without a GPU: no larger than the kernels' offsets reach,
+whatever is asked for."""
+from __future__ import annotations
+
+import pytest
+
+from hffn_amd import _lib
+
+F32, BF16 = 0, 1
+
+
+def loss_bytes(value_type, n, d, vocab, piece):
+    return _lib.query_bytes(_lib.load().hffn_loss_workspace, value_type, n, d, vocab, 1, 1, piece)
+
+
+@pytest.mark.parametrize("value_type,n,rows", [(BF16, 256, 256), (BF16, 1000, 256), (F32, 256, 128), (F32, 300, 128)])
+def test_rows_of_a_piece_lie_within_32_bits(value_type, n, rows):
+    """A tile of ``rows`` tokens is read by 32-bit byte offsets: its last row starts below 2^32 bytes after the first. Asking for
+    more gives the piece, and the workspace, of the largest row that does."""
+    vocab, per_row = 1 << 24, (1 << 32) // (rows - 1)
+    tokens = -(-n // 256) * 256
+    assert loss_bytes(value_type, n, 8, vocab, 1 << 50) <= loss_bytes(value_type, n, 8, vocab, per_row * tokens)
