@@ -18,6 +18,7 @@
 // 1.97 GHz with the units busy 54 % of the time, a library product of the same operands 1472 us, at 1.56 GHz and 71 %.
 // 2048 tokens of 1024: 232 to 274 us a product (211 GFLOP). 512 float32 tokens of 1024: 184 to 245 us (158 GFLOP in fp16), and 95 us
 // that pack the weight (412 MB). One bfloat16 token of 2048: 49 us for the weight's 206 MB, 4.2 TB/s.
+#include <algorithm>
 #include <type_traits>
 
 #include "common.hpp"
@@ -1254,9 +1255,12 @@ Plan plan_of(int vt, uint32_t n, uint32_t d, uint32_t vocab, bool aligned, bool 
     p.pieces = 1;
     p.piece = padded(vocab, kTile);
     if (gradients) {
-        // A tile of D's rows is read by 32-bit byte offsets from its first (Operand::begin), which its last row must not pass.
+        // A tile of D's rows is read by 32-bit byte offsets from its first (Operand::begin), which its last row must not pass; a
+        // launch has below 2^32 threads, and loss_turn_kernel's one for 8 entries of D, in whole blocks of a row.
         const uint64_t reach = ((1ull << 32) - 256) / (2ull * p.words * (p.token_tile - 1) * kTile);
-        const uint64_t asked = (piece_bytes == 0 ? kLossPieceBytes : piece_bytes) / (2ull * p.words * p.n_pad * kTile), most = asked < reach ? asked : reach;
+        const uint64_t turned = (1ull << 32) / (kTile / 8 * static_cast<uint64_t>(p.n_pad)) - 8 * kTurnThreads / kTile;
+        const uint64_t asked = (piece_bytes == 0 ? kLossPieceBytes : piece_bytes) / (2ull * p.words * p.n_pad * kTile);
+        const uint64_t most = std::min({asked, reach, turned});
         const uint32_t tiles = ceil_div(vocab, kTile), fit = most < 1 ? 1 : most < tiles ? static_cast<uint32_t>(most) : tiles;
         p.piece = ceil_div(tiles, ceil_div(tiles, fit)) * kTile;
         p.pieces = ceil_div(vocab, p.piece);

@@ -48,7 +48,7 @@ class HeadLoss:
                  piece_bytes: int = PIECE_BYTES) -> None:
         """``max_tokens``: the calls the buffers are first sized for (``losses``; ``step``'s own come with its first call or
         ``reserve``). ``piece_bytes``: what a piece of the vocabulary's softmax may take in ``step`` (N tokens times its rows, 2
-        bytes an entry in bfloat16, 4 in float32; 256 rows at least, 8.4 million at most): the last piece's logits are computed
+        bytes an entry in bfloat16, 4 in float32; 256 rows at least, 8.4 million and 2^35 entries at most): the last piece's logits are computed
         once, the others' twice."""
         self.device = _device(weight.device)
         if weight.dim() != 2 or not weight.is_contiguous() or weight.numel() == 0:

@@ -438,7 +438,7 @@ int hffn_clip(uint32_t arrays, void* const* p, void* const* out, const uint64_t*
  * gradients of scale times it: gx [n, d_model] (zero rows for ignored tokens, whatever their x holds) and gw [vocab, d_model],
  * of the value type; a label outside the vocabulary makes all of them NaN. Logits are not kept; the gradients are computed in
  * pieces of the vocabulary whose softmax (16 bits an entry, float32: 32) takes at most piece_bytes (0:
- * HFFN_LOSS_PIECE_BYTES; 256 vocabulary rows at least, 8.4 million at most). The last piece's logits are computed once, the
+ * HFFN_LOSS_PIECE_BYTES; 256 vocabulary rows at least, 8.4 million and 2^35 entries at most). The last piece's logits are computed once, the
  * others' twice: a larger piece is faster. Workspace: hffn_loss_workspace bytes (aligned: the weight starts on a 16-byte boundary;
  * gradients: for hffn_loss_step with this piece_bytes), any content, 256-byte aligned. Outputs may not overlap inputs. */
 #define HFFN_MAX_VOCAB (1u << 24)

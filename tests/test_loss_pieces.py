@@ -20,3 +20,10 @@ def test_rows_of_a_piece_lie_within_32_bits(value_type, n, rows):
     vocab, per_row = 1 << 24, (1 << 32) // (rows - 1)
     tokens = -(-n // 256) * 256
     assert loss_bytes(value_type, n, 8, vocab, 1 << 50) <= loss_bytes(value_type, n, 8, vocab, per_row * tokens)
+
+
+@pytest.mark.parametrize("value_type,size", [(BF16, 2), (F32, 4)])
+@pytest.mark.parametrize("n", (1 << 18, (1 << 18) - 1, 100_000))
+def test_a_piece_fits_a_launch(value_type, size, n):
+    """A launch of below 2^32 threads turns a piece's exponentials into D, 8 entries a thread."""
+    assert loss_bytes(value_type, n, 8, 1 << 20, 1 << 50) <= loss_bytes(value_type, n, 8, 1 << 20, (1 << 35) * size)
