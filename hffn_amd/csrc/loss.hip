@@ -9,9 +9,10 @@
 // Every product is out[b][a] = sum_k A[a, k] B[b, k] on 16-bit MFMA operands with float32 sums. bfloat16 calls multiply
 // their entries as they are (D rounded to bfloat16: 2^-8 of an entry, as the gradients themselves are rounded). float32
 // calls hold every operand as fp16 hi + lo of the entry times a power of two of its tensor (22 bits down to 2^-12 of the
-// largest entry) and take hi hi + hi lo + lo hi; those of a few tokens, which wait for the weight's bytes, read it as it is
-// and split it where it is multiplied into three bfloat16 parts (no power of two to know first), of whose nine products the six
-// down to 2^-16 count.
+// largest entry, 2^-34 of that below) and take hi hi + hi lo + lo hi; those of a few tokens, which wait for the weight's bytes,
+// read it as it is and split it where it is multiplied into three bfloat16 parts (no power of two to know first), of whose nine
+// products the six down to 2^-16 count. Calls whose entries spread too far for one power of two (kSpread) take the three parts
+// as well: the kernels of both forms are launched, and what the preparing launches saw says which ones do the work.
 //
 // What bounds it: many tokens, the matrix units and their power. 8192 bfloat16 tokens of 2048 x 50304: five products per half of
 // the vocabulary (844 GFLOP each) of 720 to 850 us, 1.0 to 1.17 PFLOP/s; the forward's over the whole vocabulary takes 1508 us, at
@@ -47,12 +48,20 @@ typedef __attribute__((address_space(3))) const float* LdsFloat;
 constexpr int kLift = 10;      // the entry an operand's power of two is taken from lies in [2^9, 2^10) ...
 constexpr int kRoom = 5;       // ... and its largest up to kRoom binades above
 constexpr int kGradLift = 14;  // |D| <= 1 is kept times 2^kGradLift
-constexpr int kChain = 4;      // k-tiles whose products are summed in the MFMA accumulators (float32 calls)
+// Eight neighbouring entries of a row whose largest lies this many binades below the entry that the tensor's power of two is
+// taken from would keep fewer than 20 bits of that largest: one row of 1e7 times the others cost these 1e-3 in their losses. Three
+// parts in their place: losses of 512 tokens of 512 x 50304 in 225 us, not 158, steps of 1024 x 50304 in 1350, not 720; the
+// launches of the form that does not run cost 1 % of either.
+constexpr int kSpread = 14;
+// k-tiles whose products are summed in the MFMA accumulators (float32 calls): of two parts, of three (twice the additions; logits of
+// 10^3, gx's 2-norm: 1.2e-5 off with 4, below 1e-5 with 1, at the same time)
+constexpr int kChain2 = 4, kChain3 = 1;
 
 // What the first launches leave for the others: counted tokens, labels outside the vocabulary, and (float32) the bits of
 // the magnitudes that the powers of two are taken from, and of the samples they were first taken from.
 struct Meta {
     uint32_t valid, invalid, weight_bits, x_bits, weight_sample, x_sample;
+    uint32_t wide;  // float32 of many tokens: entries spread beyond kSpread
 };
 __device__ __forceinline__ int lift_of(uint32_t bits) {  // e with 2^-e times that magnitude in [2^9, 2^10)
     return bits == 0 ? 0 : ilogbf(__uint_as_float(bits)) - (kLift - 1);
@@ -98,7 +107,7 @@ struct Prepare {
     float* losses;
     Meta* meta;
     uint16_t *x_out, *w_out, *x_split;  // x_split: RAW, the counted rows of x as per 32 entries 3 x 32 bfloat16 parts
-    uint32_t *x_most, *w_most;  // float32: largest finite magnitude of each block's rows, bits
+    uint2 *x_most, *w_most;  // float32: the Seen of each block's rows
     uint32_t x_blocks, w_blocks;
 };
 
@@ -159,6 +168,20 @@ __device__ __forceinline__ uint32_t magnitude(float v) {  // bits of |v|, 0 for 
     return bits < 0x7f800000u ? bits : 0u;
 }
 
+// What a thread saw of a tensor's finite magnitudes (bits): the largest; and of the largest of every eight neighbours, where not
+// zero, the smallest, as its complement (0: none seen), so that both are joined by the larger.
+struct Seen {
+    uint32_t most = 0, small = 0;
+    __device__ __forceinline__ void take(uint32_t of_eight) {
+        most = max(most, of_eight);
+        if (of_eight != 0) small = max(small, ~of_eight);
+    }
+    __device__ __forceinline__ void join(uint2 other) {
+        most = max(most, other.x);
+        small = max(small, other.y);
+    }
+};
+
 constexpr uint32_t kPrepThreads = 256, kPrepWaves = kPrepThreads / kWave, kWeightRows = 16;  // weight rows a block
 
 // The largest of the threads' values, in every thread (one barrier before and after: lds may be used again).
@@ -199,13 +222,12 @@ __device__ __forceinline__ void split_pair(float low, float high, uint32_t (&wor
     }
 }
 
-// One operand row by a wave, eight entries a lane and step; returns the largest finite magnitude that the lane saw. RAW:
-// float32 as they are, and their parts to `split_to`.
+// One operand row by a wave, eight entries a lane and step; `seen`: of the lane's finite magnitudes. RAW: float32 as they are, and
+// their parts to `split_to`.
 template <typename T, bool RAW>
-__device__ __forceinline__ uint32_t pack_row(const T* __restrict__ from, uint16_t* __restrict__ to, uint32_t d, uint32_t width, int e,
-                                             uint16_t* __restrict__ split_to = nullptr) {
+__device__ __forceinline__ void pack_row(const T* __restrict__ from, uint16_t* __restrict__ to, uint32_t d, uint32_t width, int e,
+                                         Seen& seen, uint16_t* __restrict__ split_to = nullptr) {
     const uint32_t lane = threadIdx.x % kWave;
-    uint32_t most = 0;
     for (uint32_t c = 8 * lane; c < width; c += 8 * kWave) {
         if constexpr (sizeof(T) == 4) {
             float v[8];
@@ -232,7 +254,7 @@ __device__ __forceinline__ uint32_t pack_row(const T* __restrict__ from, uint16_
                         make_uint4(words[0][part], words[1][part], words[2][part], words[3][part]);
                 continue;
             }
-            uint32_t hi[4], lo[4];
+            uint32_t hi[4], lo[4], most = 0;
 #pragma unroll
             for (uint32_t k = 0; k < 8; k += 2) {
                 uint16_t h[2], l[2];
@@ -242,6 +264,9 @@ __device__ __forceinline__ uint32_t pack_row(const T* __restrict__ from, uint16_
                 hi[k / 2] = h[0] | static_cast<uint32_t>(h[1]) << 16;
                 lo[k / 2] = l[0] | static_cast<uint32_t>(l[1]) << 16;
             }
+            if (c < d && c + 8 > d)  // the row's last entries: with those before them
+                for (uint32_t k = d < 8 ? d : 8; k > 0; --k) most = max(most, magnitude(from[d - k]));
+            seen.take(most);
             uint16_t* out = to + c / 32 * 64 + c % 32;
             *reinterpret_cast<uint4*>(out) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
             *reinterpret_cast<uint4*>(out + 32) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
@@ -259,19 +284,22 @@ __device__ __forceinline__ uint32_t pack_row(const T* __restrict__ from, uint16_
             *reinterpret_cast<uint4*>(to + c) = make_uint4(v[0], v[1], v[2], v[3]);
         }
     }
-    return most;
 }
 
-// The weight's rows of block `block`; returns the thread's largest magnitude.
+// The weight's rows of block `block`.
 template <typename T>
-__device__ __forceinline__ uint32_t pack_weight(const Prepare& p, uint32_t block, int e) {
+__device__ __forceinline__ void pack_weight(const Prepare& p, uint32_t block, int e, Seen& seen) {
     constexpr uint64_t kParts = sizeof(T) == 4 ? 2 : 1;
-    uint32_t most = 0;
     for (uint32_t r = threadIdx.x / kWave; r < kWeightRows; r += kPrepWaves) {
         const uint64_t row = static_cast<uint64_t>(block) * kWeightRows + r;
-        if (row < p.vocab) most = max(most, pack_row<T, false>(static_cast<const T*>(p.weight) + row * p.d, p.w_out + row * kParts * p.width, p.d, p.width, e));
+        if (row < p.vocab) pack_row<T, false>(static_cast<const T*>(p.weight) + row * p.d, p.w_out + row * kParts * p.width, p.d, p.width, e, seen);
     }
-    return most;
+}
+
+// Compact row i of x_split to zeros, by a wave.
+__device__ __forceinline__ void clear_split(const Prepare& p, uint32_t i) {
+    uint4* parts = reinterpret_cast<uint4*>(p.x_split + static_cast<uint64_t>(i) * 3 * p.width);
+    for (uint32_t c = threadIdx.x % kWave; c < 3 * p.width / 8; c += kWave) parts[c] = make_uint4(0, 0, 0, 0);
 }
 
 // A block per kPrepWaves tokens (a wave each, and the compact row of the same number where zeros belong) and, after those,
@@ -290,9 +318,10 @@ __global__ __launch_bounds__(kPrepThreads) void loss_prepare_kernel(Prepare p) {
             e = lift_of(sample);
             if (block == 0 && threadIdx.x == 0) p.meta->weight_sample = sample;
         }
-        const uint32_t most = pack_weight<T>(p, block, e);
+        Seen seen;
+        pack_weight<T>(p, block, e, seen);
         if constexpr (kScaled) {
-            const uint32_t all = block_most(most, most_lds);
+            const uint2 all = make_uint2(block_most(seen.most, most_lds), block_most(seen.small, most_lds));
             if (threadIdx.x == 0) p.w_most[block] = all;
         }
         return;
@@ -354,47 +383,56 @@ __global__ __launch_bounds__(kPrepThreads) void loss_prepare_kernel(Prepare p) {
         e = lift_of(sample);
         if (blockIdx.x == 0 && threadIdx.x == 0) p.meta->x_sample = sample;
     }
-    uint32_t most = 0;
-    uint16_t* const split_rows = RAW ? p.x_split : nullptr;
+    Seen seen;
     if (counted)
-        most = pack_row<T, RAW>(static_cast<const T*>(p.x) + i * p.x_stride, p.x_out + at * kParts * p.width, p.d, p.width, e,
-                                RAW ? split_rows + static_cast<uint64_t>(at) * 3 * p.width : nullptr);
+        pack_row<T, RAW>(static_cast<const T*>(p.x) + i * p.x_stride, p.x_out + at * kParts * p.width, p.d, p.width, e, seen,
+                         RAW ? p.x_split + static_cast<uint64_t>(at) * 3 * p.width : nullptr);
     if (i >= valid && i < (valid + 63) / 64 * 64) {
         uint4* out = reinterpret_cast<uint4*>(p.x_out + i * kParts * p.width);
         for (uint32_t c = lane; c < kParts * p.width / 8; c += kWave) out[c] = make_uint4(0, 0, 0, 0);
-        if constexpr (RAW) {
-            uint4* parts = reinterpret_cast<uint4*>(split_rows + static_cast<uint64_t>(i) * 3 * p.width);
-            for (uint32_t c = lane; c < 3 * p.width / 8; c += kWave) parts[c] = make_uint4(0, 0, 0, 0);
-        }
+        if constexpr (RAW) clear_split(p, i);
     }
     if constexpr (kScaled) {
-        const uint32_t all = block_most(most, most_lds);
+        const uint2 all = make_uint2(block_most(seen.most, most_lds), block_most(seen.small, most_lds));
         if (threadIdx.x == 0) p.x_most[blockIdx.x] = all;
     }
 }
 
 // float32: the powers of two that hold, from the blocks' largest magnitudes, and the operands packed again where the
-// sample's did not.
+// sample's did not. Where entries spread beyond kSpread, x's counted rows are packed as they are and as three parts instead
+// (the weight is read in place then).
 __global__ __launch_bounds__(kPrepThreads) void loss_settle_kernel(Prepare p) {
     __shared__ uint32_t lds[kPrepWaves];
-    const auto settled = [&](const uint32_t* most, uint32_t blocks, uint32_t sample) -> uint32_t {
-        uint32_t largest = 0;
-        for (uint32_t i = threadIdx.x; i < blocks; i += kPrepThreads) largest = max(largest, most[i]);
-        largest = block_most(largest, lds);
-        return largest == 0 || (sample != 0 && lift_of(largest) - lift_of(sample) <= kRoom) ? sample : largest;
+    bool wide = false;
+    const auto settled = [&](const uint2* blocks_seen, uint32_t blocks, uint32_t sample) -> uint32_t {
+        Seen seen;
+        for (uint32_t i = threadIdx.x; i < blocks; i += kPrepThreads) seen.join(blocks_seen[i]);
+        const uint32_t largest = block_most(seen.most, lds), small = block_most(seen.small, lds);
+        const uint32_t bits = largest == 0 || (sample != 0 && lift_of(largest) - lift_of(sample) <= kRoom) ? sample : largest;
+        wide = wide || (small != 0 && lift_of(bits) - lift_of(~small) > kSpread);
+        return bits;
     };
     const uint32_t x_sample = p.meta->x_sample, w_sample = p.meta->weight_sample, valid = p.meta->valid;
     const uint32_t x_bits = settled(p.x_most, p.x_blocks, x_sample), w_bits = settled(p.w_most, p.w_blocks, w_sample);
     if (blockIdx.x == 0 && threadIdx.x == 0) {
         p.meta->x_bits = x_bits;
         p.meta->weight_bits = w_bits;
+        p.meta->wide = wide;
     }
-    if (x_bits != x_sample)
-        for (uint32_t i = blockIdx.x * kPrepWaves + threadIdx.x / kWave; i < valid; i += gridDim.x * kPrepWaves)
-            pack_row<float, false>(static_cast<const float*>(p.x) + p.rows[i] * p.x_stride, p.x_out + static_cast<uint64_t>(i) * 2 * p.width, p.d, p.width,
-                     lift_of(x_bits));
-    if (w_bits != w_sample)
-        for (uint32_t block = blockIdx.x; block < p.w_blocks; block += gridDim.x) pack_weight<float>(p, block, lift_of(w_bits));
+    Seen again;
+    if (wide || x_bits != x_sample)
+        for (uint32_t i = blockIdx.x * kPrepWaves + threadIdx.x / kWave; i < (valid + 63) / 64 * 64; i += gridDim.x * kPrepWaves) {
+            if (i >= valid) {  // x_out's rows are zeros already
+                if (wide) clear_split(p, i);
+                continue;
+            }
+            const float* from = static_cast<const float*>(p.x) + p.rows[i] * p.x_stride;
+            uint16_t* to = p.x_out + static_cast<uint64_t>(i) * 2 * p.width;
+            if (wide) pack_row<float, true>(from, to, p.d, p.width, 0, again, p.x_split + static_cast<uint64_t>(i) * 3 * p.width);
+            else pack_row<float, false>(from, to, p.d, p.width, lift_of(x_bits), again);
+        }
+    if (!wide && w_bits != w_sample)
+        for (uint32_t block = blockIdx.x; block < p.w_blocks; block += gridDim.x) pack_weight<float>(p, block, lift_of(w_bits), again);
 }
 
 // --------------------------------------------------------------------------------------------------------- the product
@@ -605,6 +643,10 @@ __device__ __forceinline__ uint64_t slice_at(uint32_t slice, uint32_t t, uint32_
 // Stats: slices' maxima and sums; Keep: those, and the exponentials kept where D belongs; Grad: D.
 enum class Use { Stats, Keep, Grad, GradX, GradW };
 
+// float32 calls of many tokens: whether a launch is for entries that lie near enough for one power of two a tensor, or for others.
+enum class Spread : uint8_t { Any, Near, Wide };
+__device__ __forceinline__ bool skipped(Spread only, const Meta& meta) { return only != Spread::Any && (only == Spread::Wide) != (meta.wide != 0); }
+
 // One product of a loss call: which operands, how far they go, and what becomes of the results.
 struct Product {
     const uint16_t *a, *b;
@@ -632,6 +674,7 @@ struct Product {
     uint64_t out_stride;
     float scale;
     bool mean, out_bf16;
+    Spread only;                  // the calls that this launch does the work of
 };
 
 // WA x WB waves of TA x TB 32 x 32 results each; k-tiles go through a ring of kStages tile pairs.
@@ -733,11 +776,12 @@ __device__ __forceinline__ void meet() {
 // The sums of a tile whose first k-tiles are under way. Operands of a step (16 k) are read from LDS while the step before it
 // multiplies; the last step of a k-tile reads the first of the next, behind the barrier that says every wave's transfers
 // of it have landed and every wave has read the last of the k-tile before it, whose stage the transfers of k-tile
-// kt + kStages then take. float32: sums of kChain k-tiles in the MFMA accumulators (whose own sums round downwards), added to
+// kt + kStages then take. float32: sums of kChain2 or kChain3 k-tiles in the MFMA accumulators (whose own sums round downwards), added to
 // others.
 template <typename S>
 __device__ __forceinline__ void accumulate(const Tile<S>& tile, const char* ring, Acc (&sums)[S::TA][S::TB]) {
     constexpr int PARTS = S::PARTS, TA = S::TA, TB = S::TB, kSteps = PARTS == 1 ? 4 : 2, kTransfers = static_cast<int>(S::kTransfers);
+    constexpr uint32_t kChain = PARTS == 3 ? kChain3 : kChain2;
     static_assert(kSteps % 2 == 0, "a k-tile's first step always reads into the same registers");
     const uint32_t wave = threadIdx.x / kWave, lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(ring));
     const uint32_t a_place = S::OpA::place(wave % S::WA * TA * 32), b_place = S::OpB::place(wave / S::WA * TB * 32);
@@ -792,9 +836,11 @@ __device__ __forceinline__ void accumulate(const Tile<S>& tile, const char* ring
 #pragma unroll
                 for (int j = 0; j < TB; ++j)
 #pragma unroll
-                    for (int k = 0; k < PARTS; ++k)  // the parts' products down to the last part's weight
+                    for (int q = 0; q < PARTS; ++q) {  // the parts' products down to the last part's weight; three parts: the least first
+                        const int sum = PARTS == 3 ? PARTS - 1 - q : q;
 #pragma unroll
-                        for (int m = 0; k + m < PARTS; ++m) acc(i, j) = multiply<PARTS>(a[i].part[k], b[j].part[m], acc(i, j));
+                        for (int k = 0; k <= sum; ++k) acc(i, j) = multiply<PARTS>(a[i].part[k], b[j].part[sum - k], acc(i, j));
+                    }
         }
         if constexpr (PARTS != 1) {
             if ((kt - k_begin) % kChain == kChain - 1 || kt + 1 == k_end) {
@@ -1023,6 +1069,7 @@ __global__ __launch_bounds__(WA* WB* kWave) __attribute__((amdgpu_waves_per_eu(2
                                                           : (Quarter::kLds > Half::kLds ? Quarter::kLds : Half::kLds);
     __shared__ __attribute__((aligned(1024))) char ring[kLds];
     const Meta meta = *p.meta;
+    if (PARTS != 1 && skipped(p.only, meta)) return;
     const uint32_t live_b = USE == Use::GradW ? p.b_tiles : (meta.valid + Whole::kB - 1) / Whole::kB;
     const uint64_t tiles = static_cast<uint64_t>(p.a_tiles) * live_b * p.splits;
     const uint32_t xcd = blockIdx.x % kXcds, local = blockIdx.x / kXcds, blocks = gridDim.x / kXcds;
@@ -1057,7 +1104,14 @@ __global__ __launch_bounds__(WA* WB* kWave) __attribute__((amdgpu_waves_per_eu(2
 
 // ------------------------------------------------------------------------------------------- the sums over the vocabulary
 
-// lse and loss of every counted token from the slices: TOKENS tokens a block, 1024 / TOKENS threads each over the slices.
+// Where a product left its slices: how many there are, and the pitch of slice_at.
+struct Slices {
+    const float2* at;
+    uint32_t count, pitch;
+};
+
+// lse and loss of every counted token from the slices: TOKENS tokens a block, 1024 / TOKENS threads each over the slices. `wide`:
+// the slices, token by token, of calls whose entries spread (null: there are no such calls).
 constexpr uint32_t kLseThreads = 1024, kLseWaves = kLseThreads / kWave;
 __device__ __forceinline__ float2 joined(float2 a, float2 b) {
     const float most = fmaxf(a.x, b.x);
@@ -1071,18 +1125,21 @@ __device__ __forceinline__ float2 joined_lanes(float2 v) {  // over the lanes of
     return v;
 }
 template <uint32_t TOKENS>
-__global__ __launch_bounds__(kLseThreads) void loss_lse_kernel(const float2* __restrict__ slices, uint32_t count, uint32_t pitch,
-                                                              const float* __restrict__ picked, const int32_t* __restrict__ rows,
+__global__ __launch_bounds__(kLseThreads) void loss_lse_kernel(Slices near, Slices wide, const float* __restrict__ picked, const int32_t* __restrict__ rows,
                                                               const int32_t* __restrict__ labels, const Meta* __restrict__ meta,
                                                               float* __restrict__ lse, float* __restrict__ losses) {
+    const bool by_token = wide.at != nullptr && meta->wide != 0;
     constexpr uint32_t kLanes = kLseThreads / TOKENS;
     __shared__ float2 lds[kLseWaves * TOKENS];
     const uint32_t in = threadIdx.x % TOKENS, t = blockIdx.x * TOKENS + in, valid = meta->valid, lane = threadIdx.x % kWave;
     if (blockIdx.x * TOKENS >= valid) return;
     float2 all = make_float2(-__builtin_huge_valf(), 0.0f);
-    if (t < valid)
+    if (t < valid && by_token) {
+        for (uint32_t s = threadIdx.x / TOKENS; s < wide.count; s += kLanes) all = joined(all, wide.at[slice_at<true>(s, t, wide.pitch)]);
+    } else if (t < valid) {
 #pragma unroll 4
-        for (uint32_t s = threadIdx.x / TOKENS; s < count; s += kLanes) all = joined(all, slices[slice_at<TOKENS == 1>(s, t, pitch)]);
+        for (uint32_t s = threadIdx.x / TOKENS; s < near.count; s += kLanes) all = joined(all, near.at[slice_at<TOKENS == 1>(s, t, near.pitch)]);
+    }
     all = joined_lanes<TOKENS>(all);
     if (lane < TOKENS) lds[threadIdx.x / kWave * TOKENS + in] = all;
     __syncthreads();
@@ -1104,12 +1161,15 @@ __global__ __launch_bounds__(kLseThreads) void loss_lse_kernel(const float2* __r
 // stores take less than its logits again: 2048 tokens of 1024 x 50304 bfloat16 75 + 25 against 283 us, 512 float32 40 + 5
 // against 222 us.
 constexpr uint32_t kTurnThreads = 256;
+// What the product that kept them was: its slices (of the piece's first on), vocabulary rows of a tile, slices of a tile and
+// rows of a slice.
+struct Kept {
+    const float2* slices;
+    uint32_t height, per_tile, slice_rows, pitch;
+};
 template <int PARTS>
-__global__ __launch_bounds__(kTurnThreads) void loss_turn_kernel(uint16_t* __restrict__ grad, uint64_t stride, uint32_t first, uint32_t count,
-                                                                uint32_t across, const float2* __restrict__ slices, uint32_t height,
-                                                                uint32_t per_tile, uint32_t slice_rows, uint32_t pitch,
-                                                                const float* __restrict__ lse, const int32_t* __restrict__ labels,
-                                                                const Meta* __restrict__ meta) {
+__device__ __forceinline__ void turn(uint16_t* __restrict__ grad, uint64_t stride, uint32_t first, uint32_t count, uint32_t across, const Kept& kept_by,
+                                     const float* __restrict__ lse, const int32_t* __restrict__ labels, const Meta* __restrict__ meta) {
     const uint32_t t = blockIdx.x / across, valid = meta->valid, c = (blockIdx.x % across * kTurnThreads + threadIdx.x) * 8;
     if (t >= (valid + 63) / 64 * 64 || c >= count) return;
     uint4* const at = reinterpret_cast<uint4*>(grad + t * stride + (PARTS == 1 ? c : PARTS == 2 ? c / 32 * 64 + c % 32 : 2 * c));
@@ -1119,7 +1179,8 @@ __global__ __launch_bounds__(kTurnThreads) void loss_turn_kernel(uint16_t* __res
         if constexpr (PARTS != 1) *low = make_uint4(0, 0, 0, 0);
         return;
     }
-    const float most = slices[slice_at<PARTS == 3>(c / height * per_tile + c % height / slice_rows, t, pitch)].x;
+    const uint32_t slice = c / kept_by.height * kept_by.per_tile + c % kept_by.height / kept_by.slice_rows;
+    const float most = kept_by.slices[slice_at<PARTS == 3>(slice, t, kept_by.pitch)].x;
     const float factor = exponential<2>(most - lse[t]) * (PARTS == 2 ? 1.0f / (1 << kGradLift) : 1.0f);
     const uint32_t label = static_cast<uint32_t>(labels[t]) - first - c;
     const uint4 kept = *at, rest = PARTS != 1 ? *low : make_uint4(0, 0, 0, 0);
@@ -1152,6 +1213,14 @@ __global__ __launch_bounds__(kTurnThreads) void loss_turn_kernel(uint16_t* __res
         *at = make_uint4(h[0], h[1], h[2], h[3]);
         *low = make_uint4(l[0], l[1], l[2], l[3]);
     }
+}
+template <int PARTS>
+__global__ __launch_bounds__(kTurnThreads) void loss_turn_kernel(uint16_t* __restrict__ grad, uint64_t stride, uint32_t first, uint32_t count,
+                                                                uint32_t across, Kept near, Kept wide, const float* __restrict__ lse,
+                                                                const int32_t* __restrict__ labels, const Meta* __restrict__ meta) {
+    if constexpr (PARTS == 2)
+        if (meta->wide != 0) return turn<3>(grad, stride, first, count, across, wide, lse, labels, meta);
+    turn<PARTS>(grad, stride, first, count, across, near, lse, labels, meta);
 }
 
 // gx of every token: the splits' sums in order times the factor; zeros for tokens that do not count. A wave per token and 256
@@ -1294,11 +1363,11 @@ Plan plan_of(int vt, uint32_t n, uint32_t d, uint32_t vocab, bool aligned, bool 
     p.losses = take(4ull * p.n_pad);
     p.slice_sums = take(sizeof(float2) * p.slices * p.n_pad);
     if (p.parts == 2) {
-        p.x_most = take(4ull * ceil_div(p.n_pad, kPrepWaves));
-        p.w_most = take(4ull * ceil_div(vocab, kWeightRows));
+        p.x_most = take(sizeof(uint2) * ceil_div(p.n_pad, kPrepWaves));
+        p.w_most = take(sizeof(uint2) * ceil_div(vocab, kWeightRows));
     }
     p.x = take(2ull * p.words * p.n_pad * p.width);
-    p.x_split = p.parts == 3 ? take(6ull * p.n_pad * p.width) : 0;
+    p.x_split = p.parts != 1 ? take(6ull * p.n_pad * p.width) : 0;
     p.weight = p.in_place ? 0 : take(2ull * p.words * vocab * p.width);
     if (gradients) {
         // splits of the vocabulary that give every CU a block (few tokens: two), each of 8 k-tiles at least
@@ -1319,17 +1388,28 @@ hipError_t launch_product(const Product& p, hipStream_t stream) {
     return hipGetLastError();
 }
 
+// One way to run a call's products: where the operands lie, and the tiles of the kernels that multiply them.
+struct Form {
+    uint32_t parts;
+    Spread only;
+    const uint16_t *weight, *x;  // x: as the weight's products read it
+    uint32_t w_columns;
+    uint64_t w_row, x_row;
+    uint32_t vocab_tile, height, per_tile, stats_tiles, keep_tiles, gw_tile, gw_rows;
+    Slices slices;
+};
+
 template <Use USE>
-hipError_t product(const Plan& plan, const Product& p, hipStream_t stream) {
+hipError_t product(const Plan& plan, const Form& form, const Product& p, hipStream_t stream) {
     if constexpr (USE != Use::GradW)  // which does not read the weight
-        if (plan.parts == 3 && !plan.whole) return launch_product<3, USE, 4, 1, 1, 2, 4>(p, stream);
-    if (plan.parts == 3) return launch_product<3, USE, 4, 1, 1, 2>(p, stream);
+        if (form.parts == 3 && !plan.whole) return launch_product<3, USE, 4, 1, 1, 2, 4>(p, stream);
+    if (form.parts == 3) return launch_product<3, USE, 4, 1, 1, 2>(p, stream);
     // gw of a few bfloat16 tokens, one k-tile a tile: 128 x 128, two blocks a CU (1 token of 1024 x 50304: a step of 113 us, 107 so)
     if constexpr (USE == Use::GradW)
         if (plan.few) return launch_product<1, USE, 4, 1, 1, 4>(p, stream);
     if constexpr (USE != Use::GradW && USE != Use::Keep)
         if (plan.few) return launch_product<1, USE, 4, 1, 1, 2>(p, stream);
-    return plan.parts == 1 ? launch_product<1, USE, 2, 4, 4, 2>(p, stream) : launch_product<2, USE, 4, 2, 2, 2>(p, stream);
+    return form.parts == 1 ? launch_product<1, USE, 2, 4, 4, 2>(p, stream) : launch_product<2, USE, 4, 2, 2, 2>(p, stream);
 }
 
 template <typename T>
@@ -1343,15 +1423,15 @@ hipError_t run(const LossCall& c, hipStream_t stream) {
     float *const lse = reinterpret_cast<float*>(work + plan.lse), *const picked = reinterpret_cast<float*>(work + plan.picked);
     float* const losses = c.losses != nullptr ? c.losses : reinterpret_cast<float*>(work + plan.losses);
     uint16_t* const x = reinterpret_cast<uint16_t*>(work + plan.x);
-    const uint16_t* const weight = plan.in_place ? static_cast<const uint16_t*>(c.weight) : reinterpret_cast<const uint16_t*>(work + plan.weight);
-    const uint32_t w_columns = plan.in_place ? c.d : plan.width, depth = 64 / plan.words;
-    const uint64_t x_row = static_cast<uint64_t>(plan.width) * plan.words, w_row = static_cast<uint64_t>(w_columns) * plan.words;
+    const uint16_t *const given = static_cast<const uint16_t*>(c.weight), *const x_split = reinterpret_cast<const uint16_t*>(work + plan.x_split);
+    const uint32_t depth = 64 / plan.words;
+    const uint64_t x_row = static_cast<uint64_t>(plan.width) * plan.words;
     const auto failed = [](hipError_t& status) { return (status = hipGetLastError()) != hipSuccess; };
     hipError_t status;
 
     const Prepare prepare{c.labels, c.x, c.weight, c.labels_stride, c.ignore, c.x_stride, c.wide_labels, c.n, c.d, plan.width, c.vocab, rows, labels,
                           place, losses, meta, x, reinterpret_cast<uint16_t*>(work + plan.weight), reinterpret_cast<uint16_t*>(work + plan.x_split),
-                          reinterpret_cast<uint32_t*>(work + plan.x_most), reinterpret_cast<uint32_t*>(work + plan.w_most),
+                          reinterpret_cast<uint2*>(work + plan.x_most), reinterpret_cast<uint2*>(work + plan.w_most),
                           ceil_div(padded(c.n, 64), kPrepWaves), plan.in_place ? 0 : ceil_div(c.vocab, kWeightRows)};
     if (c.n > kScanTokens) {
         hipLaunchKernelGGL(loss_scan_kernel, dim3(1), dim3(kScanThreads), 0, stream, prepare);
@@ -1368,45 +1448,76 @@ hipError_t run(const LossCall& c, hipStream_t stream) {
     }
     if (failed(status)) return status;
 
-    Product p{};
-    p.meta = meta;
-    p.labels = labels;
-    p.lse = lse;
-    p.vocab = c.vocab;
-    p.n_pad = plan.n_pad;
-    p.scale = c.scale;
-    p.mean = c.mean;
-    p.out_bf16 = c.value_type == kBF16;
-    p.splits = 1;
-    const uint32_t token_tiles = ceil_div(c.n, plan.token_tile);
-    Product stats = p;
-    stats.a = weight;
-    stats.a_stride = w_row;
-    stats.a_columns = w_columns;
-    stats.b = plan.parts == 3 ? reinterpret_cast<const uint16_t*>(work + plan.x_split) : x;
-    stats.b_stride = plan.parts == 3 ? 3ull * plan.width : x_row;
-    stats.b_columns = plan.width;
-    stats.k_tiles = plan.width / depth;
-    stats.a_tiles = plan.stats_tiles;
-    stats.b_tiles = token_tiles;
-    stats.height = plan.height;
-    stats.a_columns_out = plan.last;
-    stats.picked = picked;
-    stats.slices = reinterpret_cast<float2*>(work + plan.slice_sums);
-    stats.slice_pitch = plan.few ? plan.slices : plan.n_pad;
-    Product keep = stats;
-    keep.a_first = plan.last;
-    keep.a_tiles = plan.keep_tiles;
-    keep.a_columns_out = plan.keeps ? padded(c.vocab - plan.last, kTile) : 0;
-    keep.slice_first = plan.stats_tiles * plan.per_tile;
-    keep.grad = reinterpret_cast<uint16_t*>(work + plan.grad);
-    keep.grad_stride = static_cast<uint64_t>(plan.piece) * plan.words;
-    if (stats.a_tiles != 0 && (status = product<Use::Stats>(plan, stats, stream)) != hipSuccess) return status;
-    if (plan.keeps && (status = product<Use::Keep>(plan, keep, stream)) != hipSuccess) return status;
+    float2* const slice_sums = reinterpret_cast<float2*>(work + plan.slice_sums);
+    const uint32_t kept = plan.keeps ? padded(c.vocab - plan.last, kTile) : 0;
+    const auto of_raw = [&](uint32_t height, Spread only) {  // float32: the weight as it is, x split
+        const uint32_t stats_tiles = ceil_div(plan.last, height), keep_tiles = ceil_div(kept, height), slices = (stats_tiles + keep_tiles) * 4;
+        return Form{3, only, given, x_split, c.d, 2ull * c.d, 3ull * plan.width, kFewTile, height, 4, stats_tiles, keep_tiles, kFewTile, 64,
+                    {slice_sums, slices, slices}};
+    };
+    Form forms[2];
+    uint32_t form_count = 1;
+    if (plan.parts == 3) {
+        forms[0] = of_raw(plan.height, Spread::Any);
+    } else {
+        const uint32_t w_columns = plan.in_place ? c.d : plan.width;
+        forms[0] = {plan.parts, plan.parts == 2 ? Spread::Near : Spread::Any, plan.in_place ? given : reinterpret_cast<const uint16_t*>(work + plan.weight), x,
+                    w_columns, static_cast<uint64_t>(w_columns) * plan.words, x_row, plan.vocab_tile, plan.height, plan.per_tile, plan.stats_tiles,
+                    plan.keep_tiles, plan.few ? kFewTile : kTile, plan.few || plan.parts == 2 ? 128u : 256u,
+                    {slice_sums, plan.slices, plan.few ? plan.slices : plan.n_pad}};
+        if (plan.parts == 2) forms[form_count++] = of_raw(kFewTile, Spread::Wide);
+    }
+    // `what` of every form, until one fails
+    const auto each = [&](auto what) -> hipError_t {
+        for (uint32_t k = 0; k < form_count; ++k)
+            if (hipError_t failure = what(forms[k]); failure != hipSuccess) return failure;
+        return hipSuccess;
+    };
+    const auto begun = [&](const Form& form) {
+        Product p{};
+        p.meta = meta;
+        p.labels = labels;
+        p.lse = lse;
+        p.vocab = c.vocab;
+        p.n_pad = plan.n_pad;
+        p.scale = c.scale;
+        p.mean = c.mean;
+        p.out_bf16 = c.value_type == kBF16;
+        p.splits = 1;
+        p.only = form.only;
+        return p;
+    };
+    // the logits of `rows` vocabulary rows from `first` on
+    const auto logits = [&](const Form& form, uint32_t first, uint32_t rows) {
+        Product p = begun(form);
+        p.a = form.weight;
+        p.a_stride = form.w_row;
+        p.a_columns = form.w_columns;
+        p.a_first = first;
+        p.a_tiles = ceil_div(rows, form.height);
+        p.a_columns_out = rows;
+        p.b = form.x;
+        p.b_stride = form.x_row;
+        p.b_columns = plan.width;
+        p.k_tiles = plan.width / depth;
+        p.height = form.height;
+        p.picked = picked;
+        p.slices = slice_sums;
+        p.slice_pitch = form.slices.pitch;
+        p.slice_first = first == plan.last ? form.stats_tiles * form.per_tile : 0;
+        p.grad = reinterpret_cast<uint16_t*>(work + plan.grad);
+        p.grad_stride = static_cast<uint64_t>(plan.piece) * plan.words;
+        return p;
+    };
+    if (plan.last != 0 && (status = each([&](const Form& form) { return product<Use::Stats>(plan, form, logits(form, 0, plan.last), stream); })) != hipSuccess)
+        return status;
+    if (plan.keeps && (status = each([&](const Form& form) { return product<Use::Keep>(plan, form, logits(form, plan.last, kept), stream); })) != hipSuccess)
+        return status;
+    const Slices none{};
     const auto lse_of = [&](auto tokens) {
         constexpr uint32_t kTokens = decltype(tokens)::value;
-        hipLaunchKernelGGL(loss_lse_kernel<kTokens>, dim3(ceil_div(c.n, kTokens)), dim3(kLseThreads), 0, stream, stats.slices, plan.slices, stats.slice_pitch,
-                           picked, rows, labels, meta, lse, losses);
+        hipLaunchKernelGGL(loss_lse_kernel<kTokens>, dim3(ceil_div(c.n, kTokens)), dim3(kLseThreads), 0, stream, forms[0].slices,
+                           form_count == 2 ? forms[1].slices : none, picked, rows, labels, meta, lse, losses);
     };
     // tokens a block: one where few are all there are, more where that still fills the CUs (runs of 128 bytes of a slice; 8192
     // tokens: 15 us, in fours 46; 512 float32 tokens in fours 10 us, in sixteens 16)
@@ -1416,61 +1527,67 @@ hipError_t run(const LossCall& c, hipStream_t stream) {
     if (failed(status)) return status;
     if (!gradients) return hipSuccess;
 
-    const uint32_t gw_tile = plan.few ? kFewTile : kTile, gw_rows = plan.parts == 3 ? 64 : plan.few || plan.parts == 2 ? 128 : 256;
     for (uint32_t piece = plan.pieces; piece-- > 0;) {
-        const uint32_t first = piece * plan.piece, count = c.vocab - first < plan.piece ? c.vocab - first : plan.piece;
-        Product grad = keep;
+        const uint32_t first = piece * plan.piece, count = c.vocab - first < plan.piece ? c.vocab - first : plan.piece, columns = padded(count, kTile);
+        uint16_t* const grad = reinterpret_cast<uint16_t*>(work + plan.grad);
+        const uint64_t grad_row = static_cast<uint64_t>(plan.piece) * plan.words;
         if (first == plan.last) {
-            const uint32_t columns = padded(count, kTile), across = ceil_div(columns, 8 * kTurnThreads), slice_rows = plan.vocab_tile / plan.per_tile;
-            const float2* slices = stats.slices + static_cast<uint64_t>(keep.slice_first) * (plan.few ? 1 : stats.slice_pitch);
-            const auto turn = [&](auto parts) {
-                constexpr int kParts = decltype(parts)::value;
-                hipLaunchKernelGGL(loss_turn_kernel<kParts>, dim3(across * padded(c.n, 64)), dim3(kTurnThreads), 0, stream, grad.grad, grad.grad_stride,
-                                   first, columns, across, slices, plan.height, plan.per_tile, slice_rows, stats.slice_pitch, lse, labels, meta);
+            const uint32_t across = ceil_div(columns, 8 * kTurnThreads);
+            const auto kept_by = [&](const Form& form) {
+                const uint64_t before = static_cast<uint64_t>(form.stats_tiles) * form.per_tile;
+                return Kept{slice_sums + before * (plan.few || form.parts == 3 ? 1 : form.slices.pitch), form.height, form.per_tile,
+                            form.vocab_tile / form.per_tile, form.slices.pitch};
             };
-            if (plan.parts == 1) turn(std::integral_constant<int, 1>{});
-            else if (plan.parts == 2) turn(std::integral_constant<int, 2>{});
-            else turn(std::integral_constant<int, 3>{});
+            const auto turned = [&](auto parts) {
+                constexpr int kParts = decltype(parts)::value;
+                hipLaunchKernelGGL(loss_turn_kernel<kParts>, dim3(across * padded(c.n, 64)), dim3(kTurnThreads), 0, stream, grad, grad_row, first, columns,
+                                   across, kept_by(forms[0]), kept_by(forms[form_count - 1]), lse, labels, meta);
+            };
+            if (plan.parts == 1) turned(std::integral_constant<int, 1>{});
+            else if (plan.parts == 2) turned(std::integral_constant<int, 2>{});
+            else turned(std::integral_constant<int, 3>{});
             if (failed(status)) return status;
-        } else {
-            grad.a_first = first;
-            grad.a_columns_out = padded(count, kTile);
-            grad.a_tiles = ceil_div(grad.a_columns_out, plan.height);
-            if ((status = product<Use::Grad>(plan, grad, stream)) != hipSuccess) return status;
+        } else if ((status = each([&](const Form& form) { return product<Use::Grad>(plan, form, logits(form, first, columns), stream); })) != hipSuccess) {
+            return status;
         }
 
-        Product gx = p;
-        gx.a = weight + first * w_row;
-        gx.a_stride = w_row;
-        gx.a_columns = w_columns;
-        gx.b = grad.grad;
-        gx.b_stride = grad.grad_stride;
-        gx.b_columns = plan.piece;
-        gx.a_first = first;
-        gx.a_count = plan.width;
-        gx.k_tiles = ceil_div(count, depth);
-        gx.a_tiles = ceil_div(w_columns, plan.vocab_tile);
-        gx.b_tiles = token_tiles;
-        gx.splits = plan.splits;
-        gx.partial = reinterpret_cast<float*>(work + plan.partial);
-        gx.out_stride = plan.width;
-        gx.add = piece + 1 != plan.pieces;
-        if ((status = product<Use::GradX>(plan, gx, stream)) != hipSuccess) return status;
+        status = each([&](const Form& form) {
+            Product gx = begun(form);
+            gx.a = form.weight + first * form.w_row;
+            gx.a_stride = form.w_row;
+            gx.a_columns = form.w_columns;
+            gx.b = grad;
+            gx.b_stride = grad_row;
+            gx.b_columns = plan.piece;
+            gx.a_first = first;
+            gx.a_count = plan.width;
+            gx.k_tiles = ceil_div(count, depth);
+            gx.a_tiles = ceil_div(form.w_columns, form.vocab_tile);
+            gx.splits = plan.splits;
+            gx.partial = reinterpret_cast<float*>(work + plan.partial);
+            gx.out_stride = plan.width;
+            gx.add = piece + 1 != plan.pieces;
+            return product<Use::GradX>(plan, form, gx, stream);
+        });
+        if (status != hipSuccess) return status;
 
-        Product gw = p;
-        gw.a = x;
-        gw.a_stride = x_row;
-        gw.a_columns = plan.width;
-        gw.b = grad.grad;
-        gw.b_stride = grad.grad_stride;
-        gw.b_columns = plan.piece;
-        gw.a_count = c.d;
-        gw.b_count = count;
-        gw.a_tiles = ceil_div(c.d, gw_tile);
-        gw.b_tiles = ceil_div(count, gw_rows);
-        gw.out = static_cast<T*>(c.gw) + static_cast<uint64_t>(first) * c.d;
-        gw.out_stride = c.d;
-        if ((status = product<Use::GradW>(plan, gw, stream)) != hipSuccess) return status;
+        status = each([&](const Form& form) {
+            Product gw = begun(form);
+            gw.a = x;
+            gw.a_stride = x_row;
+            gw.a_columns = plan.width;
+            gw.b = grad;
+            gw.b_stride = grad_row;
+            gw.b_columns = plan.piece;
+            gw.a_count = c.d;
+            gw.b_count = count;
+            gw.a_tiles = ceil_div(c.d, form.gw_tile);
+            gw.b_tiles = ceil_div(count, form.gw_rows);
+            gw.out = static_cast<T*>(c.gw) + static_cast<uint64_t>(first) * c.d;
+            gw.out_stride = c.d;
+            return product<Use::GradW>(plan, form, gw, stream);
+        });
+        if (status != hipSuccess) return status;
     }
     const auto finish = [&](auto ways) {
         constexpr uint32_t kWays = decltype(ways)::value;
