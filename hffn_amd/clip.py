@@ -84,7 +84,8 @@ def clip_grad_norm_(tensors: Iterable[torch.Tensor], max_norm: float, norm_type:
     """``grad_norm`` of the tensors, every entry of which is then scaled by ``min(1, max_norm / (norm + 1e-6))``: in place, or into
     ``out``, a tensor of the same shape and strides for each (float32 or bfloat16). No two tensors may share memory. Returns the
     norm before scaling. An infinite norm makes the entries zero (infinite ones NaN), a NaN one makes all NaN;
-    ``max_norm=inf`` scales nothing while the norm is finite."""
+    ``max_norm=inf`` scales nothing while the norm is finite. Autograd does not record the scaling; it sees that the tensors (or
+    ``out``) were written."""
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm={max_norm} must not be negative")
@@ -99,4 +100,5 @@ def clip_grad_norm_(tensors: Iterable[torch.Tensor], max_norm: float, norm_type:
     work, norm, stream = _buffers(len(tensors), norm_type)
     _lib.check(_lib.load().hffn_clip(len(tensors), _at(pointers), to[0], _at(counts), _at(types), to[1], int(norm_type == math.inf), max_norm,
                                      work.data_ptr(), work.numel(), norm.data_ptr(), stream), "clip")
+    torch.autograd.graph.increment_version(tensors if out is None else into)
     return norm

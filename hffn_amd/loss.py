@@ -26,11 +26,14 @@ _LABEL_BYTES = {torch.int32: 4, torch.int64: 8}
 
 def rows_of(t: torch.Tensor, name: str, width: int, dtype: torch.dtype) -> tuple[torch.Tensor, int]:
     """``t`` as rows of ``width`` entries the kernels read, and their stride: itself where a row's entries are adjacent and rows
-    do not overlap, else a contiguous copy. Raises ``ValueError`` for another shape, type or device."""
+    do not overlap, else a contiguous copy. Raises ``ValueError`` for another shape, type or device, and where autograd would
+    expect the call to be recorded."""
     if t.dim() != 2 or t.dtype != dtype or t.get_device() != 0 or t.shape[1] != width:
         raise ValueError(f"{name}: a {dtype} [N, {width}] tensor on cuda:0 is required, not {t.dtype} {list(t.shape)} on {t.device}")
     if t.shape[0] > MAX_TOKENS:
         raise ValueError(f"{name}: N={t.shape[0]} above {MAX_TOKENS}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires gradients, and autograd does not record this call: pass it detached, or under torch.no_grad()")
     if t.is_contiguous():
         return t, width
     if t.stride(1) == 1 and t.stride(0) >= width:
@@ -41,7 +44,8 @@ def rows_of(t: torch.Tensor, name: str, width: int, dtype: torch.dtype) -> tuple
 class HeadLoss:
     """The loss of one head (see the module docstring). Buffers are the object's own and grow with the calls; what a
     call returns are views of them that the next call overwrites. Calls are queued on PyTorch's current stream; calls of one
-    object on several streams have to be ordered by the caller. A captured graph holds the buffers of its capture: ``reserve``
+    object on several streams have to be ordered by the caller. Autograd records none of them: the gradients are those that
+    ``step`` returns, the weight's too where it requires gradients, and an x that does is refused. A captured graph holds the buffers of its capture: ``reserve``
     the sizes that later calls will have before it, so that none of these replaces them."""
 
     def __init__(self, weight: torch.Tensor, max_tokens: int = 1, ignore_index: int = -100, reduction: str = "mean",

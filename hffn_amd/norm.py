@@ -40,7 +40,8 @@ def _pointer(t: torch.Tensor | None) -> int | None:
 class ResidualNorm:
     """One boundary (see the module docstring). Parameters are float32 [d] tensors, held as given and read at every call; rows are
     float32 or bfloat16 [N, d] with any row stride, all of one type. r, h, gx and gf are new contiguous tensors of that
-    type; sums are taken in float32. Calls are queued on PyTorch's current stream."""
+    type; sums are taken in float32. Calls are queued on PyTorch's current stream. Autograd records none of them: gradients are those
+    of ``backward`` and ``gradients()``, and rows that require gradients are refused."""
 
     def __init__(self, weight: torch.Tensor, bias: torch.Tensor | None = None, *, gate: torch.Tensor | None = None,
                  post_weight: torch.Tensor | None = None, post_bias: torch.Tensor | None = None, scale: float = 1.0,
