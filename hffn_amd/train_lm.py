@@ -31,6 +31,7 @@ from .train_runtime import HFFNTrainRuntime
 
 IGNORE = -100
 _ADAM_ARRAYS = 4  # arrays of one AdamW launch
+_ADAM_ENTRIES = 1 << 30  # of one of them: the library counts in 32 bits
 
 
 class LMTrainer:
@@ -106,9 +107,9 @@ class LMTrainer:
         self.steps += 1
         scalars = (train.lr * train.weight_decay, beta1, 1.0 - beta1, beta2, 1.0 - beta2, train.lr / (1.0 - beta1 ** self.steps),
                    math.sqrt(1.0 - beta2 ** self.steps), train.eps)
-        for first in range(0, len(parameters), _ADAM_ARRAYS):
-            part = slice(first, first + _ADAM_ARRAYS)
-            rows = list(zip(parameters[part], gradients[part], *zip(*self._moments[part])))
+        parts = [part for row in zip(parameters, gradients, *zip(*self._moments)) for part in zip(*(t.view(-1).split(_ADAM_ENTRIES) for t in row))]
+        for first in range(0, len(parts), _ADAM_ARRAYS):
+            rows = parts[first:first + _ADAM_ARRAYS]
             pointers = [(ctypes.c_void_p * len(rows))(*(t.data_ptr() for t in column)) for column in zip(*rows)]
             counts = (ctypes.c_uint32 * len(rows))(*(row[0].numel() for row in rows))
             _lib.check(train._lib.hffn_adamw_arrays(len(rows), *pointers, counts, *scalars, current_stream(self.device)), "AdamW")

@@ -1,0 +1,25 @@
+"""``hffn_amd.train_lm``: parameters that AdamW takes in parts are updated as whole ones are."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from hffn_amd import train_lm
+from hffn_amd.bench_train import make_cell
+from hffn_amd.ffn import hip_layer
+
+pytestmark = pytest.mark.gpu
+
+
+def test_adamw_in_parts(monkeypatch):
+    ids = torch.arange(50, device="cuda")
+
+    def trained():
+        trainer = train_lm.LMTrainer([hip_layer(make_cell("128_256_d020", 5))], 300, 50, seed=2)
+        for _ in range(3):
+            trainer.step(ids, ids + 7)
+        return trainer.parameters()
+
+    whole = trained()
+    monkeypatch.setattr(train_lm, "_ADAM_ENTRIES", 100)
+    assert all(torch.equal(a, b) for a, b in zip(trained(), whole))
