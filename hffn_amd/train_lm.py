@@ -61,7 +61,9 @@ class LMTrainer:
         return [self._embedding_grad, self.head.grad, *(t for b in self.boundaries for t in b.gradients().values())]
 
     def gradients(self) -> list[torch.Tensor]:
-        """Of ``parameters()``, then of every layer."""
+        """Of ``parameters()``, then of every layer, by the last ``backward``. Raises ``RuntimeError`` before the first."""
+        if self.head.grad is None:
+            raise RuntimeError("no gradients before the first backward")
         layers = range(len(self.boundaries) - 1)
         return self._gradients() + [t for i in layers for t in self.train.gradients(i).values()]
 
