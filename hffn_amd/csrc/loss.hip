@@ -6,13 +6,18 @@
 // themselves, where D belongs; the backward turns those into D, computes the other pieces' logits again, and multiplies D
 // by the weight's rows and by x.
 //
-// Every product is out[b][a] = sum_k A[a, k] B[b, k] on 16-bit MFMA operands with float32 sums. bfloat16 calls multiply
-// their entries as they are (D rounded to bfloat16: 2^-8 of an entry, as the gradients themselves are rounded). float32
-// calls hold every operand as fp16 hi + lo of the entry times a power of two of its tensor (22 bits down to 2^-12 of the
-// largest entry, 2^-34 of that below) and take hi hi + hi lo + lo hi; those of a few tokens, which wait for the weight's bytes,
-// read it as it is and split it where it is multiplied into three bfloat16 parts (no power of two to know first), of whose nine
-// products the six down to 2^-16 count. Calls whose entries spread too far for one power of two (kSpread) take the three parts
-// as well: the kernels of both forms are launched, and what the preparing launches saw says which ones do the work.
+// Every product is out[b][a] = sum_k A[a, k] B[b, k] on 16-bit MFMA operands with float32 sums. bfloat16 calls multiply their
+// entries as they are. Many tokens' D is rounded to bfloat16, 2^-8 of an entry as the gradients themselves are: roundings of
+// many entries that do not add up (2048 tokens: the gradients' error is 1.9e-3 of them, 1.7e-3 by their own rounding alone), where
+// two parts would double two products of three. A few tokens' gradients may come from a single entry of D, and their calls wait for
+// the weight and for gw, not for the matrix unit: they hold D in two bfloat16 parts (a step of 1 token of 1024 x 50304 112 us,
+// 106 with one).
+// float32 calls hold every operand as fp16 hi + lo of the entry times a power of two of its tensor (22 bits down to 2^-12 of
+// the largest entry, 2^-34 of that below; D, at most 1, to 2^-38) and take hi hi + hi lo + lo hi. Those of a few tokens read the
+// weight as it is and split it where it is multiplied into three bfloat16 parts (no power of two to know first), of whose nine
+// products the six down to 2^-16 count, and hold D in float32. Calls whose entries spread too far for one power of two (kSpread)
+// take the three parts as well: the kernels of both forms are launched, and what the preparing launches saw says which ones do
+// the work. The parts of an infinity cancel: what it enters is NaN.
 //
 // What bounds it: many tokens, the matrix units and their power. 8192 bfloat16 tokens of 2048 x 50304: five products per half of
 // the vocabulary (844 GFLOP each) of 720 to 850 us, 1.0 to 1.17 PFLOP/s; the forward's over the whole vocabulary takes 1508 us, at
@@ -455,6 +460,7 @@ struct Operand {
     static constexpr uint32_t kRow = TR ? TILE * 2 * kWords : 128, kDepth = 64 / kWords;
     static_assert(kPieces % WAVES == 0, "every wave transfers as many pieces");
     static_assert(GRAIN == 16 || (GRAIN == 4 && RAW), "16-byte transfers, or single float32");
+    static_assert(!TR || RAW || kRow >= 256, "the swizzle stays within a row");
 
     const char* base;        // of the tile at k = 0 (index-major) or of its first column (k-major)
     uint64_t stride;         // bytes of a memory row
@@ -497,19 +503,19 @@ struct Operand {
         if constexpr (GRAIN == 16) dma16(from, at, lds);
         else dma4(from, at, lds);
     }
-    // the tile of k-tile kt into LDS
-    __device__ __forceinline__ void fetch(uint32_t kt, const char* lds) const {
+    // the tile of k-tile kt into LDS, from `shift` bytes on
+    __device__ __forceinline__ void fetch(uint32_t kt, const char* lds, uint64_t shift = 0) const {
         const uint32_t wave = uniform(threadIdx.x / kWave);
         if constexpr (TR) {
             const uint32_t k0 = kt * kDepth;
-            const char* from = base + k0 * stride;
+            const char* from = base + shift + k0 * stride;
 #pragma unroll
             for (uint32_t j = 0; j < kPerWave; ++j) {
                 const uint32_t r = k0 + row[j] <= last ? row[j] : last - k0;  // beyond: the other operand holds zeros
                 transfer(from, r * static_cast<uint32_t>(stride) + offset[j], lds + (wave * kPerWave + j) * kPiece);
             }
         } else {
-            const char* from = base + kt * 128;
+            const char* from = base + shift + kt * 128;
 #pragma unroll
             for (uint32_t j = 0; j < kPerWave; ++j) transfer(from, kt == whole ? offset[j] - back[j] : offset[j], lds + (wave * kPerWave + j) * kPiece);
         }
@@ -666,7 +672,7 @@ struct Product {
     uint32_t slice_pitch;         // slices of many tokens [slice][n_pad]; of a few [n_pad][slice]: n_pad, or the slices there are
     uint32_t slice_first;         // the piece's first
     uint16_t* grad;               // Grad: D, [n_pad][piece]; Keep: the exponentials
-    uint64_t grad_stride;
+    uint64_t grad_stride, grad_low;  // LOW: 16-bit entries from D's first part to its second
     uint32_t n_pad;
     float* partial;               // GradX: [split][n_pad][d]
     bool add;
@@ -677,21 +683,25 @@ struct Product {
     Spread only;                  // the calls that this launch does the work of
 };
 
-// WA x WB waves of TA x TB 32 x 32 results each; k-tiles go through a ring of kStages tile pairs.
-template <int PARTS_, Use USE_, int WA_, int WB_, int TA_, int TB_, uint32_t GRAIN = 16>
+// WA x WB waves of TA x TB 32 x 32 results each; k-tiles go through a ring of kStages tile pairs. LOW: bfloat16 calls that hold D as
+// two bfloat16 parts, its rounding and what that left, a plane each; its products multiply the other operand by both.
+template <int PARTS_, Use USE_, int WA_, int WB_, int TA_, int TB_, uint32_t GRAIN = 16, bool LOW_ = false>
 struct Shape {
     static constexpr int PARTS = PARTS_, WA = WA_, WB = WB_, TA = TA_, TB = TB_;
     static constexpr Use USE = USE_;
+    static constexpr bool LOW = LOW_, kLowB = LOW && (USE == Use::GradX || USE == Use::GradW);
+    static_assert(!LOW || PARTS == 1, "other parts hold D to more bits by themselves");
     static constexpr bool kATr = USE == Use::GradX || USE == Use::GradW, kBTr = USE == Use::GradW;
     static constexpr int kA = WA * TA * 32, kB = WB * TB * 32, kWaves = WA * WB;
     using OpA = Operand<PARTS, kATr, kA, kWaves, GRAIN>;
     // float32 as it is: x's rows come split, D's do not
     static constexpr bool kBSplit = PARTS == 3 && USE != Use::GradX && USE != Use::GradW;
     using OpB = typename std::conditional<kBSplit, SplitOperand<kB, kWaves>, Operand<PARTS, kBTr, kB, kWaves>>::type;
-    static constexpr uint32_t kStage = OpA::kBytes + OpB::kBytes, kTransfers = OpA::kPerWave + OpB::kPerWave;
+    static constexpr uint32_t kPlanes = kLowB ? 2 : 1, kStage = OpA::kBytes + kPlanes * OpB::kBytes;
+    static constexpr uint32_t kTransfers = OpA::kPerWave + kPlanes * OpB::kPerWave;
     static constexpr int kStages = kWaves == 4 ? 81920 / kStage : 163840 / kStage < 4 ? 163840 / kStage : 4;  // 4 waves: two blocks a CU
     static constexpr uint32_t kLds = kStage * kStages;
-    static_assert(kStages >= 2, "two stages at least");
+    static_assert(kStages >= 1, "a stage at least");
 };
 
 // Tiles in groups of kGroup inner ones, a group's outer tiles one after the other: the 32 blocks that an XCD runs at a time
@@ -719,6 +729,7 @@ struct Tile {
     uint32_t k_begin, k_end;
     typename S::OpA a;
     typename S::OpB b;
+    uint64_t low;  // bytes from D's first part to its second
 
     // part `part` (of tiles WHOLE::kA x WHOLE::kB cut into tiles of this shape) of tile `index` of the live_b token tiles;
     // false where it has no results
@@ -736,6 +747,7 @@ struct Tile {
         at.b0 = (kTokensFirst ? tile.inner : tile.outer) * WHOLE::kB + part / kPartsA * S::kB;
         k_begin = 0;
         k_end = p.k_tiles;
+        if constexpr (S::kLowB) low = p.grad_low * 2;
         if constexpr (kTokensFirst) {
             if (at.b0 >= valid) return false;
             a.begin(p.a, p.a_stride, p.a_first + at.a0, min(p.vocab, p.a_first + at.a_end), p.a_columns);
@@ -758,6 +770,7 @@ struct Tile {
         const char* stage = ring + (kt - k_begin) % S::kStages * S::kStage;
         a.fetch(kt, stage);
         b.fetch(kt, stage + S::OpA::kBytes);
+        if constexpr (S::kLowB) b.fetch(kt, stage + S::OpA::kBytes + S::OpB::kBytes, low);
     }
     __device__ __forceinline__ void ahead(const char* ring) const {  // the first k-tiles
         for (uint32_t kt = k_begin; kt < k_end && kt < k_begin + S::kStages; ++kt) fetch(kt, ring);
@@ -804,12 +817,16 @@ __device__ __forceinline__ void accumulate(const Tile<S>& tile, const char* ring
     };
     typename std::conditional<PARTS == 3, Raw, Parts<PARTS>>::type fa[2][TA];
     typename std::conditional<PARTS == 3 && !S::kBSplit, Raw, Parts<PARTS>>::type fb[2][TB];
+    Parts<PARTS> fb_low[2][S::kLowB ? TB : 1];
     const auto read = [&](uint32_t kt, int step, int to) {
         const uint32_t tile_a = lds + (kt - k_begin) % S::kStages * S::kStage, tile_b = tile_a + S::OpA::kBytes;
 #pragma unroll
         for (int i = 0; i < TA; ++i) fa[to][i].template read<typename S::OpA>(tile_a, a_place, i, step);
 #pragma unroll
-        for (int j = 0; j < TB; ++j) fb[to][j].template read<typename S::OpB>(tile_b, b_place, j, step);
+        for (int j = 0; j < TB; ++j) {
+            fb[to][j].template read<typename S::OpB>(tile_b, b_place, j, step);
+            if constexpr (S::kLowB) fb_low[to][j].template read<typename S::OpB>(tile_b + S::OpB::kBytes, b_place, j, step);
+        }
     };
     if (k_end - k_begin >= static_cast<uint32_t>(S::kStages)) meet<kTransfers * (S::kStages - 1)>();
     else meet<0>();
@@ -821,9 +838,11 @@ __device__ __forceinline__ void accumulate(const Tile<S>& tile, const char* ring
             if (step + 1 < kSteps) {
                 read(kt, step + 1, 1 - now);
             } else if (kt + 1 < k_end) {
-                if (k_end - kt >= static_cast<uint32_t>(S::kStages)) meet<kTransfers * (S::kStages - 2)>();
+                constexpr int kLater = S::kStages > 1 ? kTransfers * (S::kStages - 2) : 0;
+                if (k_end - kt >= static_cast<uint32_t>(S::kStages)) meet<kLater>();
                 else meet<0>();
                 if (kt + S::kStages < k_end) tile.fetch(kt + S::kStages, ring);
+                if constexpr (S::kStages == 1) meet<0>();  // the only stage: its transfers have only begun
                 read(kt + 1, 0, 1 - now);
             }
             Parts<PARTS> a[TA], b[TB];
@@ -834,13 +853,15 @@ __device__ __forceinline__ void accumulate(const Tile<S>& tile, const char* ring
 #pragma unroll
             for (int i = 0; i < TA; ++i)
 #pragma unroll
-                for (int j = 0; j < TB; ++j)
+                for (int j = 0; j < TB; ++j) {
+                    if constexpr (S::kLowB) acc(i, j) = multiply<PARTS>(a[i].part[0], fb_low[now][j].part[0], acc(i, j));
 #pragma unroll
                     for (int q = 0; q < PARTS; ++q) {  // the parts' products down to the last part's weight; three parts: the least first
                         const int sum = PARTS == 3 ? PARTS - 1 - q : q;
 #pragma unroll
                         for (int k = 0; k <= sum; ++k) acc(i, j) = multiply<PARTS>(a[i].part[k], b[j].part[sum - k], acc(i, j));
                     }
+                }
         }
         if constexpr (PARTS != 1) {
             if ((kt - k_begin) % kChain == kChain - 1 || kt + 1 == k_end) {
@@ -879,17 +900,17 @@ __device__ __forceinline__ void finish(const Product& p, const Meta& meta, const
         }
     }
     const auto result = [&](int i, int j, int r) -> float { return sums[i][j][r]; };
-    // 16 consecutive entries of a lane into row t of D, from its block i on: 16-bit ones (PARTS 2: hi and lo), or the bits of
-    // 16 float32 (PARTS 3: eight and eight)
+    // 16 consecutive entries of a lane into row t of D, from its block i on: 16-bit ones (PARTS 2: hi and lo; LOW: the two planes'),
+    // or the bits of 16 float32 (PARTS 3: eight and eight)
     const auto store = [&](uint32_t t, int i, const uint32_t (&hi)[8], const uint32_t (&lo)[8]) {
         if (a_lane + i * 32 >= a_end) return;
         uint16_t* to = p.grad + t * p.grad_stride + (a_lane - 16 * half + i * 32) * (PARTS == 1 ? 1 : 2) + (PARTS == 3 ? 32 : 16) * half;
         *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
         *reinterpret_cast<uint4*>(to + 8) = make_uint4(hi[4], hi[5], hi[6], hi[7]);
-        constexpr int kLow = PARTS == 3 ? 16 : 32;
-        if constexpr (PARTS != 1) {
-            *reinterpret_cast<uint4*>(to + kLow) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-            *reinterpret_cast<uint4*>(to + kLow + 8) = make_uint4(lo[4], lo[5], lo[6], lo[7]);
+        if constexpr (PARTS != 1 || S::LOW) {
+            uint16_t* const low = to + (S::LOW ? p.grad_low : PARTS == 3 ? 16 : 32);
+            *reinterpret_cast<uint4*>(low) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            *reinterpret_cast<uint4*>(low + 8) = make_uint4(lo[4], lo[5], lo[6], lo[7]);
         }
     };
     if constexpr (USE == Use::Stats || USE == Use::Keep) {
@@ -976,6 +997,7 @@ __device__ __forceinline__ void finish(const Product& p, const Meta& meta, const
                     }
                     if constexpr (PARTS == 1) {
                         hi[r / 2] = bf16_pair(v[0], v[1]);
+                        if constexpr (S::LOW) lo[r / 2] = bf16_pair(v[0] - __uint_as_float(hi[r / 2] << 16), v[1] - __uint_as_float(hi[r / 2] & 0xffff0000u));
                     } else if constexpr (PARTS == 3) {
                         uint32_t* const to = r < 8 ? hi : lo;
                         to[r % 8] = __float_as_uint(v[0]);
@@ -1058,12 +1080,12 @@ __device__ __forceinline__ void take_part(const Product& p, const Meta& meta, ui
 // or quarters, one a block (1 / 2 or 1 / 4 of the whole shape): 788 tiles of 256 blocks take 3.25 rounds, not 4. bfloat16 tiles
 // are of 8 waves of 128 x 64 results (4 of 128 x 128: the forward's product of 8192 tokens of 2048 1540 -> 1780 us).
 constexpr int kXcds = 8;
-template <int PARTS, Use USE, int WA, int WB, int TA, int TB, uint32_t GRAIN>
+template <int PARTS, Use USE, int WA, int WB, int TA, int TB, uint32_t GRAIN, bool LOW>
 __global__ __launch_bounds__(WA* WB* kWave) __attribute__((amdgpu_waves_per_eu(2, 2))) void loss_product_kernel(Product p) {
     constexpr bool kCut = TA % 2 == 0 && TB % 2 == 0;
-    using Whole = Shape<PARTS, USE, WA, WB, TA, TB, GRAIN>;
-    using Half = Shape<PARTS, USE, WA, WB, TA, kCut ? TB / 2 : TB, GRAIN>;
-    using Quarter = Shape<PARTS, USE, WA, WB, kCut ? TA / 2 : TA, kCut ? TB / 2 : TB, GRAIN>;
+    using Whole = Shape<PARTS, USE, WA, WB, TA, TB, GRAIN, LOW>;
+    using Half = Shape<PARTS, USE, WA, WB, TA, kCut ? TB / 2 : TB, GRAIN, LOW>;
+    using Quarter = Shape<PARTS, USE, WA, WB, kCut ? TA / 2 : TA, kCut ? TB / 2 : TB, GRAIN, LOW>;
     constexpr uint32_t kSlices = kCut ? 2 * WA : WA;
     constexpr uint32_t kLds = Whole::kLds > Quarter::kLds ? (Whole::kLds > Half::kLds ? Whole::kLds : Half::kLds)
                                                           : (Quarter::kLds > Half::kLds ? Quarter::kLds : Half::kLds);
@@ -1302,7 +1324,7 @@ uint32_t padded(uint32_t v, uint32_t to) { return ceil_div(v, to) * to; }
 // 115, 192 151 / 126; of 16384 rows 64 tokens 58 / 62, 128 102 / 64; of 10000 rows 64 tokens 57 / 48. Steps gain less (their
 // products with D split what they read): 64 tokens of 50304 rows 229 / 324 us, 128 362 / 350.
 struct Plan {
-    uint32_t parts, words, n_pad, width, vocab_tile, token_tile, height, per_tile, slices, piece, pieces, last, stats_tiles, keep_tiles, splits;
+    uint32_t parts, words, planes, n_pad, width, vocab_tile, token_tile, height, per_tile, slices, piece, pieces, last, stats_tiles, keep_tiles, splits;
     bool whole, few, in_place, keeps;  // whole: the weight's rows are made of whole 16-byte pieces
     uint64_t meta, rows, labels, place, lse, picked, losses, slice_sums, x_most, w_most, x, x_split, weight, grad, partial, bytes;
 };
@@ -1326,16 +1348,17 @@ Plan plan_of(int vt, uint32_t n, uint32_t d, uint32_t vocab, bool aligned, bool 
     if (gradients) {
         // A tile of D's rows is read by 32-bit byte offsets from its first (Operand::begin), which its last row must not pass; a
         // launch has below 2^32 threads, and loss_turn_kernel's one for 8 entries of D, in whole blocks of a row.
+        p.planes = p.few && p.parts == 1 ? 2 : 1;
         const uint64_t reach = ((1ull << 32) - 256) / (2ull * p.words * (p.token_tile - 1) * kTile);
         const uint64_t turned = (1ull << 32) / (kTile / 8 * static_cast<uint64_t>(p.n_pad)) - 8 * kTurnThreads / kTile;
-        const uint64_t asked = (piece_bytes == 0 ? kLossPieceBytes : piece_bytes) / (2ull * p.words * p.n_pad * kTile);
+        const uint64_t asked = (piece_bytes == 0 ? kLossPieceBytes : piece_bytes) / (2ull * p.words * p.planes * p.n_pad * kTile);
         const uint64_t most = std::min({asked, reach, turned});
         const uint32_t tiles = ceil_div(vocab, kTile), fit = most < 1 ? 1 : most < tiles ? static_cast<uint32_t>(most) : tiles;
         p.piece = ceil_div(tiles, ceil_div(tiles, fit)) * kTile;
         p.pieces = ceil_div(vocab, p.piece);
     }
     // The last piece's exponentials stay where its D belongs. Not those of a few bfloat16 tokens, whose products wait for the
-    // weight and whose gradients may come from a single entry of D: it is rounded once.
+    // weight.
     p.keeps = gradients && !(p.few && p.parts == 1);
     p.last = p.keeps ? (p.pieces - 1) * p.piece : vocab;
     // A few tokens' vocabulary tiles share the rows evenly between the blocks that the CUs hold (50304 rows: 99 or 112 of 128
@@ -1374,17 +1397,17 @@ Plan plan_of(int vt, uint32_t n, uint32_t d, uint32_t vocab, bool aligned, bool 
         const uint32_t blocks = ceil_div(p.width, p.vocab_tile) * (p.n_pad / p.token_tile), k_tiles = p.piece / (64 / p.words);
         const uint32_t fill = ceil_div(p.few ? 2 * kCus : kCus, blocks), limit = k_tiles / 8 < 1 ? 1 : k_tiles / 8;
         p.splits = fill < limit ? fill : limit;
-        p.grad = take(2ull * p.words * p.n_pad * p.piece);
+        p.grad = take(2ull * p.words * p.planes * p.n_pad * p.piece);
         p.partial = take(4ull * p.splits * p.n_pad * p.width);
     }
     p.bytes = at;
     return p;
 }
 
-template <int PARTS, Use USE, int WA, int WB, int TA, int TB, uint32_t GRAIN = 16>
+template <int PARTS, Use USE, int WA, int WB, int TA, int TB, uint32_t GRAIN = 16, bool LOW = false>
 hipError_t launch_product(const Product& p, hipStream_t stream) {
     constexpr uint32_t kBlocks = WA * WB == 4 ? 2 * kCus : kCus;  // as many as the CUs hold
-    hipLaunchKernelGGL((loss_product_kernel<PARTS, USE, WA, WB, TA, TB, GRAIN>), dim3(kBlocks), dim3(WA * WB * kWave), 0, stream, p);
+    hipLaunchKernelGGL((loss_product_kernel<PARTS, USE, WA, WB, TA, TB, GRAIN, LOW>), dim3(kBlocks), dim3(WA * WB * kWave), 0, stream, p);
     return hipGetLastError();
 }
 
@@ -1404,11 +1427,14 @@ hipError_t product(const Plan& plan, const Form& form, const Product& p, hipStre
     if constexpr (USE != Use::GradW)  // which does not read the weight
         if (form.parts == 3 && !plan.whole) return launch_product<3, USE, 4, 1, 1, 2, 4>(p, stream);
     if (form.parts == 3) return launch_product<3, USE, 4, 1, 1, 2>(p, stream);
-    // gw of a few bfloat16 tokens, one k-tile a tile: 128 x 128, two blocks a CU (1 token of 1024 x 50304: a step of 113 us, 107 so)
-    if constexpr (USE == Use::GradW)
-        if (plan.few) return launch_product<1, USE, 4, 1, 1, 4>(p, stream);
-    if constexpr (USE != Use::GradW && USE != Use::Keep)
+    if constexpr (USE == Use::Stats)
         if (plan.few) return launch_product<1, USE, 4, 1, 1, 2>(p, stream);
+    // gw of a few bfloat16 tokens, one k-tile a tile: 128 x 128 in one stage, two blocks a CU (1 token of 1024 x 50304: a step of 112 us,
+    // 123 with 8 waves and one block a CU)
+    if constexpr (USE == Use::GradW)
+        if (plan.few) return launch_product<1, USE, 4, 1, 1, 4, 16, true>(p, stream);
+    if constexpr (USE == Use::Grad || USE == Use::GradX)
+        if (plan.few) return launch_product<1, USE, 4, 1, 1, 2, 16, true>(p, stream);
     return form.parts == 1 ? launch_product<1, USE, 2, 4, 4, 2>(p, stream) : launch_product<2, USE, 4, 2, 2, 2>(p, stream);
 }
 
@@ -1487,6 +1513,7 @@ hipError_t run(const LossCall& c, hipStream_t stream) {
         p.only = form.only;
         return p;
     };
+    const uint64_t grad_row = static_cast<uint64_t>(plan.piece) * plan.words;
     // the logits of `rows` vocabulary rows from `first` on
     const auto logits = [&](const Form& form, uint32_t first, uint32_t rows) {
         Product p = begun(form);
@@ -1506,7 +1533,8 @@ hipError_t run(const LossCall& c, hipStream_t stream) {
         p.slice_pitch = form.slices.pitch;
         p.slice_first = first == plan.last ? form.stats_tiles * form.per_tile : 0;
         p.grad = reinterpret_cast<uint16_t*>(work + plan.grad);
-        p.grad_stride = static_cast<uint64_t>(plan.piece) * plan.words;
+        p.grad_stride = grad_row;
+        p.grad_low = plan.n_pad * grad_row;
         return p;
     };
     if (plan.last != 0 && (status = each([&](const Form& form) { return product<Use::Stats>(plan, form, logits(form, 0, plan.last), stream); })) != hipSuccess)
@@ -1530,7 +1558,6 @@ hipError_t run(const LossCall& c, hipStream_t stream) {
     for (uint32_t piece = plan.pieces; piece-- > 0;) {
         const uint32_t first = piece * plan.piece, count = c.vocab - first < plan.piece ? c.vocab - first : plan.piece, columns = padded(count, kTile);
         uint16_t* const grad = reinterpret_cast<uint16_t*>(work + plan.grad);
-        const uint64_t grad_row = static_cast<uint64_t>(plan.piece) * plan.words;
         if (first == plan.last) {
             const uint32_t across = ceil_div(columns, 8 * kTurnThreads);
             const auto kept_by = [&](const Form& form) {
@@ -1558,6 +1585,7 @@ hipError_t run(const LossCall& c, hipStream_t stream) {
             gx.a_columns = form.w_columns;
             gx.b = grad;
             gx.b_stride = grad_row;
+            gx.grad_low = plan.n_pad * grad_row;
             gx.b_columns = plan.piece;
             gx.a_first = first;
             gx.a_count = plan.width;
@@ -1578,6 +1606,7 @@ hipError_t run(const LossCall& c, hipStream_t stream) {
             gw.a_columns = plan.width;
             gw.b = grad;
             gw.b_stride = grad_row;
+            gw.grad_low = plan.n_pad * grad_row;
             gw.b_columns = plan.piece;
             gw.a_count = c.d;
             gw.b_count = count;

@@ -3,13 +3,19 @@ mean loss with the gradients of the hidden rows and of the head's weight (a trai
 
 For hidden rows ``x [N, d]``, a weight ``[V, d]`` and labels: ``l_t = log sum_v exp(x_t . w_v) - x_t . w_label(t)``; with
 ``p = softmax(x W^T)`` and ``D = (p - onehot) / counted``: ``gx = D W``, ``gw = D^T x``. Logits are computed in pieces of the
-vocabulary and not kept: the sums of exponentials first, then piece by piece the softmax (16 bits an entry,
-float32: 32) and its two products. Tokens whose label is ``ignore_index`` take no part: their losses and rows of ``gx``
+vocabulary and not kept: the sums of exponentials first, then piece by piece the softmax (16 bits an entry, 32 in float32
+and for a few tokens) and its two products. Tokens whose label is ``ignore_index`` take no part: their losses and rows of ``gx``
 are zero whatever their rows of x hold, and the products run over the others alone.
 
     head = HeadLoss(weight, max_tokens=2048)          # weight [V, d] float32 or bfloat16 on the GPU, read at every call
     losses = head.losses(x, labels)                   # float32 [N]
     loss, gx, gw = head.step(x, labels)               # the mean and its gradients; gw is head.grad
+
+Sums are float32 throughout (over tokens and slices of the vocabulary in fixed orders: results repeat bit for bit). bfloat16 steps
+of more than 64 tokens round D to bfloat16 for its two products, which adds about a seventh to the error that the gradients' own
+rounding makes; float32 calls multiply entries of 22 bits or more and keep D to 2^-38, so that a vocabulary row whose probability
+stays below that for every token gets no gradient. Whose gradients need more than bfloat16 steps give passes float32 tensors. An
+infinity in a float32 row makes what it enters NaN.
 """
 from __future__ import annotations
 
@@ -45,15 +51,15 @@ class HeadLoss:
     """The loss of one head (see the module docstring). Buffers are the object's own and grow with the calls; what a
     call returns are views of them that the next call overwrites. Calls are queued on PyTorch's current stream; calls of one
     object on several streams have to be ordered by the caller. Autograd records none of them: the gradients are those that
-    ``step`` returns, the weight's too where it requires gradients, and an x that does is refused. A captured graph holds the buffers of its capture: ``reserve``
-    the sizes that later calls will have before it, so that none of these replaces them."""
+    ``step`` returns, the weight's too where it requires gradients, and an x that does is refused. A captured graph holds the
+    buffers of its capture: ``reserve`` the sizes that later calls will have before it, so that none of these replaces them."""
 
     def __init__(self, weight: torch.Tensor, max_tokens: int = 1, ignore_index: int = -100, reduction: str = "mean",
                  piece_bytes: int = PIECE_BYTES) -> None:
         """``max_tokens``: the calls the buffers are first sized for (``losses``; ``step``'s own come with its first call or
         ``reserve``). ``piece_bytes``: what a piece of the vocabulary's softmax may take in ``step`` (N tokens times its rows, 2
-        bytes an entry in bfloat16, 4 in float32; 256 rows at least, 8.4 million and 2^35 entries at most): the last piece's logits are computed
-        once, the others' twice."""
+        bytes an entry in bfloat16 above 64 tokens, 4 else; 256 rows at least, 8.4 million and 2^35 entries at most): the last
+        piece's logits are computed once, the others' twice."""
         self.device = _device(weight.device)
         if weight.dim() != 2 or not weight.is_contiguous() or weight.numel() == 0:
             raise ValueError(f"weight must be a contiguous, non-empty [V, d] tensor, not {list(weight.shape)}")

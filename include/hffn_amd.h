@@ -437,10 +437,11 @@ int hffn_clip(uint32_t arrays, void* const* p, void* const* out, const uint64_t*
  * hffn_loss_step: *loss, the mean (mean 1; 0 where every token is ignored) or the sum of the counted losses, and the
  * gradients of scale times it: gx [n, d_model] (zero rows for ignored tokens, whatever their x holds) and gw [vocab, d_model],
  * of the value type; a label outside the vocabulary makes all of them NaN. Logits are not kept; the gradients are computed in
- * pieces of the vocabulary whose softmax (16 bits an entry, float32: 32) takes at most piece_bytes (0:
- * HFFN_LOSS_PIECE_BYTES; 256 vocabulary rows at least, 8.4 million and 2^35 entries at most). The last piece's logits are computed once, the
- * others' twice: a larger piece is faster. Workspace: hffn_loss_workspace bytes (aligned: the weight starts on a 16-byte boundary;
- * gradients: for hffn_loss_step with this piece_bytes), any content, 256-byte aligned. Outputs may not overlap inputs. */
+ * pieces of the vocabulary whose softmax (16 bits an entry, float32 and up to 64 tokens: 32) takes at most piece_bytes (0:
+ * HFFN_LOSS_PIECE_BYTES; 256 vocabulary rows at least, 8.4 million and 2^35 entries at most). The last piece's logits are
+ * computed once, the others' twice: a larger piece is faster. Workspace: hffn_loss_workspace bytes (aligned: the weight starts on
+ * a 16-byte boundary; gradients: for hffn_loss_step with this piece_bytes), any content, 256-byte aligned. Outputs may not
+ * overlap inputs. */
 #define HFFN_MAX_VOCAB (1u << 24)
 #define HFFN_LOSS_PIECE_BYTES (512ull << 20)
 int hffn_loss_workspace(int value_type, uint32_t n, uint32_t d_model, uint32_t vocab, int aligned, int gradients, uint64_t piece_bytes,
