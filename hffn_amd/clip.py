@@ -83,8 +83,9 @@ def clip_grad_norm_(tensors: Iterable[torch.Tensor], max_norm: float, norm_type:
                     out: Iterable[torch.Tensor] | None = None) -> torch.Tensor:
     """``grad_norm`` of the tensors, every entry of which is then scaled by ``min(1, max_norm / (norm + 1e-6))``: in place, or into
     ``out``, a tensor of the same shape and strides for each (float32 or bfloat16). No two tensors may share memory. Returns the
-    norm before scaling. An infinite norm makes the entries zero (infinite ones NaN), a NaN one makes all NaN;
-    ``max_norm=inf`` scales nothing while the norm is finite. Autograd does not record the scaling; it sees that the tensors (or
+    norm before scaling; the factor is taken from the float64 norm, so that one beyond float32's range (returned as infinity)
+    scales as any other. Infinite entries become NaN and all others zero, a NaN makes all NaN; ``max_norm=inf`` scales nothing
+    while the entries are finite. Autograd does not record the scaling; it sees that the tensors (or
     ``out``) were written."""
     max_norm = float(max_norm)
     if not max_norm >= 0.0:

@@ -172,8 +172,9 @@ __device__ __forceinline__ void scale_chunk(const T* p, U* out, uint64_t count, 
     for (uint32_t i = before + pieces * V + threadIdx.x; i < all; i += kThreads) put(out + i, factor * widen(p[i]));
 }
 
-// The arrays of one table scaled, last entries first: they were read last and lie in the caches. What goes to other tensors is
-// stored past the caches (331 -> 311 us of the call above). `count` partials are all tables'. In place with a factor of one
+// The arrays of one table scaled, last entries first: they were read last and lie in the caches. float32 entries are stored past the
+// caches (331 -> 311 us of the call above, into other tensors; in place, and with an AdamW step behind, the same time either way:
+// 101 million entries 85 us, 719 with the step). `count` partials are all tables'. In place with a factor of one
 // nothing is written: every entry would be itself.
 template <bool LARGEST>
 __global__ __launch_bounds__(kThreads) void clip_kernel(Table table, const double* __restrict__ partials, uint32_t count, double limit,
