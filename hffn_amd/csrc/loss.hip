@@ -1390,8 +1390,10 @@ Plan plan_of(int vt, uint32_t n, uint32_t d, uint32_t vocab, bool aligned, bool 
         p.w_most = take(sizeof(uint2) * ceil_div(vocab, kWeightRows));
     }
     p.x = take(2ull * p.words * p.n_pad * p.width);
-    p.x_split = p.parts != 1 ? take(6ull * p.n_pad * p.width) : 0;
     p.weight = p.in_place ? 0 : take(2ull * p.words * vocab * p.width);
+    // (packed weights are not read by the form that reads x split, which then may lie in their place)
+    const bool within = p.parts == 2 && 6ull * p.n_pad <= 4ull * vocab;
+    p.x_split = p.parts == 1 ? 0 : within ? p.weight : take(6ull * p.n_pad * p.width);
     if (gradients) {
         // splits of the vocabulary that give every CU a block (few tokens: two), each of 8 k-tiles at least
         const uint32_t blocks = ceil_div(p.width, p.vocab_tile) * (p.n_pad / p.token_tile), k_tiles = p.piece / (64 / p.words);

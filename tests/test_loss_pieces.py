@@ -27,3 +27,11 @@ def test_rows_of_a_piece_lie_within_32_bits(value_type, n, rows):
 def test_a_piece_fits_a_launch(value_type, size, n):
     """A launch of below 2^32 threads turns a piece's exponentials into D, 8 entries a thread."""
     assert loss_bytes(value_type, n, 8, 1 << 20, 1 << 50) <= loss_bytes(value_type, n, 8, 1 << 20, (1 << 35) * size)
+
+
+def test_float32_calls_take_the_packed_weight_and_little_more():
+    """x's three parts lie where the packed weight is not read; where the weight is smaller they have their own place."""
+    lib, n, d, vocab = _lib.load(), 2048, 1024, 50304
+    losses = lambda vocab: _lib.query_bytes(lib.hffn_loss_workspace, F32, n, d, vocab, 1, 0, 0)  # noqa: E731
+    assert losses(vocab) < 4 * d * (vocab + n) + 8 * n * (vocab // 32 + 8) + (1 << 20)
+    assert losses(1000) > 4 * d * (1000 + n) + 6 * d * n
