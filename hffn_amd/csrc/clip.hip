@@ -3,7 +3,7 @@
 // of L2), so that no block waits for another, and scales its share.
 //
 // Bound by memory: 152 million entries in 145 tensors (506 MB; two tables) take 93 us for the norm, 5.4 TB/s, and 217 us scaled into 609 MB
-// of others, 5.1 TB/s, a copy's rate. 36 tensors, 10 MB in all: 5.2 and 3.3 us, less than the host's part of the calls (22 us).
+// of others, 5.1 TB/s, a copy's rate. 36 tensors, 10 MB in all: 5.2 and 3.3 us, less than the host's part of the calls (24 us).
 #include <vector>
 
 #include "common.hpp"

@@ -55,7 +55,7 @@ constexpr int kRoom = 5;       // ... and its largest up to kRoom binades above
 constexpr int kGradLift = 14;  // |D| <= 1 is kept times 2^kGradLift
 // Eight neighbouring entries of a row whose largest lies this many binades below the entry that the tensor's power of two is
 // taken from would keep fewer than 20 bits of that largest: one row of 1e7 times the others cost these 1e-3 in their losses. Three
-// parts in their place: losses of 512 tokens of 512 x 50304 in 225 us, not 158, steps of 1024 x 50304 in 1350, not 720; the
+// parts in their place: losses of 512 tokens of 512 x 50304 in 226 us, not 158, steps of 1024 x 50304 in 1300, not 715; the
 // launches of the form that does not run cost 1 % of either.
 constexpr int kSpread = 14;
 // k-tiles whose products are summed in the MFMA accumulators (float32 calls): of two parts, of three (twice the additions; logits of
@@ -1322,7 +1322,13 @@ uint32_t padded(uint32_t v, uint32_t to) { return ceil_div(v, to) * to; }
 // of 1001 x 50304 in 69 us, packed 164). Losses, width 1024, as it is against packed: 1
 // token of 50304 rows 67 against 161 us, 128 tokens 110 / 159, 192 156 / 195, 256 202 / 202; of 32768 rows 128 tokens 107 /
 // 115, 192 151 / 126; of 16384 rows 64 tokens 58 / 62, 128 102 / 64; of 10000 rows 64 tokens 57 / 48. Steps gain less (their
-// products with D split what they read): 64 tokens of 50304 rows 229 / 324 us, 128 362 / 350.
+// products with D split what they read): 64 tokens of 50304 rows 229 / 324 us, 128 362 / 350. The width moves little: losses of
+// 50304 rows, width 512, 192 tokens 90 / 118, 256 116 / 122, of 16384 rows 64 tokens 37 / 40, 128 60 / 42; width 2048 192 tokens
+// 315 / 371, 256 413 / 376, 64 of 16384 rows 110 / 115, 128 198 / 115; steps of 50304 rows, width 512, 64 tokens 139 / 188, 128
+// 224 / 214, width 2048 440 / 595 and 726 / 652.
+// bfloat16 calls of up to 64 tokens take tiles of 128 x 64, two blocks a CU, instead of 256 x 256 (D in one part on either
+// side): losses of 64 tokens of 50304 rows at widths 512, 1024 and 2048 21 / 29, 31 / 44 and 58 / 78 us, of 96 27 / 29, 42 / 44 and
+// 75 / 77; steps of 64 75 / 87, 116 / 127, 204 / 215. (Of 8192 rows 64 tokens 24 / 20 and 57 / 45: few tiles favour the large ones.)
 struct Plan {
     uint32_t parts, words, planes, n_pad, width, vocab_tile, token_tile, height, per_tile, slices, piece, pieces, last, stats_tiles, keep_tiles, splits;
     bool whole, few, in_place, keeps;  // whole: the weight's rows are made of whole 16-byte pieces

@@ -12,8 +12,8 @@ are zero whatever their rows of x hold, and the products run over the others alo
     loss, gx, gw = head.step(x, labels)               # the mean and its gradients; gw is head.grad
 
 Sums are float32 throughout (over tokens and slices of the vocabulary in fixed orders: results repeat bit for bit). bfloat16 steps
-of more than 64 tokens round D to bfloat16 for its two products, which adds about a seventh to the error that the gradients' own
-rounding makes; float32 calls multiply entries of 22 bits or more and keep D to 2^-38, so that a vocabulary row whose probability
+of more than 64 tokens round D to bfloat16 for its two products, which makes the gradients' error 1.1 to 1.4 times what their own
+rounding makes it (more where three tokens or fewer of them count); float32 calls multiply entries of 22 bits or more and keep D to 2^-38, so that a vocabulary row whose probability
 stays below that for every token gets no gradient. Whose gradients need more than bfloat16 steps give passes float32 tensors. An
 infinity in a float32 row makes what it enters NaN.
 """

@@ -36,7 +36,7 @@ _ADAM_ENTRIES = 1 << 30  # of one of them: the library counts in 32 bits
 
 class LMTrainer:
     """The model above and its step. ``boundaries`` has one more entry than there are layers; the first is a norm alone, the others
-    have a gate, a vector that starts at ``1 / sqrt(layers)``."""
+    have a gate, a vector that starts at ``1 / sqrt(layers)``. Calls of one trainer belong on one stream."""
 
     def __init__(self, layers: list[HFFNLayer], vocab: int, max_tokens: int = 1, max_norm: float = 1.0, lr: float = 1e-3,
                  betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, seed: int = 0) -> None:
