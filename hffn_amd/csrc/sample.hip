@@ -519,8 +519,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleCall a, int bits
 }  // namespace
 
 hipError_t launch_sample(int vt, const SampleCall& a, hipStream_t stream) {
-    int bits = 50;  // a row's weights sum to at most 2^62
-    while (static_cast<uint64_t>(a.vocab) << bits > 1ull << 62) --bits;
+    int bits = 50;  // a row's weights sum to at most 2^62 (vocab 2^bits itself may pass 64 bits)
+    while (a.vocab > (1ull << 62) >> bits) --bits;
     const uint32_t per = vt == kBF16 ? 8 : 4;
     const bool whole = reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 && a.vocab % per == 0 && a.stride % per == 0;
 #define HFFN_SAMPLE(T, WHOLE) hipLaunchKernelGGL((sample_kernel<T, WHOLE>), dim3(a.n), dim3(kThreads), 0, stream, a, bits)
