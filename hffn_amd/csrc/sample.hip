@@ -24,7 +24,9 @@ constexpr uint32_t kTable = 256;
 
 typedef unsigned long long Sum;
 
-// Order-preserving bits of a logit: 0 for minus infinity and NaN, which are never drawn; both zeros the same.
+// Order-preserving bits of a logit: 0 for minus infinity and NaN, which are never drawn; both zeros the same (the key below theirs
+// would be the negative one's: no logit has it, and a float made of it is no smaller than zero).
+constexpr uint32_t kZeroKey = 0x80000000u;
 __device__ __forceinline__ uint32_t order_key(float z) {
     const uint32_t bits = __float_as_uint(z + 0.0f), key = bits ^ (static_cast<uint32_t>(static_cast<int>(bits) >> 31) | 0x80000000u);
     return z > -INFINITY ? key : 0;
@@ -411,7 +413,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleCall a, int bits
     if (min_p > 0.0f) {
         const float enough = weights.lowest(fminf(min_p, 1.0f), temperature, lane);
         if (enough > lowest) {
-            lowest = key_logit<float>(order_key(enough) - 1);
+            const uint32_t key = order_key(enough);
+            lowest = key_logit<float>(key - (key == kZeroKey ? 2 : 1));
             ties = 0;
         }
     }

@@ -26,3 +26,13 @@ def test_flat_rows(vocab, dtype):
     for logits, temperature in ((torch.full((n, vocab), 0.25, dtype=dtype, device="cuda"), 1.0), (untrained, 1.0), (peaked, 1e4), (peaked, math.inf)):
         for settings in (dict(), dict(top_p=0.9), dict(top_k=vocab - 5), dict(top_k=vocab // 2, top_p=0.8, min_p=0.001)):
             check(logits, uniform, temperature, **settings)
+
+
+@pytest.mark.parametrize("dtype", (F32, BF16))
+def test_min_p_at_a_zero(dtype):
+    """The lowest logit of weight enough is a zero, of either sign: at a temperature that parts a zero from the largest negative number."""
+    rows = torch.tensor([[0.0, -1.0, 0.0, -2.0], [-0.0, -1.0, -0.0, -3.0], [-1.0, 0.0, -0.0, -1e-38], [-5.0, -1.0, -1e-30, 0.0]], device="cuda").to(dtype)
+    for u in (0.0, 0.4, 0.6, 0.999):
+        for temperature in (1e-30, 1e-38):
+            for settings in (dict(), dict(top_k=2), dict(top_k=3, top_p=0.9), dict(top_p=0.7)):
+                check(rows, torch.full((4,), u, device="cuda"), temperature, min_p=1.0, **settings)
