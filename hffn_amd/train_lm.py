@@ -162,13 +162,21 @@ class LMTrainer:
 
     @torch.no_grad()
     def generate(self, ids: torch.Tensor, uniform: torch.Tensor, bounds: torch.Tensor | None = None, **settings) -> torch.Tensor:
-        """int64 [K, S]: the tokens that follow each of the S prompts laid end to end in ids [N] (``bounds`` as in ``forward``; no
-        prompt may be empty), drawn with the numbers ``uniform``, float32 [K, S]; ``settings`` are ``sample``'s."""
+        """int64 [K, S]: the tokens that follow each of the S prompts laid end to end in ids [N] (``bounds`` as in ``forward``, all of it in
+        [0, N]; no prompt may be empty), drawn with the numbers ``uniform``, float32 [K, S]; ``settings`` are ``sample``'s."""
+        if bounds is not None and (bounds.dim() != 1 or bounds.shape[0] < 2):
+            raise ValueError(f"bounds: an [S + 1] tensor is required, not {list(bounds.shape)}")
         sequences = 1 if bounds is None else bounds.shape[0] - 1
         if uniform.dim() != 2 or uniform.shape[1] != sequences:
             raise ValueError(f"uniform: a [K, {sequences}] tensor is required, not {list(uniform.shape)}")
-        if ids.shape[0] == 0 or bounds is not None and bool((bounds.diff() <= 0).any()):
+        if ids.shape[0] == 0:
             raise ValueError("an empty prompt")
+        if bounds is not None:
+            empty, begin, end = torch.stack([(bounds[1:] <= bounds[:-1]).any().long(), bounds[0].long(), bounds[-1].long()]).tolist()
+            if empty:
+                raise ValueError("an empty prompt")
+            if begin < 0 or end > ids.shape[0]:
+                raise ValueError(f"bounds: prompts from {begin} to {end} of {ids.shape[0]} tokens")
         ends = torch.tensor([ids.shape[0] - 1], device=self.device) if bounds is None else bounds[1:].long() - 1
         states: list[torch.Tensor] = []
         h = self._walk(self._tokens(ids), self._sequences(bounds, states))[1][-1][ends]
