@@ -55,6 +55,7 @@ class LMTrainer:
         self.train = HFFNTrainRuntime(HFFNRuntime(layers, "cuda"), lr, betas, eps, weight_decay, max_tokens)
         device, d = self.train.runtime.device, self.train.d_model
         self.device, self.max_norm, self.steps = device, float(max_norm), 0
+        self._moments: list[tuple[torch.Tensor, torch.Tensor]] = []
         g = torch.Generator(device).manual_seed(seed)
         self.embedding = torch.randn(vocab, d, generator=g, dtype=torch.float32, device=device)
         self.head = HeadLoss(torch.randn(vocab, d, generator=g, dtype=torch.float32, device=device) / math.sqrt(d), max_tokens, IGNORE)
@@ -67,17 +68,27 @@ class LMTrainer:
             self.gates.append(torch.randn(d, d, generator=g, dtype=torch.float32, device=device) / math.sqrt(d))
             self.mixers.append(GatedRecurrence(torch.linspace(-5.0, 1.0, d, dtype=torch.float32, device=device), mixing))
         self._gate_grads = [torch.empty_like(t) for t in self.gates]
-        self._moments: list[tuple[torch.Tensor, torch.Tensor]] = []
         self._z: torch.Tensor | None = None
 
     @property
     def embedding(self) -> torch.Tensor:
-        """float32 [vocab, d]."""
+        """float32 [vocab, d], contiguous. Another may be assigned (a copy is taken where it is not contiguous): gradients and AdamW's
+        moments stay as they are; one of another vocabulary has no gradients before its first ``backward``, and comes before the first
+        ``step``, which makes the moments."""
         return self._table.weight
 
     @embedding.setter
     def embedding(self, weight: torch.Tensor) -> None:
-        self._table = TokenEmbedding(weight)
+        old = self.__dict__.get("_table")
+        d = self.train.d_model
+        if weight.dim() != 2 or weight.shape[1] != d or weight.dtype != torch.float32:
+            raise ValueError(f"embedding: a float32 [vocab, {d}] tensor is required, not {weight.dtype} {list(weight.shape)}")
+        same = old is not None and weight.shape == old.weight.shape
+        if self._moments and not same:
+            raise ValueError(f"embedding: a vocabulary of {weight.shape[0]} for AdamW's moments of {old.weight.shape[0]}")
+        self._table = TokenEmbedding(weight.detach().contiguous())
+        if same:
+            self._table.grad = old.grad
 
     def parameters(self) -> list[torch.Tensor]:
         """Embedding, head, boundaries, with mixing the gates' matrices and the mixers' biases: what AdamW updates beside the layers."""
@@ -89,8 +100,9 @@ class LMTrainer:
                 *(t for m in self.mixers for t in m.gradients().values())]
 
     def gradients(self) -> list[torch.Tensor]:
-        """Of ``parameters()``, then of every layer, by the last ``backward``. Raises ``RuntimeError`` before the first."""
-        if self.head.grad is None:
+        """Of ``parameters()``, then of every layer, by the last ``backward``. Raises ``RuntimeError`` before the first
+        (of the table that is assigned, where its vocabulary is another)."""
+        if self.head.grad is None or self._table.grad is None:
             raise RuntimeError("no gradients before the first backward")
         layers = range(len(self.boundaries) - 1)
         return self._gradients() + [t for i in layers for t in self.train.gradients(i).values()]
