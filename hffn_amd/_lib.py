@@ -10,7 +10,7 @@ import ctypes
 from pathlib import Path
 
 LIBRARY = Path(__file__).resolve().with_name("libhffn_amd.so")
-ABI_VERSION = 22
+ABI_VERSION = 23
 
 OK = 0
 VALUE_F32, VALUE_BF16 = 0, 1
@@ -60,6 +60,7 @@ SIGNATURES = {
     "hffn_losses": [_I, _P, _U64, _P, _P, _I64, _I, _I64, _P, _P, _U64, _U32, _U32, _U32, _P],
     "hffn_loss_step": [_I, _P, _U64, _P, _P, _I64, _I, _I64, _I, _F32, _U64] + [_P] * 4 + [_U64, _U32, _U32, _U32, _P],
     "hffn_embedding": [_I, _P, _P, _I64, _I, _F32, _P] + [_U32] * 3 + [_P],
+    "hffn_embedding_guarded": [_I, _P, _P, _I64, _I, _F32, _P, _P] + [_U32] * 3 + [_P],
     "hffn_embedding_gradient_workspace": [_I, _U32, _U32, _U32, ctypes.POINTER(_U64)],
     "hffn_embedding_gradient": [_I, _P, _U64, _P, _I64, _I, _I64, _F32, _I, _P, _P, _U64] + [_U32] * 3 + [_P],
     "hffn_scan_workspace": [_U32, _U32, _I, ctypes.POINTER(_U64)],

@@ -1163,6 +1163,12 @@ int check_whole(const void* p, int bytes, const char* name, const char* what) {
     if (reinterpret_cast<uintptr_t>(p) % bytes != 0) return fail(HFFN_ERROR_ARGUMENT, "%s: misaligned %s", what, name);
     return HFFN_OK;
 }
+// Takes HFFN_IDS_FROM_END off id_bytes: what is added to negative ids.
+int64_t from_end(int* id_bytes, uint32_t vocab) {
+    if ((*id_bytes & HFFN_IDS_FROM_END) == 0) return 0;
+    *id_bytes &= ~HFFN_IDS_FROM_END;
+    return vocab;
+}
 int check_room(const void* workspace, uint64_t bytes, uint64_t needed, const char* what) {
     if (!workspace) return fail(HFFN_ERROR_ARGUMENT, "%s: null pointer", what);
     if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return fail(HFFN_ERROR_ARGUMENT, "%s: the workspace must be 16-byte aligned", what);
@@ -1172,15 +1178,22 @@ int check_room(const void* workspace, uint64_t bytes, uint64_t needed, const cha
 }
 }  // namespace
 
-int hffn_embedding(int value_type, const void* weight, const void* ids, int64_t ids_stride, int id_bytes, float scale, void* out, uint32_t d_model,
-                   uint32_t vocab, uint32_t n, void* stream) {
+int hffn_embedding_guarded(int value_type, const void* weight, const void* ids, int64_t ids_stride, int id_bytes, float scale, void* out, uint32_t* outside,
+                           uint32_t d_model, uint32_t vocab, uint32_t n, void* stream) {
     const char* what = "embedding";
     if (int status = check_loss(value_type, n, d_model, vocab, what)) return status;
     if (!weight || !ids || !out) return fail(HFFN_ERROR_ARGUMENT, "%s: null pointer", what);
+    const int64_t end = from_end(&id_bytes, vocab);
     if (int status = check_whole(ids, id_bytes, "ids", what)) return status;
     if (int status = check_entries(value_type, {weight, out}, {}, what)) return status;
-    const hffn::EmbeddingForward call{weight, {ids, ids_stride, id_bytes == 8}, out, scale, n, d_model, vocab};
+    if (reinterpret_cast<uintptr_t>(outside) % 4 != 0) return fail(HFFN_ERROR_ARGUMENT, "%s: misaligned outside", what);
+    const hffn::EmbeddingForward call{weight, {ids, ids_stride, id_bytes == 8, end}, out, outside, scale, n, d_model, vocab};
     return launched(hffn::launch_embedding(value_type, call, static_cast<hipStream_t>(stream)), what);
+}
+
+int hffn_embedding(int value_type, const void* weight, const void* ids, int64_t ids_stride, int id_bytes, float scale, void* out, uint32_t d_model,
+                   uint32_t vocab, uint32_t n, void* stream) {
+    return hffn_embedding_guarded(value_type, weight, ids, ids_stride, id_bytes, scale, out, nullptr, d_model, vocab, n, stream);
 }
 
 int hffn_embedding_gradient_workspace(int value_type, uint32_t n, uint32_t d_model, uint32_t vocab, uint64_t* bytes) {
@@ -1197,10 +1210,11 @@ int hffn_embedding_gradient(int value_type, const void* g, uint64_t g_stride, co
     if (int status = check_loss(value_type, n, d_model, vocab, what)) return status;
     if (!g || !ids || !gw) return fail(HFFN_ERROR_ARGUMENT, "%s: null pointer", what);
     if (g_stride < d_model) return fail(HFFN_ERROR_ARGUMENT, "%s: row stride %llu smaller than d_model=%u", what, static_cast<unsigned long long>(g_stride), d_model);
+    const int64_t end = from_end(&id_bytes, vocab);
     if (int status = check_whole(ids, id_bytes, "ids", what)) return status;
     if (int status = check_entries(value_type, {g, gw}, {}, what)) return status;
     if (int status = check_room(workspace, workspace_bytes, hffn::embedding_workspace_bytes(value_type, n, d_model, vocab), what)) return status;
-    const hffn::EmbeddingGradient call{g, g_stride, {ids, ids_stride, id_bytes == 8}, padding, gw, scale, into != 0, n, d_model, vocab};
+    const hffn::EmbeddingGradient call{g, g_stride, {ids, ids_stride, id_bytes == 8, end}, padding, gw, scale, into != 0, n, d_model, vocab};
     return launched(hffn::launch_embedding_gradient(value_type, call, workspace, static_cast<hipStream_t>(stream)), what);
 }
 

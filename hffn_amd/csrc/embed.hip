@@ -18,7 +18,8 @@ namespace {
 
 __device__ __forceinline__ int64_t id_at(const EmbeddingIds& ids, uint32_t i) {
     const int64_t at = static_cast<int64_t>(i) * ids.stride;
-    return ids.wide ? static_cast<const int64_t*>(ids.p)[at] : static_cast<const int32_t*>(ids.p)[at];
+    const int64_t id = ids.wide ? static_cast<const int64_t*>(ids.p)[at] : static_cast<const int32_t*>(ids.p)[at];
+    return id < 0 ? id + ids.end : id;
 }
 
 // A lane's share of one slice (64 E columns) of a row of d entries: 16 bytes of it, or, where rows start anywhere or end inside
@@ -102,6 +103,7 @@ __global__ __launch_bounds__(kLookupThreads) void lookup_kernel(EmbeddingForward
         } else {
 #pragma unroll
             for (int e = 0; e < L::E; ++e) v[e] = __builtin_nanf("");
+            if (a.outside != nullptr) *a.outside = 1;
         }
         lane.store(static_cast<T*>(a.out) + static_cast<uint64_t>(first + k) * a.d, v);
     }

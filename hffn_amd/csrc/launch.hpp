@@ -297,18 +297,21 @@ uint64_t loss_workspace_bytes(int vt, uint32_t n, uint32_t d, uint32_t vocab, bo
 hipError_t launch_loss(const LossCall& call, hipStream_t stream);
 
 // Embedding lookup and its gradient (embed.hip): ids int32 or (wide) int64, `stride` entries apart; rows of d entries of the
-// value type, weight, out and gw contiguous. out = scale weight[id], NaN for ids outside [0, vocab); gw = scale times the sums of
+// value type, weight, out and gw contiguous. out = scale weight[id], NaN for ids outside [0, vocab), which also set *outside (null: not
+// wanted) to 1; gw = scale times the sums of
 // g's rows by token (into: added to what gw holds), tokens outside [0, vocab) and `padding` left out. Workspace:
 // embedding_workspace_bytes, 16-byte aligned.
 struct EmbeddingIds {
     const void* p;
     int64_t stride;
     bool wide;
+    int64_t end;  // added to negative ones
 };
 struct EmbeddingForward {
     const void* weight;
     EmbeddingIds ids;
     void* out;
+    uint32_t* outside;
     float scale;
     uint32_t n, d, vocab;
 };

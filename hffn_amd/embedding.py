@@ -22,6 +22,7 @@ from .loss import MAX_VOCAB, MAX_WIDTH, rows_of
 from .runtime import MAX_TOKENS, StreamUses, _device, _value_type, current_stream
 
 _ID_BYTES = {torch.int32: 4, torch.int64: 8}
+_FROM_END = 16
 
 
 @functools.lru_cache(maxsize=4096)
@@ -31,7 +32,7 @@ def _gradient_workspace(value_type: int, n: int, d_model: int, vocab: int) -> in
 
 class TokenEmbedding:
     """One table (see the module docstring). Ids are int32 or int64 [N], any stride; one outside [0, V) gives a row of NaN and
-    has no part in the gradient, nor has ``padding_index``. The buffer of ``grad`` is the object's own, made by its first
+    has no part in the gradient, nor has ``padding_index``; with ``from_end`` those from -V on are ids too, as tensors are indexed. The buffer of ``grad`` is the object's own, made by its first
     ``backward`` without ``into`` and overwritten by the next. Calls are queued on PyTorch's current stream; calls of one object
     on several streams have to be ordered by the caller. Autograd records none of them: a g that requires gradients is refused, the
     weight's gradient is the one returned."""
@@ -52,27 +53,31 @@ class TokenEmbedding:
         self._streams = StreamUses()
         self._lib = _lib.load()
 
-    def _ids(self, ids: torch.Tensor) -> tuple:
+    def _ids(self, ids: torch.Tensor, from_end: bool) -> tuple:
         if ids.dim() != 1 or ids.dtype not in _ID_BYTES or ids.get_device() != 0:
             raise ValueError(f"ids: an int32 or int64 [N] tensor on cuda:0 is required, not {ids.dtype} {list(ids.shape)} on {ids.device}")
         n = ids.shape[0]
         if n > MAX_TOKENS:
             raise ValueError(f"ids: N={n} above {MAX_TOKENS}")
-        return n, (ids.data_ptr(), ids.stride(0) if n > 1 else 1, _ID_BYTES[ids.dtype])
+        return n, (ids.data_ptr(), ids.stride(0) if n > 1 else 1, _ID_BYTES[ids.dtype] + (_FROM_END if from_end else 0))
 
-    def forward(self, ids: torch.Tensor) -> torch.Tensor:
-        """The scaled rows of tokens ids [N]: a new [N, d] tensor of the weight's type."""
-        n, args = self._ids(ids)
+    def forward(self, ids: torch.Tensor, *, from_end: bool = False, outside: torch.Tensor | None = None) -> torch.Tensor:
+        """The scaled rows of tokens ids [N]: a new [N, d] tensor of the weight's type. ``outside``, int32 [1] on the device, becomes 1
+        if an id has no row, and is not written else."""
+        n, args = self._ids(ids, from_end)
+        if outside is not None and (outside.dtype != torch.int32 or outside.shape != (1,) or outside.get_device() != 0):
+            raise ValueError(f"outside: an int32 [1] tensor on {self.device} is required, not {outside.dtype} {list(outside.shape)} on {outside.device}")
         out = self.weight.new_empty(n, self.d_model)
         if n:
-            _lib.check(self._lib.hffn_embedding(self.value_type, self.weight.data_ptr(), *args, self.scale, out.data_ptr(), self.d_model, self.vocab, n,
-                                                current_stream(self.device)), "embedding")
+            _lib.check(self._lib.hffn_embedding_guarded(self.value_type, self.weight.data_ptr(), *args, self.scale, out.data_ptr(),
+                                                        None if outside is None else outside.data_ptr(), self.d_model, self.vocab, n,
+                                                        current_stream(self.device)), "embedding")
         return out
 
-    def backward(self, ids: torch.Tensor, g: torch.Tensor, into: torch.Tensor | None = None) -> torch.Tensor:
+    def backward(self, ids: torch.Tensor, g: torch.Tensor, into: torch.Tensor | None = None, *, from_end: bool = False) -> torch.Tensor:
         """The weight's gradient, for g [N, d] of the forward's output, of the weight's type and any row stride: ``self.grad``, or
         ``into``, a contiguous [V, d] tensor of that type that the sums are added to."""
-        n, args = self._ids(ids)
+        n, args = self._ids(ids, from_end)
         g, stride = rows_of(g, "g", self.d_model, self.weight.dtype)
         if g.shape[0] != n:
             raise ValueError(f"g: {g.shape[0]} rows for {n} ids")

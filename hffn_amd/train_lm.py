@@ -46,8 +46,9 @@ _ADAM_ENTRIES = 1 << 30  # of one of them: the library counts in 32 bits
 class LMTrainer:
     """The model above and its step. ``boundaries`` has one more entry than there are layers; the first is a norm alone, the others
     have a gate, a vector that starts at ``1 / sqrt(layers)``. ``mixing`` (a kind of ``GatedRecurrence``; ``None``: tokens know of
-    no others): ``gates`` and ``mixers`` have one entry per layer, the mixers' biases spread over -5 to 1. Calls of one trainer
-    belong on one stream."""
+    no others): ``gates`` and ``mixers`` have one entry per layer, the mixers' biases spread over -5 to 1. Ids count from the
+    table's end where they are negative, as tensors are indexed; of those beyond it ``step`` and ``generate``, and on the host every call, raise
+    ``ValueError``, the other calls give NaN. Calls of one trainer belong on one stream."""
 
     def __init__(self, layers: list[HFFNLayer], vocab: int, max_tokens: int = 1, max_norm: float = 1.0, lr: float = 1e-3,
                  betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, seed: int = 0,
@@ -69,6 +70,9 @@ class LMTrainer:
             self.mixers.append(GatedRecurrence(torch.linspace(-5.0, 1.0, d, dtype=torch.float32, device=device), mixing))
         self._gate_grads = [torch.empty_like(t) for t in self.gates]
         self._z: torch.Tensor | None = None
+        self._outside = torch.zeros(1, dtype=torch.int32, device=device)  # 1: an id had no row
+        self._outside_host = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+        self._looked_up, self._unchecked = torch.cuda.Event(), False
 
     @property
     def embedding(self) -> torch.Tensor:
@@ -108,9 +112,20 @@ class LMTrainer:
         return self._gradients() + [t for i in layers for t in self.train.gradients(i).values()]
 
     def _tokens(self, ids: torch.Tensor) -> torch.Tensor:
-        """Ids as tensors are indexed: on the host too, negative ones from the end."""
-        ids = ids.to(self.device)
-        return torch.where(ids < 0, ids + self.embedding.shape[0], ids)
+        """Ids on the device; those on the host are checked there."""
+        if ids.device.type == "cpu" and ids.numel():
+            low, high = (int(v) for v in ids.aminmax())
+            vocab = self._table.vocab
+            if low < -vocab or high >= vocab:
+                raise ValueError(f"ids from {low} to {high} outside the table's {vocab} rows")
+        return ids.to(self.device)
+
+    def _check_tokens(self) -> None:
+        """Raises ``ValueError`` if an id of the last guarded ``_walk`` had no row. Waits for that lookup alone."""
+        self._looked_up.synchronize()
+        self._unchecked = bool(self._outside_host[0])
+        if self._unchecked:
+            raise ValueError(f"ids outside the table's {self._table.vocab} rows")
 
     def _mixed(self, i: int, h: torch.Tensor, mix) -> tuple[torch.Tensor, torch.Tensor | None]:
         """(what layer i reads, its gates) of hidden rows h; ``mix(i, h, gates)`` runs the mixer."""
@@ -119,9 +134,16 @@ class LMTrainer:
         gates = h @ self.gates[i].T
         return mix(i, h, gates), gates
 
-    def _walk(self, ids: torch.Tensor, mix) -> tuple[list, list, list, list]:
-        """The boundaries' (r, h), first to last, of tokens ids [N], and the layers' inputs and gates."""
-        r, h = self.boundaries[0].forward(self._table.forward(ids))
+    def _walk(self, ids: torch.Tensor, mix, guarded: bool = False, from_end: bool = True) -> tuple[list, list, list, list]:
+        """The boundaries' (r, h), first to last, of tokens ids [N], and the layers' inputs and gates. ``guarded``: ``_check_tokens`` follows."""
+        if guarded and self._unchecked:  # the word may still be that of an earlier call
+            self._outside.zero_()
+        x = self._table.forward(ids, from_end=from_end, outside=self._outside if guarded else None)
+        if guarded:
+            self._unchecked = True
+            self._outside_host.copy_(self._outside, non_blocking=True)
+            self._looked_up.record()
+        r, h = self.boundaries[0].forward(x)
         rs, hs, ms, gates = [r], [h], [], []
         for i, boundary in enumerate(self.boundaries[1:]):
             m, gate = self._mixed(i, h, mix)
@@ -151,13 +173,16 @@ class LMTrainer:
     def backward(self, ids: torch.Tensor, labels: torch.Tensor, bounds: torch.Tensor | None = None) -> torch.Tensor:
         """The mean loss (0-d, a view that the next call overwrites), with all gradients of it computed. A layer runs again with
         its pre-activations kept where its turn comes, so one layer's are in memory at a time."""
+        return self._backward(ids, labels, bounds, False)
+
+    def _backward(self, ids: torch.Tensor, labels: torch.Tensor, bounds: torch.Tensor | None, guarded: bool) -> torch.Tensor:
         ids, n = self._tokens(ids), ids.shape[0]
         if n == 0:
             raise ValueError("no tokens")
         entries = self.train.d_ff * leading_dim(n)
         if self._z is None or self._z.numel() < entries:
             self._z = torch.empty(entries, dtype=torch.float32, device=self.device)
-        rs, hs, ms, gates = self._walk(ids, self._sequences(bounds))
+        rs, hs, ms, gates = self._walk(ids, self._sequences(bounds), guarded)
         loss, gh, _ = self.head.step(hs[-1], labels)
         gr = None
         for i in reversed(range(len(self.boundaries) - 1)):
@@ -169,7 +194,7 @@ class LMTrainer:
                 torch.mm(ggate.T, hs[i], out=self._gate_grads[i])
                 gh = torch.addmm(gx, ggate, self.gates[i])
         gr, _ = self.boundaries[0].backward(rs[0], None, gr, gh)
-        self._table.backward(ids, gr)
+        self._table.backward(ids, gr, from_end=True)
         return loss
 
     @torch.no_grad()
@@ -191,11 +216,12 @@ class LMTrainer:
                 raise ValueError(f"bounds: prompts from {begin} to {end} of {ids.shape[0]} tokens")
         ends = torch.tensor([ids.shape[0] - 1], device=self.device) if bounds is None else bounds[1:].long() - 1
         states: list[torch.Tensor] = []
-        h = self._walk(self._tokens(ids), self._sequences(bounds, states))[1][-1][ends]
+        h = self._walk(self._tokens(ids), self._sequences(bounds, states), guarded=True)[1][-1][ends]
+        self._check_tokens()
         tokens = torch.empty(uniform.shape, dtype=torch.int64, device=self.device)
         for k in range(uniform.shape[0]):
             if k:
-                h = self._walk(tokens[k - 1], lambda i, h, gates: self.mixers[i].step(h, gates, states[i]))[1][-1]
+                h = self._walk(tokens[k - 1], lambda i, h, gates: self.mixers[i].step(h, gates, states[i]), from_end=False)[1][-1]
             tokens[k] = sample(h @ self.head.weight.T, uniform[k], **settings)[0]
         return tokens
 
@@ -217,8 +243,12 @@ class LMTrainer:
             train.adamw(i)
 
     def step(self, ids: torch.Tensor, labels: torch.Tensor, bounds: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
-        """(loss, gradient norm before clipping), both 0-d on the device: gradients, clipping over all of them, AdamW."""
-        loss = self.backward(ids, labels, bounds)
+        """(loss, gradient norm before clipping), both 0-d on the device: gradients, clipping over all of them, AdamW. Ids outside the
+        table raise ``ValueError`` before any parameter is written (but not from a captured graph, which cannot)."""
+        guarded = not torch.cuda.is_current_stream_capturing()
+        loss = self._backward(ids, labels, bounds, guarded)
+        if guarded:
+            self._check_tokens()
         norm = clip_grad_norm_(self.gradients(), self.max_norm)
         self._adamw()
         return loss, norm

@@ -27,7 +27,7 @@
 extern "C" {
 #endif
 
-#define HFFN_ABI_VERSION 22
+#define HFFN_ABI_VERSION 23
 
 #define HFFN_OK 0
 #define HFFN_ERROR_ARGUMENT (-1) /* invalid shape, mode, pointer or workspace */
@@ -454,9 +454,14 @@ int hffn_loss_step(int value_type, const void* x, uint64_t x_stride, const void*
                    void* workspace, uint64_t workspace_bytes, uint32_t d_model, uint32_t vocab, uint32_t n, void* stream);
 
 /* Embedding: out[i] = scale weight[ids[i]] for ids (id_bytes 4 or 8, ids_stride entries apart), weight [vocab, d_model] and
- * out [n, d_model] contiguous, of the value type; an id outside [0, vocab) gives a row of NaN. */
+ * out [n, d_model] contiguous, of the value type; an id outside [0, vocab) gives a row of NaN. With HFFN_IDS_FROM_END added to
+ * id_bytes, here and for the gradient, -vocab to -1 are ids too, of the rows from the table's end. */
+#define HFFN_IDS_FROM_END 16
 int hffn_embedding(int value_type, const void* weight, const void* ids, int64_t ids_stride, int id_bytes, float scale, void* out,
                    uint32_t d_model, uint32_t vocab, uint32_t n, void* stream);
+/* The same, and *outside (a word on the device) becomes 1 if an id has no row; it is not written else. */
+int hffn_embedding_guarded(int value_type, const void* weight, const void* ids, int64_t ids_stride, int id_bytes, float scale, void* out,
+                           uint32_t* outside, uint32_t d_model, uint32_t vocab, uint32_t n, void* stream);
 /* Its gradient: gw[v] = scale times the sum, float32 and in a fixed order, of the rows g[i] (row stride in entries) with
  * ids[i] = v; rows of other tokens zero. into 1: added to what gw holds, other rows left alone. Ids outside [0, vocab) and
  * `padding` (-1: none) take no part. Workspace: hffn_embedding_gradient_workspace bytes, 16-byte aligned, any content. */
