@@ -22,6 +22,12 @@ __device__ __forceinline__ int64_t id_at(const EmbeddingIds& ids, uint32_t i) {
     return id < 0 ? id + ids.end : id;
 }
 
+// The token of position i, ~0 where it has no row (outside the vocabulary, or the padding).
+__device__ __forceinline__ uint32_t token_at(const EmbeddingGradient& a, uint32_t i) {
+    const int64_t id = id_at(a.ids, i);
+    return id >= 0 && id < a.vocab && id != a.padding ? static_cast<uint32_t>(id) : ~0u;
+}
+
 // A lane's share of one slice (64 E columns) of a row of d entries: 16 bytes of it, or, where rows start anywhere or end inside
 // 16 bytes (not WHOLE), E entries 64 columns apart.
 template <typename T, bool WHOLE>
@@ -214,44 +220,122 @@ __device__ __forceinline__ uint32_t first_from(const uint32_t* __restrict__ sort
     return low;
 }
 
-// Zeros in the rows without a position, 64 KB by a block. A row has one if the place that `where` gives, whatever that may be, holds it.
-// Pieces of 16 bytes; one that belongs to several rows goes entry by entry where one of them has a position. Rows within the block's
-// entries are told by a product with 2^32 / d, rounded up: below 2^16 entries and 2^15 a row it is exact.
+// Zeros in the rows without a position, 64 KB by a block, in pieces of 16 bytes; one that belongs to several rows goes entry by entry where
+// one of them has a position. Rows within the block's entries are told by a product with 2^32 / d, rounded up: below 2^16 entries
+// and 2^15 a row it is exact.
+template <typename T>
+struct Fill {
+    static constexpr uint32_t U = 4, E = 16 / sizeof(T), kEntries = U * kSumThreads * E;
+    uint64_t begin;
+    uint32_t first_row, inside, rest, inverse, d;
+    T* gw;
+    bool aligned;
+    __device__ __forceinline__ Fill(const EmbeddingGradient& a, uint32_t block) : begin(static_cast<uint64_t>(block) * kEntries), d(a.d) {
+        const uint64_t entries = static_cast<uint64_t>(a.vocab) * d;
+        first_row = static_cast<uint32_t>(begin / d);
+        inside = static_cast<uint32_t>(begin - static_cast<uint64_t>(first_row) * d);
+        rest = entries - begin < kEntries ? static_cast<uint32_t>(entries - begin) : kEntries;
+        inverse = d == 1 ? 0 : 0xffffffffu / d + 1;
+        gw = static_cast<T*>(a.gw) + begin;
+        aligned = reinterpret_cast<uintptr_t>(a.gw) % 16 == 0;
+    }
+    __device__ __forceinline__ uint32_t row_of(uint32_t entry) const { return first_row + (d == 1 ? entry : __umulhi(inside + entry, inverse)); }
+    __device__ __forceinline__ static uint32_t entry(uint32_t u) { return (u * kSumThreads + threadIdx.x) * E; }
+    __device__ __forceinline__ void rows(uint32_t u, uint32_t& row, uint32_t& next) const {  // of piece u's ends
+        row = row_of(entry(u) < rest ? entry(u) : rest - 1);
+        next = row_of(entry(u) + E - 1 < rest ? entry(u) + E - 1 : rest - 1);
+    }
+    __device__ __forceinline__ bool whole(uint32_t u) const { return aligned && entry(u) + E <= rest; }
+    __device__ __forceinline__ void zero(uint32_t u) const { *reinterpret_cast<uint4*>(gw + entry(u)) = make_uint4(0, 0, 0, 0); }
+    template <typename HAS>
+    __device__ __forceinline__ void zero_without(uint32_t u, HAS&& has) const {
+        for (uint32_t e = 0; e < E && entry(u) + e < rest; ++e)
+            if (!has(row_of(entry(u) + e))) gw[entry(u) + e] = 0;
+    }
+};
+
+// A row has a position if the place that `where` gives, whatever that may be, holds it.
 template <typename T>
 __device__ __forceinline__ void fill_rows(const EmbeddingGradient& a, const uint32_t* __restrict__ sorted, const uint32_t* __restrict__ where, uint32_t block) {
-    constexpr uint32_t U = 4, E = 16 / sizeof(T);
-    const uint64_t begin = static_cast<uint64_t>(block) * U * kSumThreads * E, entries = static_cast<uint64_t>(a.vocab) * a.d;
-    const uint32_t first_row = static_cast<uint32_t>(begin / a.d), inside = static_cast<uint32_t>(begin - static_cast<uint64_t>(first_row) * a.d);
-    const uint32_t rest = entries - begin < U * kSumThreads * E ? static_cast<uint32_t>(entries - begin) : U * kSumThreads * E;
-    const uint32_t inverse = a.d == 1 ? 0 : 0xffffffffu / a.d + 1;
-    const auto row_of = [&](uint32_t entry) { return first_row + (a.d == 1 ? entry : __umulhi(inside + entry, inverse)); };
+    typedef Fill<T> F;
+    const F fill(a, block);
     const auto has = [&](uint32_t row, uint32_t place) { return place < a.n && sorted[place] == row; };
-    T* const gw = static_cast<T*>(a.gw) + begin;
-    const bool aligned = reinterpret_cast<uintptr_t>(a.gw) % 16 == 0;
-    uint32_t row[U], next[U], at[U], at_next[U];
+    uint32_t row[F::U], next[F::U], at[F::U], at_next[F::U];
 #pragma unroll
-    for (uint32_t u = 0; u < U; ++u) {
-        const uint32_t entry = (u * kSumThreads + threadIdx.x) * E;
-        row[u] = row_of(entry < rest ? entry : rest - 1);
-        next[u] = row_of(entry + E - 1 < rest ? entry + E - 1 : rest - 1);
+    for (uint32_t u = 0; u < F::U; ++u) {
+        fill.rows(u, row[u], next[u]);
         at[u] = where[row[u]];
         at_next[u] = next[u] == row[u] ? at[u] : where[next[u]];
     }
-    bool none[U];
+    bool none[F::U];
 #pragma unroll
-    for (uint32_t u = 0; u < U; ++u) none[u] = !has(row[u], at[u]) && (next[u] == row[u] || !has(next[u], at_next[u]));
+    for (uint32_t u = 0; u < F::U; ++u) none[u] = !has(row[u], at[u]) && (next[u] == row[u] || !has(next[u], at_next[u]));
 #pragma unroll
-    for (uint32_t u = 0; u < U; ++u) {
-        const uint32_t entry = (u * kSumThreads + threadIdx.x) * E;
-        if (entry >= rest) break;
-        if (none[u] && next[u] <= row[u] + 1 && aligned && entry + E <= rest) {
-            *reinterpret_cast<uint4*>(gw + entry) = make_uint4(0, 0, 0, 0);
-        } else if (none[u] || next[u] != row[u]) {
-            for (uint32_t e = 0; e < E && entry + e < rest; ++e) {
-                const uint32_t of = row_of(entry + e);
-                if (!has(of, where[of])) gw[entry + e] = 0;
+    for (uint32_t u = 0; u < F::U; ++u) {
+        if (fill.entry(u) >= fill.rest) break;
+        if (none[u] && next[u] <= row[u] + 1 && fill.whole(u)) fill.zero(u);
+        else if (none[u] || next[u] != row[u]) fill.zero_without(u, [&](uint32_t of) { return has(of, where[of]); });
+    }
+}
+
+// The rows in lanes [at, end) of `place` added to acc one after the other; before(j) comes before row j is added.
+template <typename T, bool WHOLE, typename BEFORE>
+__device__ __forceinline__ void walk(const EmbeddingGradient& a, const Lane<T, WHOLE>& column, uint32_t place, uint32_t at, uint32_t end,
+                                     float (&acc)[Lane<T, WHOLE>::E], BEFORE&& before) {
+    typedef Lane<T, WHOLE> L;
+    constexpr int U = WHOLE ? 4 : 16 / L::E;
+    for (uint32_t j = at; j < end; j += U) {
+        typename L::Share share[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (j + u < end) {
+                const uint32_t row = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(place), j + u));
+                column.load(static_cast<const T*>(a.g) + row * a.g_stride, share[u]);
             }
-        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (j + u < end) {
+                before(j + u);
+                float v[L::E];
+                L::widened(share[u], v);
+#pragma unroll
+                for (int e = 0; e < L::E; ++e) acc[e] += v[e];
+            }
+    }
+}
+// A token's sum to its row; acc is zero afterwards.
+template <bool INTO, typename T, bool WHOLE>
+__device__ __forceinline__ void finish(const EmbeddingGradient& a, const Lane<T, WHOLE>& column, uint32_t token, float (&acc)[Lane<T, WHOLE>::E]) {
+    typedef Lane<T, WHOLE> L;
+    T* const row = static_cast<T*>(a.gw) + static_cast<uint64_t>(token) * a.d;
+    if constexpr (INTO) {
+        typename L::Share old;
+        column.load(row, old);
+        float v[L::E];
+        L::widened(old, v);
+#pragma unroll
+        for (int e = 0; e < L::E; ++e) acc[e] = fmaf(a.scale, acc[e], v[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < L::E; ++e) acc[e] *= a.scale;
+    }
+    column.store(row, acc);
+#pragma unroll
+    for (int e = 0; e < L::E; ++e) acc[e] = 0.0f;
+}
+// Every wave's acc, in order, to wave 0's.
+template <int E>
+__device__ __forceinline__ void join_waves(float (&lds)[kSumWaves][E][kWave], uint32_t wave, uint32_t lane, float (&acc)[E]) {
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; ++e) lds[wave][e][lane] = acc[e];
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        acc[e] = 0.0f;
+#pragma unroll 4
+        for (uint32_t v = 0; v < kSumWaves; ++v) acc[e] += lds[v][e][lane];
     }
 }
 
@@ -259,7 +343,7 @@ template <typename T, bool WHOLE, bool INTO>
 __global__ __launch_bounds__(kSumThreads, 8) void sums_kernel(EmbeddingGradient a, const uint32_t* __restrict__ sorted, const uint32_t* __restrict__ places,
                                                               uint32_t window, uint32_t* counters, float* partials, const uint32_t* __restrict__ where, uint32_t slices, uint32_t summers) {
     using L = Lane<T, WHOLE>;
-    constexpr int E = L::E, U = WHOLE ? 4 : 16 / E;
+    constexpr int E = L::E;
     __shared__ float lds[kSumWaves][E][kWave];
     __shared__ uint32_t long_first, long_end, last_piece;
     if constexpr (!INTO)
@@ -270,66 +354,14 @@ __global__ __launch_bounds__(kSumThreads, 8) void sums_kernel(EmbeddingGradient 
     const uint32_t block_at = blockIdx.x / slices, slice = blockIdx.x % slices;
     const uint32_t lane = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave), block = window * kSumWaves, from = block_at * block, begin = from + wave * window;
     const L column(slice, lane, a.d);
-    // the rows of lanes [at, end) of `place` added to acc one after the other; before(j) comes before row j is added
-    const auto walk = [&](uint32_t place, uint32_t at, uint32_t end, float (&acc)[E], auto&& before) {
-        for (uint32_t j = at; j < end; j += U) {
-            typename L::Share share[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (j + u < end) {
-                    const uint32_t row = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(place), j + u));
-                    column.load(static_cast<const T*>(a.g) + row * a.g_stride, share[u]);
-                }
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (j + u < end) {
-                    before(j + u);
-                    float v[E];
-                    L::widened(share[u], v);
-#pragma unroll
-                    for (int e = 0; e < E; ++e) acc[e] += v[e];
-                }
-        }
-    };
     const auto nothing = [](uint32_t) {};
-    const auto finish = [&](uint32_t token, float (&acc)[E]) {
-        T* const row = static_cast<T*>(a.gw) + static_cast<uint64_t>(token) * a.d;
-        if constexpr (INTO) {
-            typename L::Share old;
-            column.load(row, old);
-            float v[E];
-            L::widened(old, v);
-#pragma unroll
-            for (int e = 0; e < E; ++e) acc[e] = fmaf(a.scale, acc[e], v[e]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < E; ++e) acc[e] *= a.scale;
-        }
-        column.store(row, acc);
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-    };
-    // Every wave's acc, in order, to wave 0's.
-    const auto joined = [&](float (&acc)[E]) {
-        __syncthreads();
-#pragma unroll
-        for (int e = 0; e < E; ++e) lds[wave][e][lane] = acc[e];
-        __syncthreads();
-        if (wave != 0) return;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            acc[e] = 0.0f;
-#pragma unroll 4
-            for (uint32_t v = 0; v < kSumWaves; ++v) acc[e] += lds[v][e][lane];
-        }
-    };
     const uint32_t i = begin + lane, key = i < a.n ? sorted[i] : ~0u, before = i > 0 && i <= a.n ? sorted[i - 1] : ~0u, place = i < a.n ? places[i] : 0;
     const uint64_t heads = __ballot(i < a.n && key < a.vocab && (i == 0 || key != before)), mine = heads & ((1ull << window) - 1);
-    const auto token_at = [&](uint32_t at) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(key), at)); };
+    const auto key_at = [&](uint32_t at) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(key), at)); };
     if (threadIdx.x == 0) long_first = ~0u;
     __syncthreads();
     if (mine != 0) {
-        const uint32_t first = __ffsll(static_cast<long long>(mine)) - 1, last = 63 - __clzll(static_cast<long long>(mine)), last_token = token_at(last);
+        const uint32_t first = __ffsll(static_cast<long long>(mine)) - 1, last = 63 - __clzll(static_cast<long long>(mine)), last_token = key_at(last);
         uint32_t end = last + static_cast<uint32_t>(__popcll(__ballot(i < a.n && key == last_token)));  // of the last run, from begin on
         if (end == kWave && begin + kWave < a.n) end = first_from(sorted, begin + kWave, a.n, last_token + 1, lane) - begin;  // it goes on behind the keys at hand
         const bool whole_block = end - last > kRun;
@@ -340,14 +372,14 @@ __global__ __launch_bounds__(kSumThreads, 8) void sums_kernel(EmbeddingGradient 
         const uint32_t stop = whole_block ? last : end;
         if (stop > first) {
             float acc[E] = {};
-            uint32_t token = token_at(first);
-            walk(place, first, stop < kWave ? stop : kWave, acc, [&](uint32_t j) {
+            uint32_t token = key_at(first);
+            walk(a, column, place, first, stop < kWave ? stop : kWave, acc, [&](uint32_t j) {
                 if (j == first || !(mine >> j & 1)) return;
-                finish(token, acc);
-                token = token_at(j);
+                finish<INTO>(a, column, token, acc);
+                token = key_at(j);
             });
-            if (stop > kWave) walk(lane < stop - kWave ? places[begin + kWave + lane] : 0, 0, stop - kWave, acc, nothing);
-            finish(token, acc);
+            if (stop > kWave) walk(a, column, lane < stop - kWave ? places[begin + kWave + lane] : 0, 0, stop - kWave, acc, nothing);
+            finish<INTO>(a, column, token, acc);
         }
     }
     __syncthreads();
@@ -382,8 +414,8 @@ __global__ __launch_bounds__(kSumThreads, 8) void sums_kernel(EmbeddingGradient 
             }
         };
         float acc[E] = {};
-        walk(lane < count ? places[own + lane] : 0, 0, count < kShare ? count : kShare, acc, nothing);
-        joined(acc);
+        walk(a, column, lane < count ? places[own + lane] : 0, 0, count < kShare ? count : kShare, acc, nothing);
+        join_waves(lds, wave, lane, acc);
         if (wave == 0) {
             float* const to = slot((start - head) / kRun);
             // past the caches of this die, and there before the count is: a fence would write back all that they hold, the zeros too
@@ -402,8 +434,98 @@ __global__ __launch_bounds__(kSumThreads, 8) void sums_kernel(EmbeddingGradient 
             const float* const sums = slot(j);
             columns([&](int e, uint32_t c) { acc[e] += __hip_atomic_load(sums + c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); });
         }
-        joined(acc);
-        if (wave == 0) finish(token, acc);
+        join_waves(lds, wave, lane, acc);
+        if (wave == 0) finish<INTO>(a, column, token, acc);
+    }
+}
+
+// A few positions in one launch, without an order: every block has all of their tokens in LDS. A wave takes one position and one slice; if
+// it is its token's first, it adds the rows of that token in their order, and a token of more than 64 positions the whole block, in the
+// pieces above: the same bits as from the order. The blocks that fill look their rows up among the tokens. What that saves is the
+// launch of the order, behind which fill and sums wait.
+constexpr uint32_t kFew = kSumThreads;
+static_assert(kFew / kRun <= kSumWaves, "every piece of a run is a wave's own share");
+template <typename T, bool WHOLE, bool INTO>
+__global__ __launch_bounds__(kSumThreads, 8) void few_kernel(EmbeddingGradient a, uint32_t slices, uint32_t summers) {
+    using L = Lane<T, WHOLE>;
+    constexpr int E = L::E;
+    __shared__ float lds[kSumWaves][E][kWave];
+    __shared__ uint32_t tokens[kFew + 1], list[kFew], long_tokens[kSumWaves], counts[kSumWaves];
+    const uint32_t key = threadIdx.x < a.n ? token_at(a, threadIdx.x) : ~0u;
+    if constexpr (!INTO)
+        if (blockIdx.x >= summers) {
+            typedef Fill<T> F;
+            const F fill(a, blockIdx.x - summers);
+            uint32_t* const bits = tokens;  // of the block's rows: whether one has a position
+            const uint32_t last_row = fill.row_of(fill.rest - 1);
+            for (uint32_t w = threadIdx.x; w <= (last_row - fill.first_row) / 32; w += kSumThreads) bits[w] = 0;
+            __syncthreads();
+            const bool its = key >= fill.first_row && key <= last_row;
+            if (its) atomicOr(bits + (key - fill.first_row) / 32, 1u << (key - fill.first_row) % 32);
+            const bool any = __syncthreads_or(its);
+            const auto has = [&](uint32_t row) { return (bits[(row - fill.first_row) / 32] >> (row - fill.first_row) % 32 & 1) != 0; };
+#pragma unroll
+            for (uint32_t u = 0; u < F::U; ++u) {
+                if (fill.entry(u) >= fill.rest) break;
+                uint32_t row = 0, next = 0;
+                if (any) fill.rows(u, row, next);
+                const bool none = !any || (next <= row + 1 && !has(row) && !has(next));
+                if (none && fill.whole(u)) fill.zero(u);
+                else if (!any || !(next == row && has(row))) fill.zero_without(u, has);
+            }
+            return;
+        }
+    const uint32_t lane = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave), mine = blockIdx.x / slices * kSumWaves + wave;
+    const L column(blockIdx.x % slices, lane, a.d);
+    const auto nothing = [](uint32_t) {};
+    const auto before_me = [&](uint64_t mask) { return static_cast<uint32_t>(__popcll(mask & ((1ull << lane) - 1))); };
+    tokens[threadIdx.x] = key;
+    __syncthreads();
+    const uint32_t token = mine < a.n ? uniform(tokens[mine]) : ~0u;
+    uint32_t count = 0;  // of its positions, if this is the first
+    if (token != ~0u) {
+        uint64_t earlier = 0;
+        for (uint32_t i = lane; i - lane < mine; i += kWave) earlier |= __ballot(i < mine && tokens[i] == token);
+        if (earlier == 0)
+            for (uint32_t i = mine / kWave * kWave + lane; i - lane < a.n; i += kWave) {
+                const uint64_t its = __ballot(tokens[i] == token);
+                const uint32_t to = count + before_me(its);
+                if (its >> lane & 1 && to < kRun) list[wave * kRun + to] = i;
+                count += static_cast<uint32_t>(__popcll(its));
+            }
+    }
+    if (lane == 0) long_tokens[wave] = count > kRun ? token : ~0u;
+    __syncthreads();
+    const uint32_t place = list[wave * kRun + lane], long_token = lane < kSumWaves ? long_tokens[lane] : ~0u;
+    uint64_t long_waves = __ballot(long_token != ~0u);
+    if (count > 0 && count <= kRun) {
+        float acc[E] = {};
+        walk(a, column, place, 0, count, acc, nothing);
+        finish<INTO>(a, column, token, acc);
+    }
+    for (; long_waves != 0; long_waves &= long_waves - 1) {
+        const uint32_t of = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(long_token), __ffsll(static_cast<long long>(long_waves)) - 1));
+        const uint64_t its = __ballot(key == of);
+        if (lane == 0) counts[wave] = static_cast<uint32_t>(__popcll(its));
+        __syncthreads();  // the list was read
+        uint32_t first = 0, all = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < kSumWaves; ++w) {
+            if (w < wave) first += counts[w];
+            all += counts[w];
+        }
+        if (key == of) list[first + before_me(its)] = threadIdx.x;
+        __syncthreads();
+        float sum[E] = {};
+        for (uint32_t piece = 0; piece < all; piece += kRun) {
+            const uint32_t own = piece + wave * kShare, rows = own < all ? (all - own < kShare ? all - own : kShare) : 0;
+            float acc[E] = {};
+            walk(a, column, lane < rows ? list[own + lane] : 0, 0, rows, acc, nothing);
+            join_waves(lds, wave, lane, acc);
+#pragma unroll
+            for (int e = 0; e < E; ++e) sum[e] += acc[e];  // wave 0's is the piece's
+        }
+        if (wave == 0) finish<INTO>(a, column, of, sum);
     }
 }
 
@@ -454,14 +576,26 @@ struct Parts {
     }
 };
 
+template <typename T>
+uint64_t fill_blocks(const EmbeddingGradient& a) { return a.into ? 0 : (static_cast<uint64_t>(a.vocab) * a.d + Fill<T>::kEntries - 1) / Fill<T>::kEntries; }
+
+template <typename T, bool WHOLE>
+hipError_t few(const EmbeddingGradient& a, hipStream_t stream) {
+    constexpr uint32_t slice = Lane<T, WHOLE>::SLICE;
+    const uint32_t slices = (a.d + slice - 1) / slice, summers = (a.n + kSumWaves - 1) / kSumWaves * slices;
+    const dim3 grid(static_cast<uint32_t>(summers + fill_blocks<T>(a)));
+    if (a.into) hipLaunchKernelGGL((few_kernel<T, WHOLE, true>), grid, dim3(kSumThreads), 0, stream, a, slices, summers);
+    else hipLaunchKernelGGL((few_kernel<T, WHOLE, false>), grid, dim3(kSumThreads), 0, stream, a, slices, summers);
+    return hipGetLastError();
+}
+
 template <typename T, bool WHOLE>
 hipError_t sums(const EmbeddingGradient& a, const Parts& parts, char* workspace, const uint32_t* sorted, const uint32_t* places, hipStream_t stream) {
     uint32_t* const counters = reinterpret_cast<uint32_t*>(workspace + parts.counters);
     float* const partials = reinterpret_cast<float*>(workspace + parts.partials);
     const uint32_t* const where = reinterpret_cast<const uint32_t*>(workspace + parts.where);
     const uint32_t summers = parts.blocks * parts.slices;
-    const uint64_t fillers = a.into ? 0 : (static_cast<uint64_t>(a.vocab) * a.d * sizeof(T) + 65535) / 65536;
-    const dim3 grid(static_cast<uint32_t>(summers + fillers));
+    const dim3 grid(static_cast<uint32_t>(summers + fill_blocks<T>(a)));
     if (a.into) hipLaunchKernelGGL((sums_kernel<T, WHOLE, true>), grid, dim3(kSumThreads), 0, stream, a, sorted, places, parts.window, counters, partials, where, parts.slices, summers);
     else hipLaunchKernelGGL((sums_kernel<T, WHOLE, false>), grid, dim3(kSumThreads), 0, stream, a, sorted, places, parts.window, counters, partials, where, parts.slices, summers);
     return hipGetLastError();
@@ -478,6 +612,11 @@ hipError_t launch_embedding(int vt, const EmbeddingForward& a, hipStream_t strea
 }
 
 hipError_t launch_embedding_gradient(int vt, const EmbeddingGradient& a, void* workspace, hipStream_t stream) {
+    const bool whole = whole_rows(vt, a.d, {a.g, a.gw}, a.g_stride);
+    if (a.n <= kFew) {
+        if (vt == kBF16) return whole ? few<uint16_t, true>(a, stream) : few<uint16_t, false>(a, stream);
+        return whole ? few<float, true>(a, stream) : few<float, false>(a, stream);
+    }
     const Parts parts(vt, a.n, a.d, a.vocab);
     char* const base = static_cast<char*>(workspace);
     const auto array = [&](int k) { return reinterpret_cast<uint32_t*>(base + k * parts.one); };
@@ -497,7 +636,6 @@ hipError_t launch_embedding_gradient(int vt, const EmbeddingGradient& a, void* w
         sorted = all;
         places = order;
     }
-    const bool whole = whole_rows(vt, a.d, {a.g, a.gw}, a.g_stride);
     if (vt == kBF16) return whole ? sums<uint16_t, true>(a, parts, base, sorted, places, stream) : sums<uint16_t, false>(a, parts, base, sorted, places, stream);
     return whole ? sums<float, true>(a, parts, base, sorted, places, stream) : sums<float, false>(a, parts, base, sorted, places, stream);
 }
