@@ -219,4 +219,11 @@ __device__ __forceinline__ void dma4(const void* base, uint32_t offset, const vo
                  : "memory", "m0");
 }
 
+// A barrier for what lies in LDS alone: requests to memory stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
 }  // namespace hffn

@@ -4,9 +4,10 @@
 // runs first), then adds every run of equal tokens: no atomics on floats, the same bits at every call.
 //
 // Bound by the writes: a whole gradient of 50304 rows is one fill of the card's memory (206 MB of 2048 bfloat16 columns: 31 us by 16
-// bytes a thread, 6.7 TB/s). Measured, us of the kernels: 8192 tokens into 50304 x 2048 bfloat16 12 + 45 (240
-// MB: 4.2 TB/s), 512 into 50304 x 1024 float32 5 + 36 (5.1), 3001 of 1001 float32 channels into a gradient that is there 6 + 12;
-// the lookup of one token 1.6, a launch.
+// bytes a thread, 6.7 TB/s; stores that pass the caches by are faster where nobody reads the gradient next, 59 -> 53 us for 8192 tokens, and slower with who
+// does: with its norm 79 -> 95). Measured, us of the kernels: 8192 tokens into 50304 x 2048 bfloat16 12 + 45 (240
+// MB: 4.2 TB/s), 512 into 50304 x 1024 float32 33 to 40 in one (5.2 to 6.2), 3001 of 1001 float32 channels into a gradient that is there 6 + 12;
+// the lookup of one token 1.6, a launch; of 8192 tokens of 2048 14 bfloat16 (67 MB: 4.9 TB/s), 24.5 float32 (134 MB: 5.5).
 #include <algorithm>
 #include <type_traits>
 
@@ -442,15 +443,17 @@ __global__ __launch_bounds__(kSumThreads, 8) void sums_kernel(EmbeddingGradient 
 // A few positions in one launch, without an order: every block has all of their tokens in LDS. A wave takes one position and one slice; if
 // it is its token's first, it adds the rows of that token in their order, and a token of more than 64 positions the whole block, in the
 // pieces above: the same bits as from the order. The blocks that fill look their rows up among the tokens. What that saves is the
-// launch of the order, behind which fill and sums wait.
-constexpr uint32_t kFew = kSumThreads;
-static_assert(kFew / kRun <= kSumWaves, "every piece of a run is a wave's own share");
+// launch of the order, behind which fill and sums wait: 512 positions of 1024 float32 into 50304 rows 28.8 us for 34.5 where the caches hold
+// the gradient, 39.8 for 42.9 where they do not; added to a gradient 7.6 for 10.5. One token at all positions is a chain of pieces: 27.9 for 33.3 and 10.5 for
+// 11.8 (512 of 512 into 50304: 21.9 for 22.1), but 36.8 for 34.7 and 18.2 for 12.6 at 1024 positions, which are therefore ordered.
+constexpr uint32_t kFew = 512;
+static_assert(kFew <= kSumThreads && kFew / kRun <= kSumWaves && 8 <= kSumWaves, "a thread a position; every piece of a run is a wave's share; a wave for every entry of a lane");
 template <typename T, bool WHOLE, bool INTO>
-__global__ __launch_bounds__(kSumThreads, 8) void few_kernel(EmbeddingGradient a, uint32_t slices, uint32_t summers) {
+__global__ __launch_bounds__(kSumThreads, INTO ? 4 : 8) void few_kernel(EmbeddingGradient a, uint32_t slices, uint32_t summers) {
     using L = Lane<T, WHOLE>;
     constexpr int E = L::E;
     __shared__ float lds[kSumWaves][E][kWave];
-    __shared__ uint32_t tokens[kFew + 1], list[kFew], long_tokens[kSumWaves], counts[kSumWaves];
+    __shared__ uint32_t tokens[kSumThreads + 1], list[kSumThreads], long_tokens[kSumWaves], counts[kSumWaves];
     const uint32_t key = threadIdx.x < a.n ? token_at(a, threadIdx.x) : ~0u;
     if constexpr (!INTO)
         if (blockIdx.x >= summers) {
@@ -516,16 +519,47 @@ __global__ __launch_bounds__(kSumThreads, 8) void few_kernel(EmbeddingGradient a
         }
         if (key == of) list[first + before_me(its)] = threadIdx.x;
         __syncthreads();
-        float sum[E] = {};
-        for (uint32_t piece = 0; piece < all; piece += kRun) {
-            const uint32_t own = piece + wave * kShare, rows = own < all ? (all - own < kShare ? all - own : kShare) : 0;
-            float acc[E] = {};
-            walk(a, column, lane < rows ? list[own + lane] : 0, 0, rows, acc, nothing);
-            join_waves(lds, wave, lane, acc);
+        // Every wave's rows of a piece are requested before the last piece is joined, of which a wave takes one entry of each lane.
+        typename L::Share share[kShare];
+        const auto request = [&](uint32_t piece) {
+            const uint32_t own = piece + wave * kShare;
 #pragma unroll
-            for (int e = 0; e < E; ++e) sum[e] += acc[e];  // wave 0's is the piece's
+            for (uint32_t r = 0; r < kShare; ++r)
+                if (own + r < all) column.load(static_cast<const T*>(a.g) + uniform(list[own + r]) * a.g_stride, share[r]);
+        };
+        request(0);
+        float sum = 0.0f;
+        for (uint32_t piece = 0; piece < all; piece += kRun) {
+            float acc[E] = {};
+#pragma unroll
+            for (uint32_t r = 0; r < kShare; ++r) {
+                if (piece + wave * kShare + r >= all) break;
+                float v[E];
+                L::widened(share[r], v);
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[e] += v[e];
+            }
+            request(piece + kRun);
+            lds_barrier();
+#pragma unroll
+            for (int e = 0; e < E; ++e) lds[wave][e][lane] = acc[e];
+            lds_barrier();
+            if (wave < E) {
+                float joined = 0.0f;
+#pragma unroll
+                for (uint32_t v = 0; v < kSumWaves; ++v) joined += lds[v][wave][lane];
+                sum += joined;
+            }
         }
-        if (wave == 0) finish<INTO>(a, column, of, sum);
+        lds_barrier();
+        if (wave < E) lds[0][wave][lane] = sum;
+        lds_barrier();
+        if (wave == 0) {
+            float acc[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] = lds[0][e][lane];
+            finish<INTO>(a, column, of, acc);
+        }
     }
 }
 

@@ -264,13 +264,6 @@ struct Place {
     }
 };
 
-// A barrier for what lies in LDS alone: requests to memory stay in flight.
-__device__ __forceinline__ void lds_barrier() {
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-}
-
 // From every wave's step to what enters its rows. The first V waves hold a column a lane: they fold the waves' steps and publish the
 // tile's; every wave then waits for one tile before this in its group of kGroup, the V waves fold these, the last tile of a group
 // publishes the group's, every wave waits for one group before this one (kWaves at a time), and the V waves carry what comes
