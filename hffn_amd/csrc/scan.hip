@@ -31,18 +31,35 @@ __device__ __forceinline__ float passed(float f, float h) { return fmaf(-f, h, i
 __device__ __forceinline__ float passed_and(float f, float h, float v) { return fmaf(-f, h, is_rest(f) ? v : h + v); }  // p h + v
 __device__ __forceinline__ float factor_rest(float f) { return is_rest(f) ? -f : 1.0f - f; }
 
+// An infinity stays one until its sequence ends or meets a NaN or its opposite, however small the p; the forms above make a NaN of it
+// (inf - z inf, 0 inf). Whatever comes out not finite is looked at again: what follows an infinite h is h + v.
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) <= 3.402823466e38f; }
+__device__ __forceinline__ bool infinite(float v) { return fabsf(v) == INFINITY; }
+__device__ __forceinline__ float defined(float f, float h, float v) { return infinite(h) ? h + v : passed_and(f, h, v); }
+template <int V>
+__device__ __forceinline__ bool all_finite(const float (&h)[V]) {
+    bool good = true;
+#pragma unroll
+    for (int v = 0; v < V; ++v) good &= finite(h[v]);
+    return good;
+}
+
 // (f, b): h -> p h + b.
 struct Step {
     float f, b;
 };
-__device__ __forceinline__ float apply(const Step& s, float h) { return s.f == kCut ? s.b : passed(s.f, h) + s.b; }
+template <bool CAREFUL = false>
+__device__ __forceinline__ float apply(const Step& s, float h) {
+    return s.f == kCut ? s.b : CAREFUL && infinite(h) ? h + s.b : passed(s.f, h) + s.b;
+}
+template <bool CAREFUL = false>
 __device__ __forceinline__ Step then(const Step& first, const Step& second) {
     const float q = fmaf(-first.f, second.f, first.f) + second.f;
     const bool whole = !is_rest(first.f) && !is_rest(second.f) && q <= 0.5f;
     const float p = factor_rest(first.f) * factor_rest(second.f);
     Step s;
     s.f = first.f == kCut || second.f == kCut ? kCut : whole ? q : -p;
-    s.b = apply(second, first.b);
+    s.b = apply<CAREFUL>(second, first.b);
     return s;
 }
 
@@ -292,6 +309,11 @@ __device__ __forceinline__ void carry(Carry<V>& lds, const Chain& chain, uint32_
             own = lds.steps[order(0)][wave][lane];
 #pragma unroll
             for (uint32_t w = 1; w < kWaves; ++w) own = then(own, lds.steps[order(w)][wave][lane]);
+            if (!finite(own.b)) {
+                own = lds.steps[order(0)][wave][lane];
+#pragma unroll 1
+                for (uint32_t w = 1; w < kWaves; ++w) own = then<true>(own, lds.steps[order(w)][wave][lane]);
+            }
             if (here) publish(chain.tiles + static_cast<uint64_t>(tile) * d + mine, own);
         }
         const uint32_t reach = uniform(lds.reach < tile ? lds.reach : tile), group = tile / kGroup, in_group = tile % kGroup;
@@ -300,9 +322,17 @@ __device__ __forceinline__ void carry(Carry<V>& lds, const Chain& chain, uint32_
 #pragma unroll
             for (int v = 0; v < V; ++v) lds.before[wave][v][lane] = await(chain.tiles + static_cast<uint64_t>(tile - 1 - wave) * d + column + v);
         lds_barrier();
+        const auto fold = [&](uint32_t count) {  // of `before` to acc
+            const Step behind = acc;
+            for (uint32_t k = 0; k < count; ++k) acc = then(lds.before[k][wave][lane], acc);
+            if (finite(acc.b)) return;
+            acc = behind;
+#pragma unroll 1
+            for (uint32_t k = 0; k < count; ++k) acc = then<true>(lds.before[k][wave][lane], acc);
+        };
         if (folds) {
-            for (uint32_t k = 0; k < tiles; ++k) acc = then(lds.before[k][wave][lane], acc);
-            if (in_group == kGroup - 1 && here) publish(chain.groups + static_cast<uint64_t>(group) * d + mine, then(acc, own));
+            fold(tiles);
+            if (in_group == kGroup - 1 && here) publish(chain.groups + static_cast<uint64_t>(group) * d + mine, then<true>(acc, own));
         }
         for (uint32_t back = 0; back < groups; back += kWaves) {
             lds_barrier();
@@ -310,17 +340,26 @@ __device__ __forceinline__ void carry(Carry<V>& lds, const Chain& chain, uint32_
 #pragma unroll
                 for (int v = 0; v < V; ++v) lds.before[wave][v][lane] = await(chain.groups + static_cast<uint64_t>(group - 1 - back - wave) * d + column + v);
             lds_barrier();
-            if (folds)
-                for (uint32_t k = 0; k < kWaves && k < groups - back; ++k) acc = then(lds.before[k][wave][lane], acc);
+            if (folds) fold(groups - back < kWaves ? groups - back : kWaves);
         }
         if (V > 1) lds_barrier();  // the other folding waves' steps were read
     }
     if (folds) {
         float h = acc.b;
+        bool good = true;
 #pragma unroll
         for (uint32_t w = 0; w < kWaves; ++w) {
             lds.enters[order(w)][wave][lane] = h;
+            good &= finite(h);
             h = apply(lds.steps[order(w)][wave][lane], h);
+        }
+        if (!good) {
+            h = acc.b;
+#pragma unroll 1
+            for (uint32_t w = 0; w < kWaves; ++w) {
+                lds.enters[order(w)][wave][lane] = h;
+                h = apply<true>(lds.steps[order(w)][wave][lane], h);
+            }
         }
     }
     lds_barrier();
@@ -328,9 +367,58 @@ __device__ __forceinline__ void carry(Carry<V>& lds, const Chain& chain, uint32_
 
 // f(true_type) or f(false_type): whether all of a wave's rows lie inside one sequence; that walk has no branches.
 template <int R, typename F>
-__device__ __forceinline__ void by_rows(const Rows<R>& rows, F&& f) {
-    if (rows.plain()) f(std::true_type());
-    else f(std::false_type());
+__device__ __forceinline__ auto by_rows(const Rows<R>& rows, F&& f) {
+    return rows.plain() ? f(std::true_type()) : f(std::false_type());
+}
+
+// The state of the sequence that begins at row t; `s`: the first that begins there or later, moved behind it.
+template <int V>
+__device__ __forceinline__ void begin_at(const ScanForward& a, uint32_t t, uint32_t& s, uint32_t lane, uint32_t from, float (&h)[V]) {
+    if (s + 1 < a.bounds.count && bound_at(a.bounds, a.n, s + 1) <= t) s = first_above(a.bounds, a.n, s + 1, a.bounds.count, t, lane) - 1;
+    if (s >= a.bounds.count) s = a.bounds.count - 1;
+    load_floats<V>(a.state == nullptr ? nullptr : a.state + static_cast<uint64_t>(s) * a.d + from, 0.0f, h);
+    ++s;
+}
+
+// The rows of a wave again, from memory, where values are not finite; `fast` repeats what was stored. A function of its own, called by nearly nobody:
+// inside the kernels its registers would be theirs (bfloat16 backward 59 -> 80 us, by 11 registers in scratch memory).
+template <typename T, int V, int KIND>
+__device__ __attribute__((noinline)) void again(const void* arguments, uint32_t t0, uint32_t column, const float* enters) {
+    using C = Cell<T, V>;
+    constexpr int R = forward_rows(sizeof(T) == 4);
+    const ScanForward a = *static_cast<const ScanForward*>(arguments);
+    const uint32_t lane = __lane_id(), from = column < a.d ? column : 0;
+    t0 = uniform(t0);
+    const Rows<R> rows(a.bounds, a.n, t0, lane, Rows<R>::cache(a.bounds, a.n, lane));
+    float bias[V], fast[V], h[V];
+    load_floats<V>(a.bias == nullptr ? nullptr : a.bias + from, 0.0f, bias);
+#pragma unroll
+    for (int v = 0; v < V; ++v) h[v] = fast[v] = enters[v * kWave + lane];
+    uint32_t s = rows.next;
+#pragma unroll 1
+    for (uint32_t r = 0; r < R; ++r) {
+        const uint32_t t = t0 + r;
+        if (!(rows.live >> r & 1)) continue;
+        if (rows.begins >> r & 1) {
+            begin_at<V>(a, t, s, lane, from, h);
+#pragma unroll
+            for (int v = 0; v < V; ++v) fast[v] = h[v];
+        }
+        const typename C::Raw gate_t = C::load(a.gate, a.gate_stride, t, from), x_t = C::load(a.x, a.x_stride, t, from);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const Gate<sizeof(T) == 4> g(-C::get(gate_t, v) - bias[v]);
+            const float in_t = product(input<KIND>(g), C::get(x_t, v));
+            fast[v] = passed_and(g.f, fast[v], in_t);
+            h[v] = finite(fast[v]) ? fast[v] : defined(g.f, h[v], in_t);
+        }
+        if (column >= a.d || all_finite<V>(fast)) continue;
+        C::store(a.h, t, a.d, column, h);
+        if (!(rows.ends >> r & 1)) continue;
+        const uint64_t at = static_cast<uint64_t>(s > 0 ? s - 1 : 0) * a.d + column;
+#pragma unroll
+        for (int v = 0; v < V; ++v) a.last[at + v] = h[v];
+    }
 }
 
 template <typename T, int V, int KIND>
@@ -368,14 +456,8 @@ __global__ __launch_bounds__(kWaves* kWave, 8) void scan_kernel(ScanForward a, u
             f[r][v] = g.f;
             in[r][v] = product(input<KIND>(g), C::get(x[r], v));
         }
-    // The state of the sequence that begins at row t; `s`: the first that begins there or later, moved behind it.
-    const auto begin = [&](uint32_t t, uint32_t& s, float (&h)[V]) {
-        if (s + 1 < a.bounds.count && bound_at(a.bounds, a.n, s + 1) <= t) s = first_above(a.bounds, a.n, s + 1, a.bounds.count, t, lane) - 1;
-        if (s >= a.bounds.count) s = a.bounds.count - 1;
-        load_floats<V>(a.state == nullptr ? nullptr : a.state + static_cast<uint64_t>(s) * a.d + from, 0.0f, h);
-        ++s;
-    };
-    by_rows(rows, [&](auto plain) {
+    const auto begin = [&](uint32_t t, uint32_t& s, float (&h)[V]) { begin_at<V>(a, t, s, lane, from, h); };
+    bool good = by_rows(rows, [&](auto plain) {
         Summary<V> sum;
         uint32_t s = rows.next;
 #pragma unroll
@@ -392,9 +474,25 @@ __global__ __launch_bounds__(kWaves* kWave, 8) void scan_kernel(ScanForward a, u
         }
 #pragma unroll
         for (int v = 0; v < V; ++v) lds.steps[wave][v][lane] = sum.step(v, rows.begins != 0);
+        return all_finite<V>(sum.b);
     });
+    if (__builtin_expect(__ballot(!good) != 0, 0)) {  // b is what entered last that is not finite, by its sum
+        const int last = 31 - __clz(static_cast<int>(rows.begins));  // the last row where a sequence begins
+        float sum[V] = {};
+        uint32_t s = rows.next;
+        if (last >= 0) begin(t0 + last, s, sum);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (r >= last && rows.live >> r & 1)
+#pragma unroll
+                for (int v = 0; v < V; ++v) sum[v] += in[r][v];
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+            if (!finite(sum[v]) && !finite(lds.steps[wave][v][lane].b)) lds.steps[wave][v][lane].b = sum[v];
+    }
     carry<V>(lds, chain, place.tile, a.d, column, here, lane, wave, [](uint32_t w) { return w; });
     float h[V];
+    good = true;
 #pragma unroll
     for (int v = 0; v < V; ++v) h[v] = lds.enters[wave][v][lane];
     by_rows(rows, [&](auto plain) {
@@ -409,7 +507,10 @@ __global__ __launch_bounds__(kWaves* kWave, 8) void scan_kernel(ScanForward a, u
                     if (here) C::store(a.h, t, a.d, column, none);
                     continue;
                 }
-                if (rows.begins >> r & 1) begin(t, s, h);
+                if (rows.begins >> r & 1) {
+                    good &= all_finite<V>(h);
+                    begin(t, s, h);
+                }
             }
 #pragma unroll
             for (int v = 0; v < V; ++v) h[v] = passed_and(f[r][v], h[v], in[r][v]);
@@ -422,6 +523,8 @@ __global__ __launch_bounds__(kWaves* kWave, 8) void scan_kernel(ScanForward a, u
             }
         }
     });
+    good &= all_finite<V>(h);
+    if (__builtin_expect(__ballot(!good) != 0, 0)) again<T, V, KIND>((const void*)__builtin_amdgcn_kernarg_segment_ptr(), t0, column, &lds.enters[wave][0][0]);
 }
 
 // Before a scan: the workspace's words to all ones, and what leaves sequences without rows is what entered (zero where nothing was
@@ -438,6 +541,101 @@ __global__ __launch_bounds__(kPrepareThreads) void prepare_kernel(Word* words, u
     if (bound_at(bounds, n, s) < bound_at(bounds, n, s + 1)) return;
     for (uint32_t c = threadIdx.x; c < d; c += kPrepareThreads)
         to[static_cast<uint64_t>(s) * d + c] = from == nullptr ? 0.0f : from[static_cast<uint64_t>(s) * d + c];
+}
+
+// The sequence of row t, `s` being at or behind it.
+__device__ __forceinline__ uint32_t sequence_of(const ScanBounds& bounds, uint32_t n, uint32_t t, uint32_t& s, uint32_t lane) {
+    if (s >= bounds.count) s = bounds.count - 1;
+    if (s > 0 && bound_at(bounds, n, s) > t) --s;
+    if (s > 0 && bound_at(bounds, n, s) > t) {
+        s = first_above(bounds, n, 0, s, t, lane);
+        if (s > 0) --s;
+    }
+    return s;
+}
+template <int V>
+__device__ __forceinline__ void end_at(const ScanBackward& a, uint32_t t, uint32_t& s, uint32_t lane, uint32_t from, float (&g)[V]) {
+    const uint64_t at = static_cast<uint64_t>(sequence_of(a.bounds, a.n, t, s, lane)) * a.d + from;
+    load_floats<V>(a.g_last == nullptr ? nullptr : a.g_last + at, 0.0f, g);
+}
+
+// One row: gx and ggate of G, `whole`; h: the state before it. z and c = 1 - z from the factor; z c (dv/dz x - h) is (x - h) z c (tied), -h z c
+// (free) or, with u = 2 - z = 1 + c, (x c root / u - h z) c (normed).
+template <int KIND>
+__device__ __forceinline__ void row_back(float factor, float root, float x_t, float h, float whole, float& gx, float& ggate) {
+    const float c = factor_rest(factor), z = is_rest(factor) ? 1.0f + factor : factor;
+    if constexpr (KIND == kTied) {
+        gx = whole * z;
+        ggate = gx * (x_t - h) * c;
+    } else if constexpr (KIND == kFree) {
+        gx = whole;
+        ggate = whole * -h * z * c;
+    } else {
+        gx = whole * root;
+        ggate = whole * c * fmaf(x_t * c * root, __builtin_amdgcn_rcpf(1.0f + c), -h * z);
+    }
+}
+
+// As `again`; returns the wave's sums of the bias's gradient.
+template <int V>
+struct Columns {
+    float of[V];
+};
+template <typename T, int V, int KIND>
+__device__ __attribute__((noinline)) Columns<V> back_again(const void* arguments, uint32_t t0, uint32_t column, const float* enters) {
+    using C = Cell<T, V>;
+    constexpr int R = kBackRows;
+    const ScanBackward a = *static_cast<const ScanBackward*>(arguments);
+    const uint32_t lane = __lane_id(), from = column < a.d ? column : 0;
+    t0 = uniform(t0);
+    const Rows<R> rows(a.bounds, a.n, t0, lane, Rows<R>::cache(a.bounds, a.n, lane));
+    float bias[V], fast[V], g[V];
+    Columns<V> sums = {};
+    load_floats<V>(a.bias == nullptr ? nullptr : a.bias + from, 0.0f, bias);
+#pragma unroll
+    for (int v = 0; v < V; ++v) g[v] = fast[v] = enters[v * kWave + lane];
+    uint32_t s = rows.behind;
+#pragma unroll 1
+    for (int r = R - 1; r >= 0; --r) {
+        const uint32_t t = t0 + r;
+        if (!(rows.live >> r & 1)) continue;
+        if (rows.ends >> r & 1) {
+            end_at<V>(a, t, s, lane, from, g);
+#pragma unroll
+            for (int v = 0; v < V; ++v) fast[v] = g[v];
+        }
+        const bool begins = rows.begins >> r & 1;
+        const typename C::Raw gate_t = C::load(a.gate, a.gate_stride, t, from), gh_t = C::load(a.gh, a.gh_stride, t, from);
+        const typename C::Raw x_t = C::load(a.x, a.x_stride, t, from), before_t = C::load(a.h, a.h_stride, t == 0 ? 0 : t - 1, from);
+        float h[V], gx[V], ggate[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) h[v] = C::get(before_t, v);
+        if (begins) {
+            sequence_of(a.bounds, a.n, t, s, lane);
+            load_floats<V>(a.state == nullptr ? nullptr : a.state + static_cast<uint64_t>(s) * a.d + from, 0.0f, h);
+        }
+        bool stays = true;  // what was stored
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const Gate<sizeof(T) == 4> at(-C::get(gate_t, v) - bias[v]);
+            const float whole = g[v] + C::get(gh_t, v);
+            row_back<KIND>(at.f, at.root, C::get(x_t, v), h[v], whole, gx[v], ggate[v]);
+            sums.of[v] += ggate[v];
+            stays &= finite(fast[v]);
+            fast[v] = passed(at.f, fast[v] + C::get(gh_t, v));
+            stays &= !begins || finite(fast[v]);
+            g[v] = finite(fast[v]) ? fast[v] : defined(at.f, whole, 0.0f);
+        }
+        if (column >= a.d || stays) continue;
+        if (begins && a.g_state != nullptr) {
+            const uint64_t at = static_cast<uint64_t>(s) * a.d + column;
+#pragma unroll
+            for (int v = 0; v < V; ++v) a.g_state[at + v] = g[v];
+        }
+        C::store(a.gx, t, a.d, column, gx);
+        C::store(a.g_gate, t, a.d, column, ggate);
+    }
+    return sums;
 }
 
 template <typename T, int V, int KIND>
@@ -479,21 +677,9 @@ __global__ __launch_bounds__(kWaves* kWave, 8) void scan_back_kernel(ScanBackwar
     for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int v = 0; v < V; ++v) f[r][v] = gate_of(r, v).f;
-    // The sequence of row t, `s` being at or behind it.
-    const auto sequence = [&](uint32_t t, uint32_t& s) {
-        if (s >= a.bounds.count) s = a.bounds.count - 1;
-        if (s > 0 && bound_at(a.bounds, a.n, s) > t) --s;
-        if (s > 0 && bound_at(a.bounds, a.n, s) > t) {
-            s = first_above(a.bounds, a.n, 0, s, t, lane);
-            if (s > 0) --s;
-        }
-        return s;
-    };
-    const auto end = [&](uint32_t t, uint32_t& s, float (&g)[V]) {
-        const uint64_t at = static_cast<uint64_t>(sequence(t, s)) * a.d + from;
-        load_floats<V>(a.g_last == nullptr ? nullptr : a.g_last + at, 0.0f, g);
-    };
-    by_rows(rows, [&](auto plain) {
+    const auto sequence = [&](uint32_t t, uint32_t& s) { return sequence_of(a.bounds, a.n, t, s, lane); };
+    const auto end = [&](uint32_t t, uint32_t& s, float (&g)[V]) { end_at<V>(a, t, s, lane, from, g); };
+    const bool good = by_rows(rows, [&](auto plain) {
         Summary<V> sum;
         uint32_t s = rows.behind;
 #pragma unroll
@@ -510,7 +696,22 @@ __global__ __launch_bounds__(kWaves* kWave, 8) void scan_back_kernel(ScanBackwar
         }
 #pragma unroll
         for (int v = 0; v < V; ++v) lds.steps[wave][v][lane] = sum.step(v, rows.ends != 0);
+        return all_finite<V>(sum.b);
     });
+    if (__builtin_expect(__ballot(!good) != 0, 0)) {  // as in the forward
+        const int first = __ffs(static_cast<int>(rows.ends)) - 1;  // the first row where a sequence ends
+        float sum[V] = {};
+        uint32_t s = rows.behind;
+        if (first >= 0) end(t0 + first, s, sum);
+#pragma unroll
+        for (int r = R - 1; r >= 0; --r)
+            if ((first < 0 || r <= first) && rows.live >> r & 1)
+#pragma unroll
+                for (int v = 0; v < V; ++v) sum[v] += C::get(gh[r], v);
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+            if (!finite(sum[v]) && !finite(lds.steps[wave][v][lane].b)) lds.steps[wave][v][lane].b = sum[v];
+    }
     carry<V>(lds, chain, place.tile, a.d, column, here, lane, wave, [](uint32_t w) { return kWaves - 1 - w; });
     float g[V], g_bias[V] = {};
 #pragma unroll
@@ -538,8 +739,6 @@ __global__ __launch_bounds__(kWaves* kWave, 8) void scan_back_kernel(ScanBackwar
             if (live)
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    // z and c = 1 - z from the factor; z c (dv/dz x - h) is (x - h) z c (tied), -h z c (free) or, with u = 2 - z = 1 + c,
-                    // (x c root / u - h z) c (normed)
                     float factor, root = 1.0f;
                     if constexpr (KIND == kNormed) {
                         if (v == 0) asm volatile("" : "+v"(gate[r]));  // or the compiler keeps the first walk's values, in scratch memory
@@ -549,18 +748,8 @@ __global__ __launch_bounds__(kWaves* kWave, 8) void scan_back_kernel(ScanBackwar
                     } else {
                         factor = f[r][v];
                     }
-                    const float x_t = C::get(x[r], v), c = factor_rest(factor), z = is_rest(factor) ? 1.0f + factor : factor;
                     const float whole = g[v] + C::get(gh[r], v);
-                    if constexpr (KIND == kTied) {
-                        gx[v] = whole * z;
-                        ggate[v] = gx[v] * (x_t - h[v]) * c;
-                    } else if constexpr (KIND == kFree) {
-                        gx[v] = whole;
-                        ggate[v] = whole * -h[v] * z * c;
-                    } else {
-                        gx[v] = whole * root;
-                        ggate[v] = whole * c * fmaf(x_t * c * root, __builtin_amdgcn_rcpf(1.0f + c), -h[v] * z);
-                    }
+                    row_back<KIND>(factor, root, C::get(x[r], v), h[v], whole, gx[v], ggate[v]);
                     g_bias[v] += ggate[v];
                     g[v] = passed(factor, whole);
                 }
@@ -574,6 +763,12 @@ __global__ __launch_bounds__(kWaves* kWave, 8) void scan_back_kernel(ScanBackwar
             C::store(a.g_gate, t, a.d, column, ggate);
         }
     });
+    if (__builtin_expect(__ballot(!all_finite<V>(g_bias)) != 0, 0)) {  // as G times anything is where G is not
+        const Columns<V> sums = back_again<T, V, KIND>((const void*)__builtin_amdgcn_kernarg_segment_ptr(), t0, column, &lds.enters[wave][0][0]);
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+            if (!finite(g_bias[v])) g_bias[v] = sums.of[v];
+    }
     __syncthreads();  // what enters was read
 #pragma unroll
     for (int v = 0; v < V; ++v) lds.enters[wave][v][lane] = g_bias[v];
@@ -613,7 +808,7 @@ __global__ __launch_bounds__(256) void step_kernel(ScanStep a) {
     const float x = widen(static_cast<const T*>(a.x)[row * a.x_stride + column]);
     const Gate<sizeof(T) == 4> g(-widen(static_cast<const T*>(a.gate)[row * a.gate_stride + column]) - (a.bias == nullptr ? 0.0f : a.bias[column]));
     float* const state = a.state + row * a.state_stride + column;
-    const float h = passed_and(g.f, *state, product(input<KIND>(g), x));
+    const float h = defined(g.f, *state, product(input<KIND>(g), x));
     *state = h;
     T* const out = static_cast<T*>(a.h) + static_cast<uint64_t>(row) * a.d + column;
     if constexpr (sizeof(T) == 4) *out = h;

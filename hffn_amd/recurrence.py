@@ -13,7 +13,8 @@ variance keep it) or ``x`` itself (``"free"``).
 
 ``bounds`` [S + 1] tells where each sequence begins, and where the last one ends; without it the rows are one sequence.
 States are float32, and 1 - z is never rounded to a float by itself, so that channels that forget a millionth per token do
-not drift. The backward takes h as the forward gave it; nothing is kept between the calls.
+not drift. An infinity stays one for the rest of its sequence, however little of it is kept, until a NaN or its opposite comes in; so does
+what leaves float32 on the way, for which h + v may be enough (z up to a half takes h + v first), or a tile's inputs alone. The backward takes h as the forward gave it; nothing is kept between the calls.
 """
 from __future__ import annotations
 

@@ -475,7 +475,8 @@ int hffn_embedding_gradient(int value_type, const void* g, uint64_t g_stride, co
  * sequence of all n rows): with z = sigmoid(gate + bias), h_t = (1 - z_t) h_t-1 + v_t from h_-1 = state[s] (NULL: zeros), where v is
  * z x (tied), sqrt(1 - (1 - z)^2) x (normed) or x (free). x, gate: rows of d_model entries of the value type, strides in entries;
  * h [n, d_model] of that type, zero in rows outside every sequence; bias float32[d_model] (NULL: zeros); state and last (h after
- * each sequence, state itself where it has no rows) float32[sequences, d_model]. States are float32. Bounds that do not ascend,
+ * each sequence, state itself where it has no rows) float32[sequences, d_model]. States are float32. An infinity stays one to
+ * its sequence's end, until a NaN or its opposite comes in; so does what leaves float32, for which h + v may be enough. Bounds that do not ascend,
  * or leave [0, n], give values that mean nothing, but no access outside the arrays. Outputs may not overlap inputs.
  * Workspace: hffn_scan_workspace bytes (gradients: for the backward), 16-byte aligned, any content. */
 #define HFFN_SCAN_TIED 0
