@@ -20,6 +20,7 @@ infinity in a float32 row makes what it enters NaN.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .runtime import MAX_TOKENS, StreamUses, _device, _value_type, current_stream
@@ -30,6 +31,14 @@ MAX_WIDTH, MAX_VOCAB = 1 << 15, 1 << 24
 _LABEL_BYTES = {torch.int32: 4, torch.int64: 8}
 
 
+def refuse_recording(t: torch.Tensor, name: str) -> None:
+    """Raises ``ValueError`` where autograd, in either mode, would expect a call that reads ``t`` to be recorded."""
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires gradients, and autograd does not record this call: pass it detached, or under torch.no_grad()")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{name} carries a forward-mode tangent, and this call would drop it: pass its primal")
+
+
 def rows_of(t: torch.Tensor, name: str, width: int, dtype: torch.dtype) -> tuple[torch.Tensor, int]:
     """``t`` as rows of ``width`` entries the kernels read, and their stride: itself where a row's entries are adjacent and rows
     do not overlap, else a contiguous copy. Raises ``ValueError`` for another shape, type or device, and where autograd would
@@ -38,8 +47,7 @@ def rows_of(t: torch.Tensor, name: str, width: int, dtype: torch.dtype) -> tuple
         raise ValueError(f"{name}: a {dtype} [N, {width}] tensor on cuda:0 is required, not {t.dtype} {list(t.shape)} on {t.device}")
     if t.shape[0] > MAX_TOKENS:
         raise ValueError(f"{name}: N={t.shape[0]} above {MAX_TOKENS}")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{name} requires gradients, and autograd does not record this call: pass it detached, or under torch.no_grad()")
+    refuse_recording(t, name)
     if t.is_contiguous():
         return t, width
     if t.stride(1) == 1 and t.stride(0) >= width:

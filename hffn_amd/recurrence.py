@@ -23,7 +23,7 @@ import functools
 import torch
 
 from . import _lib
-from .loss import MAX_WIDTH, rows_of
+from .loss import MAX_WIDTH, refuse_recording, rows_of
 from .runtime import StreamUses, _device, _value_type, current_stream
 
 KINDS = ("tied", "normed", "free")
@@ -87,8 +87,7 @@ class GatedRecurrence:
             raise ValueError(f"{name}: a float32 [S, {self.d_model}] tensor on cuda:0 is required, not {t.dtype} {list(t.shape)} on {t.device}")
         if t.shape[0] != sequences:
             raise ValueError(f"{name}: {t.shape[0]} rows for {sequences} sequences")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise ValueError(f"{name} requires gradients, and autograd does not record this call: pass it detached, or under torch.no_grad()")
+        refuse_recording(t, name)
         return t.contiguous()
 
     def forward(self, x: torch.Tensor, gate: torch.Tensor, bounds: torch.Tensor | None = None,
@@ -154,8 +153,7 @@ class GatedRecurrence:
                 d > 1 and state.stride(1) != 1 or n > 1 and state.stride(0) < d):
             raise ValueError(f"state: a float32 {[n, d]} tensor on cuda:0 of rows with adjacent entries that do not overlap is required, not {state.dtype} "
                              f"{list(state.shape)} of strides {list(state.stride())} on {state.device}")
-        if state.requires_grad and torch.is_grad_enabled():
-            raise ValueError("state requires gradients, and autograd does not record this call: pass it detached, or under torch.no_grad()")
+        refuse_recording(state, "state")
         h = x.new_empty(n, d)
         if n:
             _lib.check(self._lib.hffn_scan_step(value_type, self._kind, x.data_ptr(), x_stride, gate.data_ptr(), gate_stride, self.bias.data_ptr(),
