@@ -1,7 +1,7 @@
 // Embedding lookup with scaling, and the gradient of the table:
 //   out_n = scale weight[id_n],   gw_v = scale sum over the n with id_n = v, in their order, of g_n
-// The gradient orders the positions by their tokens (equal ones by position, so that a row's terms come in one order whatever
-// runs first), then adds every run of equal tokens: no atomics on floats, the same bits at every call.
+// The gradient of more than a few positions orders them by their tokens (equal ones by position, so that a row's terms come in one order
+// whatever runs first), then adds every run of equal tokens: no atomics on floats, the same bits at every call.
 //
 // Bound by the writes: a whole gradient of 50304 rows is one fill of the card's memory (206 MB of 2048 bfloat16 columns: 31 us by 16
 // bytes a thread, 6.7 TB/s; stores that pass the caches by are faster where nobody reads the gradient next, 59 -> 53 us for 8192 tokens, and slower with who

@@ -7,10 +7,12 @@
 // its own, and walks its rows again from there. Rows are read once and written once, by one launch.
 //
 // Forward 3 N d entries moved, backward 6 N d (a large copy: 5.2 TB/s). Measured, us a call of the kernels' own time: forward 8 x 2048
-// tokens of 1024 channels, tied bfloat16, 37 (101 MB: 2.7 TB/s), 32768 tokens of 512 channels, normed float32, 52 (201 MB: 3.9); backward of
-// the former 55 (201 MB: 3.7). What bounds it: the chain of a block, for one resident round of 512 blocks whose loads and stores do not
-// overlap another's (a tile's stamps, bfloat16 forward: ticket 2 us, requests and bounds 4.5, gates and the first walk 4, the fold of the
-// waves 1.3, the tiles before 2, the groups 1, the last walk 1.4), and some 40 vector instructions an entry, a third to half of the time.
+// tokens of 1024 channels, tied bfloat16, 36 (101 MB: 2.8 TB/s), 32768 tokens of 512 channels, normed float32, 54 (201 MB: 3.7); backward of
+// the former 53 (201 MB: 3.8). What bounds it is neither the memory nor the instructions alone: of the 36 us the bytes are 19.5 and the vector
+// instructions, 43 an entry, 18 on every SIMD (float32 56, 24 of the 54; backward 58, 25 of the 53). 1024 blocks are two rounds of the 512 that
+// the card holds; a CU has 29 of its 32 waves while it has any block, 30 of the 36 us, and a wave waits 64 % of its cycles (58 and 57): a
+// block's chain (a tile's stamps, bfloat16 forward: ticket 2 us, requests and bounds 4.5, gates and the first walk 4, the fold of the
+// waves 1.3, the tiles before 2, the groups 1, the last walk 1.4) passes beside that of one other block.
 // Blocks that stay, with waves of their own for the folds and the next tile's rows requested ahead, took 62 us where this takes 40:
 // the folds are the longest chain, and had fewer waves to hide in.
 #include <algorithm>

@@ -39,7 +39,8 @@ def _workspace(n: int, d_model: int, gradients: bool) -> int:
 class GatedRecurrence:
     """One recurrence (see the module docstring). The bias is a float32 [d] tensor, held as given and read at every call; x, gate, h
     and their gradients are float32 or bfloat16 [N, d] rows, all of one type, those that come in with any row stride, those
-    returned new and contiguous; sums are taken in float32. Rows outside every sequence are read by none, and zero in h and in the
+    returned new and contiguous; sums are taken in float32, in an order that goes by the rows' places in the batch (the last bits of a sequence
+    depend on where it begins there, not on the other sequences). Rows outside every sequence are read by none, and zero in h and in the
     gradients. Calls are queued on PyTorch's current stream; calls of ``backward``
     of one object on several streams have to be ordered by the caller. Autograd records none of them: gradients are those of ``backward``
     and ``gradients()``, and rows that require gradients are refused."""
