@@ -205,7 +205,7 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const uint32_t* __
 // of 64 from its head on, each the whole block's whose positions it begins in (16 waves with 4 rows each, added in order); the
 // block that ends a run's last piece adds them up, in order too. The rows' order and these cuts depend on the run alone. Behind the
 // blocks that add come those that fill the other rows with zeros: what the long runs wait for passes beside that. (All rows
-// filled beside the order instead: 60 us for 51 with 8192 positions, 42 for 40 with 4096, 29 for 34 with 64.)
+// filled beside the order instead: 60 us for 51 with 8192 positions, 42 for 40 with 4096.)
 constexpr uint32_t kSumThreads = 1024, kSumWaves = kSumThreads / kWave, kRun = 64, kShare = kRun / kSumWaves;
 constexpr uint32_t kWindow = 4;
 static_assert(kWindow * kSumWaves <= kRun, "at most one long run begins in a block, and at most one piece of an earlier one");
